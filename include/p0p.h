@@ -45,7 +45,9 @@ enum {                                                                       /* 
 /* which kernel family served the last p0p_gemm call (p0p_last_kernel) or is forced (p0p_gemm_args.force_kernel) */
 enum { P0P_K_AUTO = 0, P0P_K_GENERIC = 1, P0P_K_DECODE = 2, P0P_K_UMMA = 3,
        /* p0p_attention: the split-key kernel / the tensor-memory kernel (p0p_attn_args.kernel forces one of them) */
-       P0P_K_ATTN_WARP = 16, P0P_K_ATTN_TMEM = 17 };
+       P0P_K_ATTN_WARP = 16, P0P_K_ATTN_TMEM = 17,
+       /* p0p_cache_attention: the split-key kernel / the tensor-memory kernel / both, each for some of the sequences */
+       P0P_K_CACHE_SPLIT = 24, P0P_K_CACHE_TMEM = 25, P0P_K_CACHE_BOTH = 26 };
 
 enum { P0P_OPT_USE_STREAM = 1 };
 
@@ -217,6 +219,70 @@ typedef struct p0p_attn_args {
                                             built before this field existed passes a smaller struct_size and gets 0. */
 } p0p_attn_args;
 int p0p_attention(p0p_ctx* ctx, const p0p_attn_args* args, double* flops);
+
+/* ---- the 8-bit key/value cache and what works on it (no counterpart in the reference, which recomputes or holds fp16 K / V) ----------
+ * A cache of one layer: pages of 64 tokens, found through a table per sequence.
+ *   codes  [pages][Hkv][2 (K, V)][64 * 128] u8: code + 128          scales [pages][Hkv][2] fp32
+ *   tail   [seqs][Hkv][2][64 * 128] fp16: the tokens of each sequence's last, unfinished page, unquantised
+ *   table  [seqs][max_pages] u32: the page that holds tokens 64 i .. 64 i + 63        lens [seqs] u32: tokens of each sequence
+ * A block of 64 tokens of one head is quantised once, when its last token arrives: scale = (largest magnitude) / 127 rounded up to 12
+ * significant bits (1 for a block of zeros), code = x / scale rounded to the nearest, ties to even.  So what the cache holds does not depend on
+ * how the tokens were cut into calls.  NaN is stored as 0, an infinity as the largest fp16 of its sign.  Within a block the elements lie as
+ * csrc/cache_plan.h says (cache_k_off, cache_v_off), the same for codes and tail.  K and V pages may be shared between sequences
+ * (a common prefix) as long as only one of them writes.
+ * `lens`, `table` and `rows` are read on the device when the call runs: a recorded sequence of calls can be replayed with new
+ * contents.  `lens` counts the tokens of the present call too: a sequence's n new tokens are its last n, at positions
+ * lens - n .. lens - 1.  The new tokens of all sequences are consecutive rows of the call's tensors; sequence b has rows rows[b] ..
+ * rows[b + 1] - 1 (u32 [seqs + 1]), or, without row offsets, M / seqs rows each.  A sequence may have none.  Rows behind the
+ * last sequence's are neither read nor written.
+ * A sequence whose numbers make no sense (row offsets that fall or exceed M; fewer tokens than rows; more than 64 * max_pages) is
+ * left out, a page number outside the cache is not followed; either makes the next p0p_sync / p0p_read return -10. */
+typedef struct p0p_cache {
+  uint32_t Hkv, pages, seqs, max_pages;                                  /* at most 1024 sequences */
+  p0p_buf *codes, *scales, *tail, *table, *lens;
+  uint64_t codes_off, scales_off, tail_off, table_off, lens_off;         /* bytes */
+} p0p_cache;
+typedef struct p0p_cache_args {
+  uint32_t struct_size;
+  uint32_t M, ldk, ldv;                  /* rows of the call; rows per head of k and v (0 = M) */
+  p0p_cache cache;
+  p0p_buf *k, *v, *rows;                 /* [Hkv][ld][128] f16 each; rows may be NULL */
+  uint64_t k_off, v_off, rows_off;       /* bytes */
+} p0p_cache_args;
+/* stores the call's keys and values: finished blocks as codes, the rest in the tail.  (Writing the same tokens again, or fewer of them, works
+ * as long as no page was finished in between: a finished page's tokens have left the tail.) */
+int p0p_cache_write(p0p_ctx* ctx, const p0p_cache_args* args);
+/* the inverse: writes each sequence's last n tokens, as the cache holds them, to k and v as f16 */
+int p0p_cache_read(p0p_ctx* ctx, const p0p_cache_args* args);
+
+typedef struct p0p_cache_attn_args {
+  uint32_t struct_size;
+  uint32_t Hq, M, ldq, ldo;              /* q [Hq][ldq][128] f16 (0 = M); o [M][ldo] f16 token-major at column h * 128 (0 = Hq * 128) */
+  uint32_t max_new;                      /* no sequence has more new tokens than this (0 = M; M / seqs without row offsets) */
+  uint32_t window, sinks;                /* a query sees the last `window` keys, itself included, and the first `sinks` (window 0: all) */
+  float scale;                           /* 0 = 1 / sqrt(128) */
+  uint32_t kernel;                       /* 0 = the library chooses; P0P_K_CACHE_SPLIT / P0P_K_CACHE_TMEM force one (tests) */
+  p0p_cache cache;
+  p0p_buf *q, *o, *rows;
+  uint64_t q_off, o_off, rows_off;
+} p0p_cache_attn_args;
+/* causal attention of the call's queries over the cache, which holds their own keys and values already (p0p_cache_write comes first).
+ * Query head h reads kv head h / (Hq / Hkv).  Partial results are kept in the context's scratch memory. */
+int p0p_cache_attention(p0p_ctx* ctx, const p0p_cache_attn_args* args);
+
+/* rotary positions: y = x with the first `rot` elements of every head turned by its token's position (y may be x).  x, y [H][ld][128] f16; positions
+ * and rows as for a cache.  mode 0 interleaved: pairs (2i, 2i + 1); 1 half: pairs (i, i + rot / 2).  Pair i turns by position * f_i,
+ * f_i = theta^(-2i / rot); with factor != 1: f_i / factor where original == 0, else f_i (g + (1 - g) / factor) with
+ * g = clamp((original f_i / 2 pi - slow) / (fast - slow), 0, 1): frequencies that turn at least `fast` times within the original context stay,
+ * those below `slow` times are divided.  The turned elements are multiplied by mscale.  Angles are reduced in 64 bits. */
+typedef struct p0p_rope_args {
+  uint32_t struct_size;
+  uint32_t H, M, ldx, ldy, seqs, mode, rot;                              /* ld 0 = M; rot even, at most 128 */
+  double theta, factor, original, fast, slow, mscale;                    /* 0 = 10000, 1, -, 32, 1, 1 */
+  p0p_buf *x, *y, *lens, *rows;                                          /* y NULL = x; rows may be NULL */
+  uint64_t x_off, y_off, lens_off, rows_off;
+} p0p_rope_args;
+int p0p_rope(p0p_ctx* ctx, const p0p_rope_args* args);
 
 /* Debug op: writes the fp16 tile values the kernels feed to the multiply, rows [r0, r0+nr) x all w_cols
  * columns, row-major into `out` (fp16).  path 0 = the fp32-FMA conversion, 1 = the packed half2 conversion

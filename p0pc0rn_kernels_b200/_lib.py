@@ -17,7 +17,7 @@ SYMBOLS = [
     "p0p_capture_begin", "p0p_capture_end", "p0p_graph_launch", "p0p_graph_free",
     "p0p_decode_q4_static", "p0p_decode_q4_static_status", "p0p_alloc_shareable", "p0p_ipc_export", "p0p_ipc_open", "p0p_peer_barrier",
     "p0p_gemm", "p0p_attention", "p0p_last_kernel", "p0p_launch_count", "p0p_last_plan", "p0p_dequant", "p0p_rowstats",
-    "p0p_pixstats", "p0p_gn_partial", "p0p_gn_finalize",
+    "p0p_pixstats", "p0p_gn_partial", "p0p_gn_finalize", "p0p_cache_write", "p0p_cache_read", "p0p_cache_attention", "p0p_rope",
     "p0p_f2h", "p0p_h2f", "p0p_to_f16", "p0p_from_f16", "p0p_pack_q4", "p0p_pack_q8", "p0p_reorder_conv_rows",
     "p0p_encoded_bytes", "p0p_shard_rows", "p0p_abi_version",
 ]
@@ -27,7 +27,8 @@ XMODE = {"f16": 0, "lnmod": 1, "rms": 2, "conv": 3, "conv3": 4}
 EPI = {"f16": 0, "f32": 1, "resadd": 2, "swiglu": 3, "heads": 4, "bias": 5, "onormgate": 6}
 F_GATE, F_RES, F_STORE, F_GN, F_UP2, F_PN, F_BIAS, F_GELU, F_ROPE_HALF = 1, 2, 4, 8, 16, 32, 64, 128, 256
 K_AUTO, K_GENERIC, K_DECODE, K_UMMA = 0, 1, 2, 3
-KERNEL_NAMES = {0: "auto", 1: "generic", 2: "decode", 3: "umma", 16: "attention (split keys)", 17: "attention (tcgen05)"}
+KERNEL_NAMES = {0: "auto", 1: "generic", 2: "decode", 3: "umma", 16: "attention (split keys)", 17: "attention (tcgen05)", 24: "cache attention (split keys)",
+                25: "cache attention (tcgen05)", 26: "cache attention (both)"}
 
 
 class Opts(C.Structure):
@@ -48,6 +49,26 @@ class GemmArgs(C.Structure):
 class AttnArgs(C.Structure):
     _fields_ = ([(n, C.c_uint32) for n in ("struct_size", "Hq", "Hkv", "Lq", "Lk", "ldo", "mode", "nvalid")] + [("scale", C.c_float)]
                 + [(n, C.c_void_p) for n in ("q", "k", "v", "o")] + [(n, C.c_uint64) for n in ("q_off", "k_off", "v_off", "o_off")] + [("kernel", C.c_uint32)])
+
+
+class Cache(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("Hkv", "pages", "seqs", "max_pages")] + [(n, C.c_void_p) for n in ("codes", "scales", "tail", "table", "lens")]
+                + [(n, C.c_uint64) for n in ("codes_off", "scales_off", "tail_off", "table_off", "lens_off")])
+
+
+class CacheArgs(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("struct_size", "M", "ldk", "ldv")] + [("cache", Cache)] + [(n, C.c_void_p) for n in ("k", "v", "rows")]
+                + [(n, C.c_uint64) for n in ("k_off", "v_off", "rows_off")])
+
+
+class CacheAttnArgs(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("struct_size", "Hq", "M", "ldq", "ldo", "max_new", "window", "sinks")] + [("scale", C.c_float), ("kernel", C.c_uint32), ("cache", Cache)]
+                + [(n, C.c_void_p) for n in ("q", "o", "rows")] + [(n, C.c_uint64) for n in ("q_off", "o_off", "rows_off")])
+
+
+class RopeArgs(C.Structure):
+    _fields_ = ([(n, C.c_uint32) for n in ("struct_size", "H", "M", "ldx", "ldy", "seqs", "mode", "rot")] + [(n, C.c_double) for n in ("theta", "factor", "original", "fast", "slow", "mscale")]
+                + [(n, C.c_void_p) for n in ("x", "y", "lens", "rows")] + [(n, C.c_uint64) for n in ("x_off", "y_off", "lens_off", "rows_off")])
 
 
 def _load():
@@ -72,6 +93,8 @@ def _load():
         "p0p_gn_finalize": (i, [vp, vp, u32, u32, C.c_float, vp, u32, u32, vp, u32]),
         "p0p_alloc_shareable": (i, [vp, u64, C.POINTER(vp)]), "p0p_ipc_export": (i, [vp, vp, vp]), "p0p_ipc_open": (i, [vp, vp, u64, C.POINTER(vp)]),
         "p0p_gemm": (i, [vp, C.POINTER(GemmArgs), C.POINTER(C.c_double)]), "p0p_attention": (i, [vp, C.POINTER(AttnArgs), C.POINTER(C.c_double)]), "p0p_last_kernel": (i, [vp]), "p0p_launch_count": (u64, [vp]), "p0p_last_plan": (i, [vp, C.POINTER(C.c_uint32)]),
+        "p0p_cache_write": (i, [vp, C.POINTER(CacheArgs)]), "p0p_cache_read": (i, [vp, C.POINTER(CacheArgs)]),
+        "p0p_cache_attention": (i, [vp, C.POINTER(CacheAttnArgs)]), "p0p_rope": (i, [vp, C.POINTER(RopeArgs)]),
         "p0p_dequant": (i, [vp, u32, vp, u64, u32, u32, u32, u32, u32, vp, u64]),
         "p0p_rowstats": (i, [vp, vp, u64, u32, u32, u32, u32, u32, C.c_float, vp, u32]),
         "p0p_f2h": (C.c_uint16, [C.c_float]), "p0p_h2f": (C.c_float, [C.c_uint16]),

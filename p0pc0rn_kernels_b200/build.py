@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libp0p.so")
-SOURCES = ["runtime.cu", "gemm.cu", "decode.cu", "umma_q4.cu", "umma_q8.cu", "umma_f16.cu", "decode_finish.cu", "attn.cu", "stats.cu", "peer.cu", "noalloc.cu", "host_codec.cpp"]
+SOURCES = ["runtime.cu", "gemm.cu", "decode.cu", "umma_q4.cu", "umma_q8.cu", "umma_f16.cu", "decode_finish.cu", "attn.cu", "cache.cu", "cache_attn.cu", "stats.cu", "peer.cu", "noalloc.cu", "host_codec.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC,-fvisibility=default,-ffp-contract=off", "-Xptxas", "-v"]
 

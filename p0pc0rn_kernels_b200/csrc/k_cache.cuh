@@ -1,0 +1,364 @@
+// Writing and reading the 8-bit key/value cache (cache_plan.h says what lies where), and rotary positions.
+#pragma once
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "cache_dev.cuh"
+#include "sync.cuh"
+
+namespace p0p {
+
+// Block x of a call's touched pages: the sequence and which of its touched pages it is.  False: there are fewer.  All 256 threads.
+__device__ __forceinline__ bool cache_find_page(const CacheP& p, uint32_t x, uint32_t per_seq, uint32_t& b, uint32_t& local) {
+  if (!p.rows) {                                                         // equal counts: as many blocks for every sequence
+    b = x / per_seq; local = x - b * per_seq;
+    return true;
+  }
+  __shared__ uint32_t warp_sum[8], found[2];
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  if (tid == 0u) found[0] = 0xffffffffu;
+  uint64_t base = 0u;
+  for (uint32_t b0 = 0; b0 < p.seqs; b0 += 256u) {
+    const uint32_t c = b0 + tid < p.seqs ? cache_touched(cache_seq(p, b0 + tid)) : 0u;
+    uint32_t inc = c;
+#pragma unroll
+    for (uint32_t o = 1; o < 32u; o <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += v; }
+    if (lane == 31u) warp_sum[warp] = inc;
+    __syncthreads();
+    uint32_t before = 0u, all = 0u;
+#pragma unroll
+    for (uint32_t w = 0; w < 8u; w++) { if (w < warp) before += warp_sum[w]; all += warp_sum[w]; }
+    const uint64_t first = base + before + inc - c;
+    if (c && x >= first && x < first + c) { found[0] = b0 + tid; found[1] = (uint32_t)(x - first); }
+    base += all;
+    __syncthreads();
+    if (found[0] != 0xffffffffu || x < base) break;
+  }
+  b = found[0]; local = found[1];
+  return b != 0xffffffffu;
+}
+
+// NaN -> 0, infinities -> the largest finite value
+__device__ __forceinline__ uint32_t cache_clean(uint32_t v) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&v);
+  uint32_t w = v & __heq2_mask(h, h);
+  const __half2 most = __halves2half2(__ushort_as_half(0x7bff), __ushort_as_half(0x7bff));
+  const __half2 c = __hmax2(__hmin2(*reinterpret_cast<const __half2*>(&w), most), __hneg2(most));
+  return *reinterpret_cast<const uint32_t*>(&c);
+}
+
+constexpr uint32_t CW_LD = 132u;        // halves per row of the staging tile: 16 rows apart is another bank
+constexpr uint32_t CW_SMEM = 2u * CACHE_PAGE * CW_LD * 2u;
+
+// New tokens t0 .. t1 - 1 of the unfinished page `pg` (positions) into the tail.  All 256 threads.
+__device__ __forceinline__ void cache_append(__half* tk, __half* tv, const __half* K, const __half* V, uint32_t row_of_pos0, uint32_t pg, uint32_t t0, uint32_t t1) {
+  for (uint32_t e = threadIdx.x; e < (t1 - t0) * 16u; e += 256u) {
+    const uint32_t pos = t0 + (e >> 4), key = pos - pg * CACHE_PAGE, d = (e & 15u) * 8u;
+    const size_t src = (size_t)(row_of_pos0 + pos) * 128u + d;
+    uint4 a = ld_now(reinterpret_cast<const uint4*>(K + src)), b = ld_now(reinterpret_cast<const uint4*>(V + src));
+    a.x = cache_clean(a.x); a.y = cache_clean(a.y); a.z = cache_clean(a.z); a.w = cache_clean(a.w);
+    *reinterpret_cast<uint4*>(tk + cache_k_off(key, d)) = a;
+    const uint32_t w[4] = {cache_clean(b.x), cache_clean(b.y), cache_clean(b.z), cache_clean(b.w)};
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) tv[cache_v_off(key, d + i)] = __ushort_as_half((unsigned short)(w[i >> 1] >> (16u * (i & 1u))));
+  }
+}
+
+// code + 128 of x in the low byte: x * inv + 768 snaps the quotient to multiples of 2^-14, then the second sum rounds it to the
+// nearest whole number, ties to even.  x has 11 significant bits and the scale 12, so that x / scale is either exactly half way between
+// two codes or at least 2^-13 away from it, while x * inv is off by 2^-17 at most: the snap restores a tie and moves nothing across one.
+__device__ __forceinline__ uint32_t cache_code(float x, float inv) { return __float_as_uint(fmaf(x, inv, 768.0f) + (12582912.0f + 128.0f - 768.0f)); }
+__device__ __forceinline__ uint32_t cache_pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+__device__ __forceinline__ float cache_scale(float amax) {
+  return amax > 0.0f ? __uint_as_float((__float_as_uint(__fdiv_rn(amax, 127.0f)) + 4095u) & ~4095u) : 1.0f;
+}
+
+// One block = one touched page of one kv head; 128 threads for K, 128 for V.  A page that the call finishes is gathered (old tokens
+// from the tail, new ones from the rows) in shared memory with its largest magnitude found on the way, then leaves as codes in the cache's
+// order: 16 codes per thread and store.  The unfinished last page only takes its new tokens into the tail; where the call also
+// finishes a page that began in the tail, that page's block does it, after it has read the tail.
+// Bound: HBM for prompts (256 bytes read and 128 written per token, head and K or V), launch latency for steps.
+__global__ void __launch_bounds__(256) k_cache_write(const CacheP p, const __half* K, const __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
+  extern __shared__ __align__(16) unsigned char cw_smem[];
+  __shared__ float sm_max[8];
+  const uint32_t tid = threadIdx.x, hk = blockIdx.y;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  uint32_t b, local;
+  if (!cache_find_page(p, blockIdx.x, per_seq, b, local)) return;
+  const CacheSeq s = cache_seq(p, b);
+  if (local >= cache_touched(s)) return;
+  const uint32_t first = cache_first_page(s), old = s.L - s.n, pg = first + local, last = s.L / CACHE_PAGE;
+  const uint32_t row0 = s.r0 - old;                                       // (wraps: only sums with positions >= old are rows)
+  __half* tk = p.tail + ((size_t)b * p.Hkv + hk) * 2u * CACHE_BLOCK; __half* tv = tk + CACHE_BLOCK;
+  const __half* Kh = K + (size_t)hk * ldk * 128u; const __half* Vh = V + (size_t)hk * ldv * 128u;
+  const bool began = (old & (CACHE_PAGE - 1u)) != 0u;                     // page `first` has tokens in the tail
+  if (pg == last) {                                                       // unfinished
+    if (pg == first || !began) cache_append(tk, tv, Kh, Vh, row0, pg, max(old, pg * CACHE_PAGE), s.L);
+    return;
+  }
+  const uint32_t w = tid >> 7, i = tid & 127u;
+  __half* tile = reinterpret_cast<__half*>(cw_smem) + w * CACHE_PAGE * CW_LD;
+  const __half* src = w ? Vh : Kh; const __half* tl = w ? tv : tk;
+  uint4 x[8];
+#pragma unroll
+  for (uint32_t it = 0; it < 8u; it++) {
+    const uint32_t key = it * 8u + (i >> 4), d = (i & 15u) * 8u, pos = pg * CACHE_PAGE + key;
+    if (pos >= old) {
+      x[it] = ld_now(reinterpret_cast<const uint4*>(src + (size_t)(row0 + pos) * 128u + d));
+      x[it].x = cache_clean(x[it].x); x[it].y = cache_clean(x[it].y); x[it].z = cache_clean(x[it].z); x[it].w = cache_clean(x[it].w);
+    } else if (w == 0u) x[it] = ld_now(reinterpret_cast<const uint4*>(tl + cache_k_off(key, d)));
+    else {
+      uint32_t v[8];
+#pragma unroll
+      for (uint32_t j = 0; j < 8u; j++) v[j] = __half_as_ushort(ld_now(tl + cache_v_off(key, d + j)));
+      x[it] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+    }
+  }
+  __half2 mx = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+#pragma unroll
+  for (uint32_t it = 0; it < 8u; it++) {
+    const uint32_t key = it * 8u + (i >> 4), d = (i & 15u) * 8u;
+    const __half2* h = reinterpret_cast<const __half2*>(&x[it]);
+#pragma unroll
+    for (int j = 0; j < 4; j++) mx = __hmax2(mx, __habs2(h[j]));
+    uint2* dst = reinterpret_cast<uint2*>(tile + key * CW_LD + d);
+    dst[0] = make_uint2(x[it].x, x[it].y); dst[1] = make_uint2(x[it].z, x[it].w);
+  }
+  float m = fmaxf(__low2float(mx), __high2float(mx));
+#pragma unroll
+  for (uint32_t o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((tid & 31u) == 0u) sm_max[tid >> 5] = m;
+  __syncthreads();                                                        // (every read of the tail has ended, too)
+  const float sc = cache_scale(fmaxf(fmaxf(sm_max[w * 4u], sm_max[w * 4u + 1u]), fmaxf(sm_max[w * 4u + 2u], sm_max[w * 4u + 3u]))), inv = __fdiv_rn(1.0f, sc);
+  const uint32_t page = ld_now(p.table + (size_t)b * p.max_pages + pg);
+  if (page >= p.pages) { if (tid == 0u) cache_tell(p.status, CACHE_BAD_PAGE); }
+  else {
+    uint4* out = reinterpret_cast<uint4*>(p.codes + (((size_t)page * p.Hkv + hk) * 2u + w) * CACHE_BLOCK);
+    if (w == 0u) {
+#pragma unroll
+      for (uint32_t it = 0; it < 4u; it++) {                              // unit u = 16 consecutive d of one key
+        const uint32_t u = it * 128u + i, key = (u >> 7) * 16u + ((u >> 3) & 3u) * 4u + ((u >> 6) & 1u) * 2u + ((u >> 2) & 1u), d = ((u >> 5) & 1u) * 64u + (u & 3u) * 16u;
+        const uint2* r = reinterpret_cast<const uint2*>(tile + key * CW_LD + d);
+        uint32_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint2 v = r[j];
+          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+          q[j] = cache_pack4(cache_code(f0.x, inv), cache_code(f0.y, inv), cache_code(f1.x, inv), cache_code(f1.y, inv));
+        }
+        out[u] = make_uint4(q[0], q[1], q[2], q[3]);
+      }
+    } else {
+#pragma unroll
+      for (uint32_t it = 0; it < 2u; it++) {                              // two units: keys 16 j + 4 t + e of d and of d + 1
+        const uint32_t u = it * 128u + i, d = (u >> 2) * 2u, t = u & 3u;
+        uint32_t q0[4], q1[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; j++) {
+          uint32_t c0[4], c1[4];
+#pragma unroll
+          for (uint32_t e = 0; e < 4u; e++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(tile + (16u * j + 4u * t + e) * CW_LD + d));
+            c0[e] = cache_code(f.x, inv); c1[e] = cache_code(f.y, inv);
+          }
+          q0[j] = cache_pack4(c0[0], c0[1], c0[2], c0[3]); q1[j] = cache_pack4(c1[0], c1[1], c1[2], c1[3]);
+        }
+        out[d * 4u + t] = make_uint4(q0[0], q0[1], q0[2], q0[3]); out[(d + 1u) * 4u + t] = make_uint4(q1[0], q1[1], q1[2], q1[3]);
+      }
+    }
+    if (i == 0u) reinterpret_cast<float*>(p.scales + (size_t)page * p.Hkv + hk)[w] = sc;
+  }
+  // (new tokens behind the last finished page: positions last * 64 >= old, since page `first` is finished)
+  if (pg == first && began) cache_append(tk, tv, Kh, Vh, row0, last, last * CACHE_PAGE, s.L);
+}
+
+// ---- read back: one block = one touched page of one kv head, as in k_cache_write; values go through shared memory to whole rows
+__global__ void __launch_bounds__(256) k_cache_read(const CacheP p, __half* K, __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
+  extern __shared__ __align__(16) unsigned char cw_smem[];
+  const uint32_t tid = threadIdx.x, hk = blockIdx.y;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  uint32_t b, local;
+  if (!cache_find_page(p, blockIdx.x, per_seq, b, local)) return;
+  const CacheSeq s = cache_seq(p, b);
+  if (local >= cache_touched(s)) return;
+  const uint32_t old = s.L - s.n, pg = cache_first_page(s) + local, row0 = s.r0 - old;
+  const uint32_t w = tid >> 7, i = tid & 127u;
+  __half* tile = reinterpret_cast<__half*>(cw_smem) + w * CACHE_PAGE * CW_LD;
+  const bool whole = pg < s.L / CACHE_PAGE;
+  uint32_t page = 0u;
+  if (whole) {
+    page = ld_now(p.table + (size_t)b * p.max_pages + pg);
+    if (page >= p.pages) { if (tid == 0u) cache_tell(p.status, CACHE_BAD_PAGE); return; }
+  }
+  const uint4* in = reinterpret_cast<const uint4*>(p.codes + (((size_t)page * p.Hkv + hk) * 2u + w) * CACHE_BLOCK);
+  const __half* tl = p.tail + (((size_t)b * p.Hkv + hk) * 2u + w) * CACHE_BLOCK;
+  const float sc = whole ? ld_now(reinterpret_cast<const float*>(p.scales + (size_t)page * p.Hkv + hk) + w) : 0.0f;
+  uint4 c[4];
+  if (whole) {
+#pragma unroll
+    for (uint32_t it = 0; it < 4u; it++) c[it] = ld_now(in + it * 128u + i);
+  }
+#pragma unroll
+  for (uint32_t it = 0; it < 4u; it++) {
+    const uint32_t u = it * 128u + i;
+    uint32_t h[8];                                                        // 16 values: of one key (K) or of one d (V)
+    if (whole) {
+      const uint32_t q[4] = {c[it].x, c[it].y, c[it].z, c[it].w};
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const uint32_t v = q[j >> 1] >> (16 * (j & 1));
+        // (a code of 127 times a scale that was rounded up may pass the largest fp16: it stays finite)
+        const float lo = fmaxf(fminf((float)((int)(v & 255u) - 128) * sc, 65504.0f), -65504.0f), hi = fmaxf(fminf((float)((int)((v >> 8) & 255u) - 128) * sc, 65504.0f), -65504.0f);
+        const __half2 r = __floats2half2_rn(lo, hi);
+        h[j] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+    } else {
+      const uint4 a = ld_now(reinterpret_cast<const uint4*>(tl) + 2u * u), z = ld_now(reinterpret_cast<const uint4*>(tl) + 2u * u + 1u);
+      h[0] = a.x; h[1] = a.y; h[2] = a.z; h[3] = a.w; h[4] = z.x; h[5] = z.y; h[6] = z.z; h[7] = z.w;
+    }
+    if (w == 0u) {
+      const uint32_t key = (u >> 7) * 16u + ((u >> 3) & 3u) * 4u + ((u >> 6) & 1u) * 2u + ((u >> 2) & 1u), d = ((u >> 5) & 1u) * 64u + (u & 3u) * 16u;
+      uint2* r = reinterpret_cast<uint2*>(tile + key * CW_LD + d);
+#pragma unroll
+      for (int j = 0; j < 4; j++) r[j] = make_uint2(h[2 * j], h[2 * j + 1]);
+    } else {
+      const uint32_t d = u >> 2, t = u & 3u;
+#pragma unroll
+      for (uint32_t j = 0; j < 16u; j++) tile[((j >> 2) * 16u + 4u * t + (j & 3u)) * CW_LD + d] = __ushort_as_half((unsigned short)(h[j >> 1] >> (16u * (j & 1u))));
+    }
+  }
+  __syncthreads();
+  __half* dst = w ? V + (size_t)hk * ldv * 128u : K + (size_t)hk * ldk * 128u;
+#pragma unroll
+  for (uint32_t it = 0; it < 8u; it++) {
+    const uint32_t key = it * 8u + (i >> 4), d = (i & 15u) * 8u, pos = pg * CACHE_PAGE + key;
+    if (pos < old || pos >= s.L) continue;
+    const uint2* r = reinterpret_cast<const uint2*>(tile + key * CW_LD + d);
+    const uint2 a = r[0], z = r[1];
+    *reinterpret_cast<uint4*>(dst + (size_t)(row0 + pos) * 128u + d) = make_uint4(a.x, a.y, z.x, z.y);
+  }
+}
+
+// ---- rotary positions
+struct RopeP {
+  const __half* X; __half* Y;
+  const uint32_t* lens; const uint32_t* rows;
+  uint32_t H, M, ldx, ldy, seqs, each, rot, hpt;      // hpt: heads per thread
+  float mscale;
+  int* status;
+  double turn[64];                                    // turns per position of pair i
+};
+
+// cos and sin of pair i at a position: the angle in turns is reduced in 64 bits (a fp32 angle of position 10^6 is off by 0.03), what is left
+// of it is within half a turn
+__device__ __forceinline__ float2 rope_cs(const RopeP& p, uint32_t i, double pos) {
+  if (2u * i >= p.rot) return make_float2(1.0f, 0.0f);
+  const double t = pos * p.turn[i];
+  float sn, cs;
+  sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
+  return make_float2(cs * p.mscale, sn * p.mscale);
+}
+// the position of row r; false for a row of no sequence
+__device__ __forceinline__ bool rope_pos(const RopeP& p, uint32_t r, double& pos) {
+  uint32_t b, r0, r1;
+  if (!p.rows) { b = r / p.each; r0 = b * p.each; r1 = r0 + p.each; }
+  else {
+    uint32_t lo = 0u, hi = p.seqs;                    // the first sequence whose end is behind r
+    while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (ld_now(p.rows + mid + 1u) > r) hi = mid; else lo = mid + 1u; }
+    if (lo == p.seqs) return false;
+    b = lo; r0 = ld_now(p.rows + b); r1 = ld_now(p.rows + b + 1u);
+    if (r < r0) { if (b > 0u) cache_tell(p.status, CACHE_BAD_ROWS); return false; }
+  }
+  CacheSeq s;
+  const int bad = cache_seq_check(r0, r1, ld_now(p.lens + b), p.M, 0xffffffffu, s);
+  cache_tell(p.status, bad);
+  if (s.n == 0u) return false;
+  pos = (double)(s.L - s.n + (r - r0));
+  return true;
+}
+__device__ __forceinline__ void rope_turn(float2 cs, float& a, float& b) { const float x = a, y = b; a = x * cs.x - y * cs.y; b = fmaf(x, cs.y, y * cs.x); }
+
+// 8 threads per row, 16 elements each as two 16-byte pieces; a thread works out its 8 angles once and turns hpt heads with them.
+// HALF: pieces l and l + rot / 16 of the row's first part pair up (rot a multiple of 16: a pair of pieces holds pairs of one
+// index each); threads whose pieces lie behind the turned part copy.  Otherwise: pieces 2 l and 2 l + 1, pairs within a piece.
+// Bound: HBM for prompts (512 bytes per row and head), launch latency for a step.
+template <bool HALF>
+__global__ void __launch_bounds__(128) k_rope(const RopeP p) {
+  const uint32_t l = threadIdx.x & 7u, r = blockIdx.x * 16u + (threadIdx.x >> 3), h0 = blockIdx.y * p.hpt, h1 = min(h0 + p.hpt, p.H);
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (r >= p.M) return;
+  double pos;
+  if (!rope_pos(p, r, pos)) return;
+  const uint32_t q = p.rot >> 4;                       // HALF: pieces per half of the turned part
+  uint32_t c0, c1, i0;                                 // the thread's two pieces, its first pair
+  if (HALF) {
+    if (l < q) { c0 = l; c1 = l + q; i0 = 8u * l; } else { c0 = 2u * q + 2u * (l - q); c1 = c0 + 1u; i0 = 64u; }
+  } else { c0 = 2u * l; c1 = c0 + 1u; i0 = 8u * l; }
+  float2 cs[8];
+#pragma unroll
+  for (uint32_t i = 0; i < 8u; i++) cs[i] = rope_cs(p, i0 + i, pos);
+  for (uint32_t h = h0; h < h1; h++) {
+    const uint4* x = reinterpret_cast<const uint4*>(p.X + ((size_t)h * p.ldx + r) * 128u);
+    uint4* y = reinterpret_cast<uint4*>(p.Y + ((size_t)h * p.ldy + r) * 128u);
+    uint4 v[2] = {ld_now(x + c0), ld_now(x + c1)};
+    __half2* e = reinterpret_cast<__half2*>(v);
+    if (HALF) {
+      if (i0 < 64u) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float2 a = __half22float2(e[i]), b = __half22float2(e[4 + i]);
+          rope_turn(cs[2 * i], a.x, b.x); rope_turn(cs[2 * i + 1], a.y, b.y);
+          e[i] = __floats2half2_rn(a.x, a.y); e[4 + i] = __floats2half2_rn(b.x, b.y);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        float2 a = __half22float2(e[i]);
+        if (2u * (i0 + i) < p.rot) { rope_turn(cs[i], a.x, a.y); e[i] = __floats2half2_rn(a.x, a.y); }
+      }
+    }
+    y[c0] = v[0]; y[c1] = v[1];
+  }
+}
+// the half layout with a part that is no multiple of 16: a warp per row, one pair (or two elements that are copied) per lane and pass
+__global__ void __launch_bounds__(128) k_rope_odd(const RopeP p) {
+  const uint32_t lane = threadIdx.x & 31u, r = blockIdx.x * 4u + (threadIdx.x >> 5), h0 = blockIdx.y * p.hpt, h1 = min(h0 + p.hpt, p.H);
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (r >= p.M) return;
+  double pos;
+  if (!rope_pos(p, r, pos)) return;
+  const uint32_t half = p.rot >> 1;
+  float2 cs[2]; uint32_t a[2], b[2];
+#pragma unroll
+  for (uint32_t k = 0; k < 2u; k++) {
+    const uint32_t i = k * 32u + lane;
+    cs[k] = rope_cs(p, i, pos);
+    if (i < half) { a[k] = i; b[k] = i + half; } else { a[k] = 2u * i; b[k] = 2u * i + 1u; }      // (element 2 i >= rot: behind the turned part)
+  }
+  for (uint32_t h = h0; h < h1; h++) {
+    const __half* x = p.X + ((size_t)h * p.ldx + r) * 128u;
+    __half* y = p.Y + ((size_t)h * p.ldy + r) * 128u;
+    __half u[2], v[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) { u[k] = ld_now(x + a[k]); v[k] = ld_now(x + b[k]); }
+    __syncwarp();                                      // (y may be x: a row is read before any of it is written)
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      if ((uint32_t)k * 32u + lane < half) {
+        float f = __half2float(u[k]), g = __half2float(v[k]);
+        rope_turn(cs[k], f, g);
+        u[k] = __float2half_rn(f); v[k] = __float2half_rn(g);
+      }
+      y[a[k]] = u[k]; y[b[k]] = v[k];
+    }
+  }
+}
+
+}  // namespace p0p

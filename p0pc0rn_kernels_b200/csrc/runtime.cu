@@ -3,6 +3,7 @@
 // is the in-order queue, so there is no batching layer and no per-dispatch bind group.
 #include <cstring>
 
+#include "cache_plan.h"
 #include "ctx.h"
 
 using namespace p0p;
@@ -41,10 +42,13 @@ int p0p_open(int device, const p0p_opts* opts, p0p_ctx** out) {
   return 0;
 }
 
-// after a stream sync: did a kernel give up on a bounded wait?
+// after a stream sync: did a kernel give up on a bounded wait, or meet numbers of a cache that make no sense?
 static int check_kernel_status(p0p_ctx* c) {
   if (c->host_status && *c->host_status) {
     int code = *c->host_status; *c->host_status = 0;
+    if (code == CACHE_BAD_ROWS) return fail(c, -10, "cache: row offsets that fall, or exceed M; the sequence was left out");
+    if (code == CACHE_BAD_LENS) return fail(c, -10, "cache: a sequence has fewer tokens than rows, or more than its table holds; it was left out");
+    if (code == CACHE_BAD_PAGE) return fail(c, -10, "cache: a page number of the table is outside the cache; results of the queued work are invalid");
     return fail(c, -10, "a kernel gave up on a bounded wait (code %d); results of the queued work are invalid", code);
   }
   return 0;

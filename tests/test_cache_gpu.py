@@ -1,0 +1,533 @@
+"""The 8-bit key/value cache, attention over it and rotary positions, against the definitions in 64 bits.
+
+Tolerances.  Codes, scales and what is read back are exact.  Attention: a weight is rounded to fp16 (half a step, 2^-11, relative; below fp16's
+normal range 2^-25 of the largest weight), its exponential is off by less than 1e-4, the result is rounded to fp16 (2^-11).  Weights that are
+off by d each move the weighted mean by at most d * 2 max|v|, so |error| <= max|v| * (2 * (2^-11 + 1e-4) + 2^-11 + keys * 2^-25).  Rotary
+positions: one rounding to fp16 (2^-11 of the result, 2^-25 where it is subnormal) and four in fp32 (2^-24 of |a| + |b| each)."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+PAGE = 64
+
+
+def _clean(x):
+    x = np.where(np.isnan(x), np.float16(0), x)
+    return np.clip(x, np.float16(-65504), np.float16(65504)).astype(np.float16)
+
+
+def _quantise(x):
+    """64 x 128 values -> (codes, scale), from the definition in 64 bits"""
+    x = x.astype(np.float64); a = np.abs(x).max()
+    if a == 0: return np.zeros_like(x), 1.0
+    m, e = np.frexp(a / 127.0)
+    s = float(np.ldexp(np.ceil(m * 4096.0), e - 12))
+    return np.rint(x / s), s
+
+
+def _offsets():
+    key, d = np.arange(PAGE)[:, None], np.arange(128)[None]
+    k = ((key >> 4) * 2 + ((key >> 1) & 1)) * 1024 + (d >> 6) * 512 + (((key & 15) >> 2) * 2 + (key & 1)) * 64 + (d & 63)
+    v = d * 64 + ((key >> 2) & 3) * 16 + (key >> 4) * 4 + (key & 3)
+    return k, v
+
+
+class Cache:
+    """a cache on the GPU and what it should hold"""
+
+    def __init__(self, P, gpu, Hkv, seqs, maxPages, spare=3, seed=0, pages=None, first_page=0):
+        self.P, self.gpu, self.Hkv, self.seqs, self.maxp = P, gpu, Hkv, seqs, maxPages
+        rng = np.random.default_rng(seed)
+        self.pages = pages or seqs * maxPages + spare
+        self.table = (first_page + rng.permutation(self.pages - first_page)[:seqs * maxPages]).reshape(seqs, maxPages).astype(np.uint32)
+        self.d = P.kvCache(gpu, {"Hkv": Hkv, "pages": self.pages, "seqs": seqs, "maxPages": maxPages})
+        self.poison()
+        gpu.upload(self.table, dst=self.d["table"]["buf"])
+        self.lens = np.zeros(seqs, np.uint32)
+        self.tok = [(np.zeros((Hkv, 0, 128), np.float16),) * 2 for _ in range(seqs)]      # every token, as written
+
+    def poison(self):
+        """what nobody has written yet: codes of any kind with a scale that is no number, a tail of NaN"""
+        n = self.P.cacheBytes(self.pages, self.Hkv, self.seqs, self.maxp)
+        if n["codes"] < 1 << 28: self.gpu.upload(np.full(n["codes"], 0xA5, np.uint8), dst=self.d["codes"]["buf"])
+        self.gpu.upload(np.full(n["scales"] // 4, np.nan, np.float32), dst=self.d["scales"]["buf"])
+        self.gpu.upload(np.full(n["tail"] // 2, 0x7E01, np.uint16), dst=self.d["tail"]["buf"])
+
+    def free(self):
+        for k in ("codes", "scales", "tail", "table", "lens"): self.gpu.free(self.d[k]["buf"])
+
+    def advance(self, news):
+        self.lens = self.lens + np.asarray(news, np.uint32)
+        self.gpu.upload(self.lens, dst=self.d["lens"]["buf"])
+
+    def write(self, news, k, v, rows=True, ld=None, extra=0):
+        """k / v: lists per sequence of [Hkv][n][128] fp16"""
+        M = int(sum(news)) + extra; ld = ld or M
+        bufs, offs = [], np.concatenate([[0], np.cumsum(news)]).astype(np.uint32)
+        for x in (k, v):
+            t = np.full((self.Hkv, ld, 128), 0x7E01, np.uint16).view(np.float16)
+            for b, xb in enumerate(x): t[:, offs[b]:offs[b + 1]] = xb
+            bufs.append(self.gpu.upload(t))
+        self.advance(news)
+        rb = self.gpu.upload(offs) if rows else None
+        self.P.cacheWrite(self.gpu, {"cache": self.d, "k": {"buf": bufs[0], "ld": ld}, "v": {"buf": bufs[1], "ld": ld}, "M": M, "rows": {"buf": rb} if rows else None})
+        for b in bufs + [rb]: self.gpu.free(b)
+        for b in range(self.seqs):
+            self.tok[b] = tuple(np.concatenate([o, _clean(x[b])], 1) for o, x in zip(self.tok[b], (k, v)))
+
+    def held(self, b):
+        """K, V [Hkv][L][128] in 64 bits, as the cache should stand for them"""
+        out = []
+        for x in self.tok[b]:
+            y = x.astype(np.float64)
+            for pg in range(x.shape[1] // PAGE):
+                for h in range(self.Hkv):
+                    q, s = _quantise(x[h, pg * PAGE:(pg + 1) * PAGE])
+                    y[h, pg * PAGE:(pg + 1) * PAGE] = q * s
+            out.append(y)
+        return out
+
+    def fill(self, lens, seed=1, std=(1.0, 1.0)):
+        rng = np.random.default_rng(seed)
+        k, v = ([rng.normal(0, s, (self.Hkv, int(L), 128)).astype(np.float16) for L in lens] for s in std)
+        self.write(list(lens), k, v)
+
+    def read(self, news, rows=True, extra=0):
+        M = int(sum(news)) + extra
+        offs = np.concatenate([[0], np.cumsum(news)]).astype(np.uint32)
+        kb, vb = (self.gpu.upload(np.full((self.Hkv, M, 128), 0x7E01, np.uint16)) for _ in range(2))
+        rb = self.gpu.upload(offs) if rows else None
+        self.P.cacheRead(self.gpu, {"cache": self.d, "k": {"buf": kb}, "v": {"buf": vb}, "M": M, "rows": {"buf": rb} if rows else None})
+        out = [self.gpu.read(x).view(np.uint16)[:self.Hkv * M * 128].reshape(self.Hkv, M, 128) for x in (kb, vb)]
+        for x in (kb, vb, rb): self.gpu.free(x)
+        return out, offs
+
+
+def _attn_want(q, K, V, window, sinks, scale=None):
+    """q [Hq][n][128], K / V [Hkv][L][128] -> [n][Hq][128] in 64 bits"""
+    import torch
+    q, K, V = (torch.from_numpy(np.asarray(t, np.float64)).cuda() for t in (q, K, V))
+    Hq, n = q.shape[:2]; Hkv, L = K.shape[:2]
+    p = torch.arange(L - n, L, device="cuda")[:, None]; j = torch.arange(L, device="cuda")[None]
+    see = j <= p
+    if window: see = see & ((p - j < window) | (j < sinks))
+    s = torch.einsum("hgnd,hld->hgnl", q.view(Hkv, Hq // Hkv, n, 128), K) * (scale or 128 ** -0.5)
+    o = torch.einsum("hgnl,hld->hgnd", torch.softmax(s.masked_fill(~see, -torch.inf), -1), V)
+    return o.permute(2, 0, 1, 3).reshape(n, Hq, 128).cpu().numpy()
+
+
+def _attend(cache, news, group, window=0, sinks=0, scale=None, rows=True, new=None, kernel=None, seed=5, qstd=1.0, extra=0, ldo=None, nan_row=None):
+    """runs cacheAttention for the last `news` tokens of each sequence; returns (out [M][Hq][128], wanted list, q list)"""
+    P, gpu, Hq = cache.P, cache.gpu, cache.Hkv * group
+    rng = np.random.default_rng(seed)
+    offs = np.concatenate([[0], np.cumsum(news)]).astype(np.uint32); M = int(offs[-1]) + extra
+    q = rng.normal(0, qstd, (Hq, M, 128)).astype(np.float16)
+    if nan_row is not None: q[nan_row[0], nan_row[1], 3] = np.nan
+    ldo = ldo or Hq * 128
+    qb, ob, rb = gpu.upload(q), gpu.upload(np.full((M, ldo), 0x7E01, np.uint16)), gpu.upload(offs)
+    P.cacheAttention(gpu, {"cache": cache.d, "q": {"buf": qb}, "o": {"buf": ob, "ld": ldo}, "Hq": Hq, "M": M, "rows": {"buf": rb} if rows else None, "new": new, "window": window,
+                           "sinks": sinks, "scale": scale, "kernel": kernel})
+    raw = gpu.read(ob).view(np.uint16)[:M * ldo].reshape(M, ldo)
+    for b in (qb, ob, rb): gpu.free(b)
+    assert (raw[:, Hq * 128:] == 0x7E01).all() and (raw[offs[-1]:] == 0x7E01).all(), "written outside the rows"
+    out = np.ascontiguousarray(raw[:, :Hq * 128]).view(np.float16).reshape(M, Hq, 128)
+    return out, [q[:, offs[b]:offs[b + 1]] for b in range(cache.seqs)], offs
+
+
+def _check(cache, news, group, window=0, sinks=0, scale=None, **kw):
+    out, q, offs = _attend(cache, news, group, window, sinks, scale, **kw)
+    for b in range(cache.seqs):
+        if not news[b]: continue
+        K, V = cache.held(b)
+        want = _attn_want(q[b], K, V, window, sinks, scale)
+        got = out[offs[b]:offs[b + 1]].astype(np.float64)
+        top = np.abs(V).max()
+        tol = top * (2 * (2.0 ** -11 + 1e-4) + 2.0 ** -11 + K.shape[1] * 2.0 ** -25)
+        err = np.abs(got - want)
+        assert err.max() <= tol, (b, err.max(), tol, np.unravel_index(err.argmax(), err.shape))
+
+
+# ------------------------------------------------------------------------------------------------------------- writing, reading back
+STEPS = [
+    dict(label="one sequence, token by token over a page's end", Hkv=2, maxp=3, steps=[[62]] + [[1]] * 4, rows=False),
+    dict(label="chunks that begin and end inside pages", Hkv=3, maxp=8, steps=[[37], [64], [27], [130], [1], [63], [65]], rows=False),
+    dict(label="several sequences, some without new tokens", Hkv=1, maxp=6, steps=[[5, 0, 70, 1], [60, 1, 0, 63], [1, 0, 64, 0], [130, 200, 3, 1]], rows=True),
+    dict(label="equal counts", Hkv=2, maxp=4, steps=[[40] * 5, [1] * 5, [23] * 5, [1] * 5, [100] * 5], rows=False),
+    dict(label="more sequences than a block has threads", Hkv=1, maxp=2, steps=[[(b * 7) % 66 for b in range(300)], [1 + b % 3 for b in range(300)]], rows=True),
+]
+
+
+@pytest.mark.parametrize("c", STEPS, ids=lambda c: c["label"])
+def test_write_and_read(gpu, c):
+    """whatever the calls, each page is quantised once, from its 64 tokens; the rest is in the tail; nothing else is touched"""
+    import p0pc0rn_kernels_b200 as P
+    Hkv, seqs = c["Hkv"], len(c["steps"][0])
+    cache = Cache(P, gpu, Hkv, seqs, c["maxp"], seed=3)
+    rng = np.random.default_rng(11)
+    try:
+        for news in c["steps"]:
+            k, v = ([(rng.normal(0, 1, (Hkv, n, 128)) * np.exp(rng.normal(0, 1, (Hkv, 1, 1)))).astype(np.float16) for n in news] for _ in range(2))
+            cache.write(news, k, v, rows=c["rows"], extra=2 if c["rows"] else 0)
+            got, offs = cache.read(news, rows=c["rows"], extra=1 if c["rows"] else 0)
+            for b in range(0, seqs, max(1, seqs // 20)):
+                for g, w in zip(got, cache.held(b)):
+                    n = news[b]
+                    assert np.array_equal(g[:, offs[b]:offs[b + 1]].view(np.float16), w[:, w.shape[1] - n:].astype(np.float16)), (b, news)
+            if c["rows"]: assert all((g[:, offs[-1]:] == 0x7E01).all() for g in got)
+        # the bytes themselves
+        n = P.cacheBytes(cache.pages, Hkv, seqs, c["maxp"])
+        codes = gpu.read(cache.d["codes"]["buf"], 0, n["codes"]).reshape(cache.pages, Hkv, 2, -1)
+        scales = gpu.read(cache.d["scales"]["buf"], 0, n["scales"]).view(np.float32).reshape(cache.pages, Hkv, 2)
+        tail = gpu.read(cache.d["tail"]["buf"], 0, n["tail"]).view(np.float16).reshape(seqs, Hkv, 2, -1)
+        used = np.zeros(cache.pages, bool)
+        for b in range(0, seqs, max(1, seqs // 20)):
+            L = int(cache.lens[b])
+            for pg in range(L // PAGE):
+                page = cache.table[b, pg]; used[page] = True
+                for h in range(Hkv):
+                    for w, off in enumerate(_offsets()):
+                        q, s = _quantise(cache.tok[b][w][h, pg * PAGE:(pg + 1) * PAGE])
+                        assert scales[page, h, w] == s and np.array_equal(codes[page, h, w][off], (q + 128).astype(np.uint8))
+            for h in range(Hkv):
+                for w, off in enumerate(_offsets()):
+                    assert np.array_equal(tail[b, h, w][off][:L % PAGE], cache.tok[b][w][h, L - L % PAGE:])
+        if seqs < 20: assert (codes[~used] == 0xA5).all() and np.isnan(scales[~used]).all()
+        all_, offs = cache.read([int(x) for x in cache.lens])                                  # whole sequences
+        for b in range(0, seqs, max(1, seqs // 20)):
+            for g, w in zip(all_, cache.held(b)): assert np.array_equal(g[:, offs[b]:offs[b + 1]].view(np.float16), w.astype(np.float16))
+    finally:
+        cache.free()
+
+
+def test_write_special_values(gpu):
+    """NaN is stored as 0, infinities as the largest finite value; blocks of zeros, of subnormals, and one whose largest value stands alone"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 5, 1, 3)
+    rng = np.random.default_rng(2)
+    k = rng.normal(0, 1, (5, 100, 128)).astype(np.float16); v = rng.normal(0, 1, (5, 100, 128)).astype(np.float16)
+    k[0, 3, 7] = np.nan; v[0, 90, 0] = np.nan; k[1, 63, 127] = np.inf; v[1, 64, 5] = -np.inf; v[1, 0, 0] = -np.inf
+    k[2, :64] = 0; v[2, :64] = -0.0
+    k[3] = (rng.integers(-40, 41, (100, 128)) * 2.0 ** -24).astype(np.float16); v[3] = 0; v[3, 5, 5] = 2.0 ** -24
+    k[4, :64] = 0; k[4, 10, 10] = -65504; v[4, :64] = 1.0; v[4, 2, 3] = 2.0                   # 63.5 steps: a tie
+    try:
+        cache.write([100], [k], [v], rows=False)
+        got, _ = cache.read([100], rows=False)
+        for g, w in zip(got, cache.held(0)):
+            w = np.clip(w, -65504, 65504).astype(np.float16)
+            assert np.isfinite(g.view(np.float16)).all() and np.array_equal(g.view(np.float16), w)
+    finally:
+        cache.free()
+
+
+# ------------------------------------------------------------------------------------------------------------- attention
+ATT = [
+    dict(label="one token of context", Hkv=2, group=4, lens=[1], news=[1]),
+    dict(label="a tail only", Hkv=1, group=1, lens=[63], news=[1]),
+    dict(label="a whole page, no tail", Hkv=3, group=4, lens=[64], news=[1]),
+    dict(label="a page and one token", Hkv=2, group=8, lens=[65], news=[1]),
+    dict(label="one token, 300 of context", Hkv=8, group=4, lens=[301], news=[1]),
+    dict(label="one token, several pages per warp", Hkv=4, group=4, lens=[40000], news=[1]),
+    dict(label="ragged batch", Hkv=2, group=4, lens=[1, 64, 500, 65, 3000, 128, 129, 7], news=[1] * 8),
+    dict(label="sequences without new tokens, rows behind the last", Hkv=2, group=3, lens=[100, 0, 300, 64, 200], news=[2, 0, 0, 5, 1], extra=3),
+    dict(label="a batch of short contexts: many items per warp", Hkv=2, group=2, lens=[1 + (b * 37) % 150 for b in range(700)], news=[1] * 700),
+    dict(label="16 rows exactly", Hkv=1, group=16, lens=[200], news=[1]),
+    dict(label="17 rows: two row blocks", Hkv=1, group=17, lens=[200], news=[1]),
+    dict(label="several new tokens, odd group", Hkv=2, group=5, lens=[333, 70], news=[7, 66]),
+    dict(label="the first tokens of a prompt", Hkv=2, group=2, lens=[150], news=[150]),
+    dict(label="prompts of several sequences", Hkv=1, group=4, lens=[500, 129, 90], news=[300, 129, 1]),
+    dict(label="window inside a page", Hkv=2, group=4, lens=[300], news=[1], window=10),
+    dict(label="window 1", Hkv=2, group=4, lens=[300, 65], news=[3, 1], window=1),
+    dict(label="window and sinks far apart", Hkv=2, group=4, lens=[5000, 900, 30], news=[1, 4, 2], window=200, sinks=4),
+    dict(label="sinks over several pages", Hkv=1, group=2, lens=[2000], news=[5], window=64, sinks=130),
+    dict(label="sinks that meet the window", Hkv=1, group=2, lens=[300], news=[2], window=100, sinks=250),
+    dict(label="window wider than the context", Hkv=1, group=2, lens=[300], news=[2], window=1000, sinks=2),
+    dict(label="prompt longer than its window", Hkv=2, group=3, lens=[700, 400], news=[700, 150], window=100, sinks=3),
+    dict(label="own scale", Hkv=2, group=2, lens=[200], news=[3], scale=0.02),
+    dict(label="peaked scores", Hkv=2, group=2, lens=[700], news=[2], qstd=12.0),
+    dict(label="output rows with a stride, 4-byte aligned", Hkv=2, group=2, lens=[200], news=[3], ldo=4 * 128 + 6),
+]
+
+
+def _att_cache(P, gpu, c):
+    cache = Cache(P, gpu, c["Hkv"], len(c["lens"]), max(1, -(-max(c["lens"]) // PAGE)) + 1, seed=9)
+    cache.fill(c["lens"], std=(1.0, np.float16(0.7)))
+    return cache
+
+
+@pytest.mark.parametrize("c", ATT, ids=lambda c: c["label"])
+def test_attention(gpu, c):
+    import p0pc0rn_kernels_b200 as P
+    cache = _att_cache(P, gpu, c)
+    try:
+        kw = {k: c[k] for k in ("window", "sinks", "scale", "qstd", "extra", "ldo") if k in c}
+        for _ in range(2): _check(cache, c["news"], c["group"], **kw)                          # (twice: a counter left over would show)
+        if len(set(c["news"])) == 1: _check(cache, c["news"], c["group"], rows=False, new=c["news"][0], **{k: v for k, v in kw.items() if k != "extra"})
+    finally:
+        cache.free()
+
+
+def test_attention_scales_far_apart(gpu):
+    """pages whose values differ by a factor of 2^20, an all-zero page, a page of the largest values"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 2, 1, 8)
+    rng = np.random.default_rng(4)
+    k = rng.normal(0, 1, (2, 400, 128)); v = rng.normal(0, 1, (2, 400, 128))
+    v[:, :64] *= 2.0 ** -14; v[:, 64:128] = 0; v[:, 128:192] *= 2.0 ** 6; k[:, 192:256] *= 2.0 ** -10; k[0, 256:320] = 0; v[1, 300, :] = 60000.0
+    try:
+        cache.write([400], [k.astype(np.float16)], [v.astype(np.float16)], rows=False)
+        _check(cache, [2], 4)
+        _check(cache, [2], 4, window=330)
+    finally:
+        cache.free()
+
+
+def test_attention_nan_query_stays_in_its_row(gpu):
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 2, 2, 10)
+    cache.fill([500, 200])
+    try:
+        for kernel in (None, "split"):
+            out, q, offs = _attend(cache, [3, 2], 4, nan_row=(5, 1), kernel=kernel)
+            bad = np.zeros(out.shape[:2], bool); bad[1, 5] = True
+            assert np.isnan(out[bad]).all() and np.isfinite(out[~bad]).all()
+    finally:
+        cache.free()
+
+
+def test_attention_of_a_later_token_does_not_reach_back(gpu):
+    """an infinite value in the newest token's value (kept as the largest finite one): the queries before it do not see it"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 1, 1, 4)
+    rng = np.random.default_rng(4)
+    k, v = (rng.normal(0, 1, (1, 70, 128)).astype(np.float16) for _ in range(2))
+    v[0, 69] = np.inf; k[0, 69] = np.nan
+    try:
+        cache.write([70], [k], [v], rows=False)
+        out, q, offs = _attend(cache, [4], 2)
+        want = _attn_want(q[0][:, :3], *(x[:, :69] for x in cache.held(0)), 0, 0)
+        top = np.abs(v[0, :69].astype(np.float64)).max()
+        assert np.abs(out[:3] - want).max() <= top * (2 * (2.0 ** -11 + 1e-4) + 2.0 ** -11 + 70 * 2.0 ** -25)
+    finally:
+        cache.free()
+
+
+def test_cache_past_32_bit_offsets(gpu):
+    """pages that lie more than 2^32 bytes into the codes"""
+    import p0pc0rn_kernels_b200 as P
+    Hkv = 8
+    cache = Cache(P, gpu, Hkv, 2, 5, pages=34000, first_page=33800)
+    try:
+        assert int(cache.table.min()) * Hkv * 16384 > 1 << 32
+        cache.fill([300, 130])
+        got, offs = cache.read([300, 130])
+        for b in range(2):
+            for g, w in zip(got, cache.held(b)): assert np.array_equal(g[:, offs[b]:offs[b + 1]].view(np.float16), w.astype(np.float16))
+        _check(cache, [3, 1], 4)
+    finally:
+        cache.free(); gpu.drainPool()
+
+
+# ------------------------------------------------------------------------------------------------------------- rotary positions
+def _freq(rot, theta=10000.0, factor=1.0, original=0.0, fast=32.0, slow=1.0):
+    i = np.arange(rot // 2); f = theta ** (-2.0 * i / rot) if rot else np.zeros(0)
+    if factor == 1.0: return f
+    g = np.clip((original * f / (2 * np.pi) - slow) / (fast - slow), 0, 1) if original else 0.0
+    return f * (g + (1 - g) / factor)
+
+
+ROPE = [
+    dict(label="half", mode="half", H=5, news=[1], lens=[1]),
+    dict(label="interleaved, far out", mode="interleaved", H=3, news=[4, 1, 0, 30], lens=[4, 900000, 7, 4000000000]),
+    dict(label="part of the head, half", mode="half", rot=64, H=2, news=[33], lens=[500]),
+    dict(label="part of the head, half, odd", mode="half", rot=38, H=2, news=[33, 2], lens=[500, 70]),
+    dict(label="half of an odd half", mode="half", rot=6, H=3, news=[5], lens=[5]),
+    dict(label="part of the head, interleaved", mode="interleaved", rot=90, H=2, news=[33], lens=[500]),
+    dict(label="nothing turned", mode="half", rot=0, H=2, news=[3], lens=[5]),
+    dict(label="scaled linearly", mode="half", H=2, news=[40], lens=[100000], factor=4.0),
+    dict(label="scaled by parts", mode="interleaved", H=2, news=[40], lens=[100000], factor=8.0, original=4096, mscale=1.2, theta=500000.0),
+    dict(label="scaled by parts, own limits, half", mode="half", rot=96, H=70, news=[40, 3], lens=[100000, 10], factor=8.0, original=8192, fast=16.0, slow=2.0),
+    dict(label="many tokens and heads", mode="half", H=40, news=[1000, 37], lens=[1000, 5000]),
+]
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("c", ROPE, ids=lambda c: c["label"])
+def test_rope(gpu, c, inplace):
+    import p0pc0rn_kernels_b200 as P
+    rng = np.random.default_rng(1)
+    H, rot, news = c["H"], c.get("rot", 128), c["news"]
+    offs = np.concatenate([[0], np.cumsum(news)]).astype(np.uint32); M, ld = int(offs[-1]) + 2, int(offs[-1]) + 5
+    x = rng.normal(0, 1, (H, ld, 128)).astype(np.float16)
+    xb, yb, lb, rb = gpu.upload(x), gpu.upload(np.full((H, M, 128), 0x7E01, np.uint16)), gpu.upload(np.array(c["lens"], np.uint32)), gpu.upload(offs)
+    extra = {k: c[k] for k in ("theta", "factor", "original", "fast", "slow", "mscale") if k in c}
+    try:
+        P.rope(gpu, {"x": {"buf": xb, "ld": ld}, "y": None if inplace else {"buf": yb}, "H": H, "M": M, "seqs": len(news), "lens": {"buf": lb}, "rows": {"buf": rb}, "mode": c["mode"], "rot": rot, **extra})
+        got = gpu.read(xb).view(np.float16)[:x.size].reshape(x.shape) if inplace else gpu.read(yb).view(np.float16)[:H * M * 128].reshape(H, M, 128)
+        if inplace: assert np.array_equal(got[:, offs[-1]:], x[:, offs[-1]:])
+        else: assert (got[:, offs[-1]:].view(np.uint16) == 0x7E01).all()
+        pos = np.concatenate([np.arange(L - n, L, dtype=np.float64) for L, n in zip(c["lens"], news)])
+        ang = pos[:, None] * _freq(rot, **{k: v for k, v in extra.items() if k != "mscale"})
+        ms = c.get("mscale", 1.0); cs, sn = np.cos(ang) * ms, np.sin(ang) * ms
+        x = x[:, :offs[-1]].astype(np.float64); want = x.copy()
+        first, second = (slice(0, rot // 2), slice(rot // 2, rot)) if c["mode"] == "half" else (slice(0, rot, 2), slice(1, rot, 2))
+        a, b = x[..., first], x[..., second]
+        want[..., first], want[..., second] = a * cs - b * sn, a * sn + b * cs
+        mag = np.zeros_like(want); mag[..., first] = mag[..., second] = (np.abs(a) + np.abs(b)) * ms
+        # (an angle in 64 bits: position * frequency in turns and the oracle's own product are each off by 2^-53 of the angle)
+        tol = np.abs(want) * 2.0 ** -11 + 2.0 ** -25 + mag * (6 * 2.0 ** -24 + float(pos.max(initial=1.0)) * 8 * 2.0 ** -53)
+        assert (np.abs(got[:, :offs[-1]].astype(np.float64) - want) <= tol).all()
+        assert np.array_equal(got[:, :offs[-1], rot:], x[..., rot:].astype(np.float16))
+    finally:
+        for t in (xb, yb, lb, rb): gpu.free(t)
+
+
+# ------------------------------------------------------------------------------------------------------------- together
+def test_decoding_loop_recorded_once(gpu):
+    """rotary positions, write and attention of a decoding step, recorded once and replayed over pages' ends with new lengths: as a program runs
+    them.  A second recording, of another batch, shares the scratch memory and is replayed in between."""
+    import p0pc0rn_kernels_b200 as P
+    rng = np.random.default_rng(8)
+    own = P.createGpu({"device": 0})
+    Hkv, group, seqs = 2, 4, 3
+    Hq = Hkv * group
+    rot = {"mode": "half", "rot": 128, "theta": 10000.0}
+
+    def turn(x, p):
+        cs, sn = np.cos(p * _freq(128)), np.sin(p * _freq(128)); x = x.astype(np.float64)
+        a, b = x[..., :64], x[..., 64:]
+        return np.concatenate([a * cs - b * sn, a * sn + b * cs], -1)
+    sets = []
+    for start in ([60, 127, 0], [700, 3, 64]):
+        cache = Cache(P, own, Hkv, seqs, 14, seed=sum(start))
+        cache.fill(start)
+        heads, ob = own.buffer((Hq + 2 * Hkv) * seqs * 256), own.buffer(seqs * Hq * 256)
+        n = seqs * 256
+
+        def step(cache=cache, heads=heads, ob=ob, n=n):
+            P.rope(own, {"x": {"buf": heads}, "H": Hq + Hkv, "M": seqs, "seqs": seqs, "lens": cache.d["lens"], **rot})
+            P.cacheWrite(own, {"cache": cache.d, "k": {"buf": heads, "off": Hq * n}, "v": {"buf": heads, "off": (Hq + Hkv) * n}, "M": seqs})
+            P.cacheAttention(own, {"cache": cache.d, "q": {"buf": heads}, "o": {"buf": ob}, "Hq": Hq, "M": seqs})
+        sets.append([cache, heads, ob, step, None])
+    try:
+        for s in sets:                                   # one eager step each, then recorded
+            s[0].advance([1] * seqs); x = rng.normal(0, 1, (Hq + 2 * Hkv, seqs, 128)).astype(np.float16); own.upload(x, dst=s[1]); s[3](); _step_check(s, x, turn, own, Hq, Hkv)
+            s[4] = own.record(s[3])
+        for it in range(8):
+            for s in sets:
+                s[0].advance([1] * seqs); x = rng.normal(0, 1, (Hq + 2 * Hkv, seqs, 128)).astype(np.float16); own.upload(x, dst=s[1]); s[4].launch(); _step_check(s, x, turn, own, Hq, Hkv)
+        assert not own.lost
+    finally:
+        for s in sets:
+            if s[4]: s[4].free()
+            s[0].free()
+        own.close()
+
+
+def _step_check(s, x, turn, own, Hq, Hkv):
+    cache, heads, ob = s[:3]
+    seqs = cache.seqs
+    y = own.read(heads).view(np.float16)[:x.size].reshape(x.shape)
+    out = own.read(ob).view(np.float16)[:seqs * Hq * 128].reshape(seqs, Hq, 128)
+    for b in range(seqs):
+        p = float(cache.lens[b] - 1)
+        want = turn(x[:Hq + Hkv, b], p)
+        assert np.abs(y[:Hq + Hkv, b] - want).max() <= np.abs(want).max() * 2.0 ** -11 + 1e-5
+        cache.tok[b] = tuple(np.concatenate([o, t[:, b:b + 1]], 1) for o, t in zip(cache.tok[b], (y[Hq:Hq + Hkv], x[Hq + Hkv:])))
+        K, V = cache.held(b)
+        w = _attn_want(y[:Hq, b:b + 1], K, V, 0, 0)[0]
+        assert np.abs(out[b] - w).max() <= np.abs(V).max() * (2 * (2.0 ** -11 + 1e-4) + 2.0 ** -11 + K.shape[1] * 2.0 ** -25)
+
+
+def test_another_stream(gpu):
+    """a context on the host framework's stream: tensors made there, no waiting in between"""
+    import torch
+
+    import p0pc0rn_kernels_b200 as P
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        own = P.createGpu({"device": 0, "stream": st.cuda_stream})
+        try:
+            cache = Cache(P, own, 2, 2, 6)
+            cache.fill([300, 100])
+            _check(cache, [2, 1], 4)
+            cache.free()
+        finally:
+            own.close()
+
+
+# ------------------------------------------------------------------------------------------------------------- refusals
+def test_refusals(gpu):
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 2, 3, 2)
+    b = gpu.buffer(1 << 20)
+    t = {"buf": b}
+    kv = {"cache": cache.d, "k": t, "v": t, "M": 6}
+    at = {"cache": cache.d, "q": t, "o": t, "Hq": 4, "M": 6}
+    ro = {"x": t, "H": 4, "M": 6, "seqs": 3, "lens": cache.d["lens"]}
+
+    def no(op, args, text, **change):
+        a = dict(args); a.update(change)
+        with pytest.raises(ValueError, match=text): op(gpu, a)
+
+    def but(**kw):
+        return dict(cache.d, **kw)
+    try:
+        for op, a in ((P.cacheWrite, kv), (P.cacheRead, kv), (P.cacheAttention, at)):
+            no(op, a, "multiple of seqs", M=7)
+            no(op, a, "codes needs", cache=but(pages=1000)); no(op, a, "table needs", cache=but(maxPages=2000)); no(op, a, "at least one", cache=but(pages=0))
+            no(op, a, "at most 1024", cache=but(seqs=1025)); no(op, a, "missing", cache=but(tail={"buf": type("B", (), {"handle": None})()}))
+            no(op, a, "16 bytes", cache=but(codes={"buf": cache.d["codes"]["buf"], "off": 8}))
+            no(op, a, "rows needs", rows={"buf": gpu.bufs and b, "off": (1 << 20) - 8})
+        no(P.cacheWrite, kv, "k needs", M=3000); no(P.cacheWrite, kv, "v.ld", v={"buf": b, "ld": 5}); no(P.cacheWrite, kv, "multiple of 16", k={"buf": b, "off": 4})
+        no(P.cacheAttention, at, "multiple of Hkv", Hq=3); no(P.cacheAttention, at, "o needs", o={"buf": b, "ld": 1 << 18}); no(P.cacheAttention, at, "o.ld", o={"buf": b, "ld": 511})
+        no(P.cacheAttention, at, "finite", scale=float("nan")); no(P.cacheAttention, at, "q needs", M=3000)
+        no(P.rope, ro, "even", rot=7); no(P.rope, ro, "even", rot=130); no(P.rope, ro, "unknown mode", mode="x"); no(P.rope, ro, "positive", theta=-1.0); no(P.rope, ro, "fast above slow", fast=1.0, slow=2.0)
+        no(P.rope, ro, "multiple of seqs", M=7); no(P.rope, ro, "x needs", M=3000); no(P.rope, ro, "sequences", seqs=0); no(P.rope, ro, "multiple of 16", x={"buf": b, "off": 2})
+        assert not gpu.lost
+        for op, a in ((P.cacheWrite, kv), (P.cacheRead, kv), (P.cacheAttention, at), (P.rope, ro)): op(gpu, dict(a, M=0))      # nothing to do
+        gpu.done()
+    finally:
+        gpu.free(b); cache.free()
+
+
+def test_numbers_on_the_device_that_make_no_sense(gpu):
+    """row offsets, lengths and page numbers are checked where they are read: the sequence is left out (a page not followed), the next wait says
+    so, and the context goes on"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 2, 2, 4, spare=0)
+    cache.fill([100, 130])
+    ok, _ = cache.read([100, 130])
+    lens, table = cache.d["lens"]["buf"], cache.d["table"]["buf"]
+    b, r = gpu.buffer(1 << 20), gpu.upload(np.array([0, 2, 3], np.uint32))
+    calls = [lambda: P.cacheWrite(gpu, {"cache": cache.d, "k": {"buf": b}, "v": {"buf": b}, "M": 3, "rows": {"buf": r}}),
+             lambda: P.cacheRead(gpu, {"cache": cache.d, "k": {"buf": b}, "v": {"buf": b}, "M": 3, "rows": {"buf": r}}),
+             lambda: P.cacheAttention(gpu, {"cache": cache.d, "q": {"buf": b}, "o": {"buf": b, "off": 1 << 19}, "Hq": 4, "M": 3, "rows": {"buf": r}})]
+    rope = lambda: P.rope(gpu, {"x": {"buf": b}, "H": 4, "M": 3, "seqs": 2, "lens": {"buf": lens}, "rows": {"buf": r}})  # noqa: E731
+
+    def fails(call, text):
+        call()
+        with pytest.raises(P.GpuError, match=text): gpu.done()
+        gpu.done()
+    try:
+        for bad in ([0, 3, 2], [0, 2, 4], [0, 4, 4]):
+            gpu.upload(np.array(bad, np.uint32), dst=r)
+            for call in calls: fails(call, "row offsets")
+        gpu.upload(np.array([0, 2, 3], np.uint32), dst=r)
+        for bad in ([1, 130], [100, 0], [100, 257], [0xffffffff, 130]):
+            gpu.upload(np.array(bad, np.uint32), dst=lens)
+            for call in calls: fails(call, "fewer tokens than rows")
+        gpu.upload(np.array([1, 130], np.uint32), dst=lens)
+        fails(rope, "fewer tokens")
+        gpu.upload(np.array([128, 130], np.uint32), dst=lens)                                  # (the write would finish page 1 of sequence 0)
+        for bad in (cache.pages, 0xffffffff):
+            t = cache.table.copy(); t[0, 1] = bad
+            gpu.upload(t, dst=table)
+            for call in calls: fails(call, "page number")
+        gpu.upload(cache.table, dst=table); gpu.upload(cache.lens, dst=lens)
+        again, offs = cache.read([100, 130])
+        assert all(np.array_equal(x[:, :64], y[:, :64]) and np.array_equal(x[:, 100:228], y[:, 100:228]) for x, y in zip(ok, again)) and not gpu.lost
+        _check_ok = [int(x) for x in cache.lens]
+        assert _check_ok == [100, 130]
+    finally:
+        for x in (b, r): gpu.free(x)
+        cache.free()

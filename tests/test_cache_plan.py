@@ -1,0 +1,189 @@
+"""The arithmetic of the 8-bit cache (csrc/cache_plan.h): orders within a page, touched and visible pages, how attention's work is dealt out,
+numbers and arguments that are refused.  Plain C++: compiled and run here without a GPU, with the address sanitizer."""
+import os
+import subprocess
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PROGRAM = r"""
+#include <cstdlib>
+#include <cstring>
+#include <vector>
+#include "cache_plan.h"
+using namespace p0p;
+#define CHECK(c) do { if (!(c)) { printf("line %d: %s\n", __LINE__, #c); exit(1); } } while (0)
+static uint32_t rnd(uint32_t n) { static uint64_t x = 88172645463325252ull; x ^= x << 13; x ^= x >> 7; x ^= x << 17; return (uint32_t)((x >> 11) % n); }
+
+int main() {
+  {   // both orders are permutations of a page
+    std::vector<int> k(CACHE_BLOCK, 0), v(CACHE_BLOCK, 0);
+    for (uint32_t key = 0; key < 64; key++) for (uint32_t d = 0; d < 128; d++) { k[cache_k_off(key, d)]++; v[cache_v_off(key, d)]++; }
+    for (uint32_t i = 0; i < CACHE_BLOCK; i++) CHECK(k[i] == 1 && v[i] == 1);
+    // a lane's 16 elements: K 16 consecutive d of one key, V keys 16 j + 4 t + i of one d
+    CHECK(cache_k_off(5, 33) == cache_k_off(5, 32) + 1 && cache_k_off(5, 47) == cache_k_off(5, 32) + 15);
+    CHECK(cache_v_off(16 + 4, 9) == cache_v_off(4, 9) + 4 && cache_v_off(7, 9) == cache_v_off(4, 9) + 3);
+  }
+  {   // numbers that make no sense leave a sequence without new tokens
+    CacheSeq s;
+    CHECK(cache_seq_check(3, 2, 10, 10, 4, s) == CACHE_BAD_ROWS && s.n == 0);
+    CHECK(cache_seq_check(3, 11, 10, 10, 4, s) == CACHE_BAD_ROWS && s.n == 0);
+    CHECK(cache_seq_check(3, 8, 4, 10, 4, s) == CACHE_BAD_LENS && s.n == 0);
+    CHECK(cache_seq_check(3, 8, 257, 10, 4, s) == CACHE_BAD_LENS && s.n == 0);
+    CHECK(cache_seq_check(3, 3, 0xffffffffu, 10, 4, s) == 0 && s.n == 0);
+    CHECK(cache_seq_check(3, 8, 256, 10, 4, s) == 0 && s.n == 5 && s.r0 == 3 && s.L == 256);
+    CHECK(cache_seq_check(0, 5, 0xffffffffu, 10, (1u << 26) - 1u, s) == CACHE_BAD_LENS);
+  }
+  for (int it = 0; it < 4000; it++) {   // touched pages and their bound
+    const uint32_t seqs = 1 + rnd(8);
+    uint32_t M = 0; uint64_t all = 0;
+    for (uint32_t b = 0; b < seqs; b++) {
+      CacheSeq s{M, rnd(4) ? rnd(5) : rnd(300), 0};
+      s.L = s.n + rnd(300);
+      M += s.n;
+      uint32_t want = 0;
+      for (uint32_t pg = 0; pg < 20; pg++) { bool t = false; for (uint32_t p = s.L - s.n; p < s.L; p++) t |= p / 64 == pg; want += t; if (t) CHECK(pg >= cache_first_page(s) && pg < cache_first_page(s) + cache_touched(s)); }
+      CHECK(cache_touched(s) == want);
+      if (s.n) CHECK(want <= cache_touched_bound(s.n, 1));
+      all += want;
+    }
+    CHECK(all <= cache_touched_bound(M, seqs));
+  }
+  for (int it = 0; it < 4000; it++) {   // visible pages: all that any new query sees, none twice, the last one last
+    CacheSeq s{0, 1 + rnd(rnd(2) ? 4 : 200), 0};
+    s.L = s.n + rnd(900);
+    const uint32_t window = rnd(3) ? 1 + rnd(rnd(2) ? 10 : 500) : 0, sinks = rnd(2) ? rnd(rnd(2) ? 5 : 300) : 0;
+    const CacheVis v = cache_visible(s, window, window ? sinks : 0);
+    std::vector<int> listed(40, 0);
+    CHECK(v.np > 0 && cache_vis_page(v, v.np - 1) == (s.L - 1) / 64);
+    for (uint32_t t = 0; t < v.np; t++) { const uint32_t pg = cache_vis_page(v, t); CHECK(pg < 40 && pg <= (s.L - 1) / 64); listed[pg]++; if (t) CHECK(pg > cache_vis_page(v, t - 1)); }
+    for (uint32_t pg = 0; pg <= (s.L - 1) / 64; pg++) {
+      bool seen = false, hidden = false;
+      for (uint32_t p = s.L - s.n; p < s.L; p++) for (uint32_t k = pg * 64; k < pg * 64 + 64; k++) {
+        const bool want = k <= p && (!window || k + window > p || k < sinks);
+        CHECK(cache_key_visible(k, p, window, sinks) == want);
+        if (want) seen = true; else hidden = true;
+      }
+      CHECK(!seen || listed[pg] == 1);
+      if (hidden && listed[pg]) CHECK(cache_page_masked(pg, s.L - s.n, s.L - 1, window, sinks));
+    }
+  }
+  for (int it = 0; it < 600; it++) {   // the units: every worker's walk, and whom a unit belongs to
+    const uint32_t seqs = 1 + rnd(rnd(2) ? 3 : 40);
+    const CacheGeo g{1 + rnd(9), 1 + rnd(20), seqs, rnd(2) ? 1 + rnd(300) : 0, rnd(70)};
+    std::vector<CacheSeq> seq(seqs);
+    std::vector<uint64_t> pre(seqs + 1, 0);
+    uint64_t U = 0;
+    struct Unit { uint32_t b, hk, rb, t; };
+    std::vector<Unit> all;
+    for (uint32_t b = 0; b < seqs; b++) {
+      seq[b] = CacheSeq{0, rnd(3) ? rnd(3) : rnd(40), 0};
+      seq[b].L = seq[b].n + rnd(400);
+      U += cache_units(seq[b], g); pre[b + 1] = U;
+      if (!seq[b].n) continue;
+      const uint32_t np = cache_visible(seq[b], g.window, g.sinks).np;
+      for (uint32_t h = 0; h < g.Hkv; h++) for (uint32_t rb = 0; rb * 16 < seq[b].n * g.group; rb++) for (uint32_t t = 0; t < np; t++) all.push_back({b, h, rb, t});
+    }
+    CHECK(U == all.size());
+    if (!U) continue;
+    const uint64_t G = U < 148 ? U : 148;
+    CHECK(deal_first(0, U, G) == 0 && deal_first(G, U, G) == U);
+    for (uint64_t c = 0; c < G; c++) {
+      const uint64_t u0 = deal_first(c, U, G), u1 = deal_first(c + 1, U, G), n = u1 - u0, W = n < 8 ? n : 8;
+      CHECK(n > 0);
+      for (uint64_t u = u0; u < u1; u++) CHECK(deal_owner(u, U, G) == c);
+      for (uint64_t w = 0; w < W; w++) {
+        const uint64_t w0 = u0 + deal_first(w, n, W), w1 = u0 + deal_first(w + 1, n, W);
+        CHECK(w1 > w0);
+        CacheCursor x;
+        x.seek(g, pre.data(), seq.data(), w0);
+        for (uint64_t u = w0; u < w1; u++) {
+          CHECK(x.b == all[u].b && x.hk == all[u].hk && x.rb == all[u].rb && x.t == all[u].t && x.page() <= (x.s.L - 1) / 64);
+          CHECK(x.tail() == (x.s.L % 64 != 0 && x.page() == x.s.L / 64) && (!x.tail() || x.t + 1 == x.v.np));
+          if (u + 1 < w1) x.next(g, pre.data(), seq.data());
+        }
+      }
+    }
+  }
+  {   // refusals
+    char msg[256];
+    CacheShape ok{8, 10, 4, 5, 10 * 8 * 16384, 10 * 8 * 8, 4 * 8 * 32768, 4 * 5 * 4, 16, 0, 0, 0, 0, 0};
+    CHECK(cache_shape_check("x", ok, msg, sizeof msg) == 0);
+    CacheShape s;
+#define BAD(field, value, rc, text) do { s = ok; s.field = value; CHECK(cache_shape_check("x", s, msg, sizeof msg) == rc); CHECK(strstr(msg, text)); } while (0)
+    BAD(Hkv, 0, -2, "at least one"); BAD(pages, 0, -2, "at least one"); BAD(seqs, 0, -2, "at least one"); BAD(max_pages, 0, -2, "at least one");
+    BAD(Hkv, 65536, -2, "65535"); BAD(seqs, 1025, -2, "1024"); BAD(max_pages, 1u << 26, -2, "2^26");
+    BAD(codes, 0, -4, "missing"); BAD(lens, 0, -4, "missing");
+    BAD(codes_off, 8, -5, "16 bytes"); BAD(tail_off, 4, -5, "16 bytes"); BAD(scales_off, 4, -5, "8 bytes"); BAD(table_off, 2, -5, "of 4"); BAD(lens_off, 1, -5, "of 4");
+    BAD(codes, ok.codes - 1, -7, "codes needs"); BAD(scales, ok.scales - 1, -7, "scales needs"); BAD(tail, ok.tail - 1, -7, "tail needs"); BAD(table, ok.table - 1, -7, "table needs");
+    BAD(lens, ok.lens - 1, -7, "lens needs"); BAD(pages, 11, -7, "codes needs"); BAD(pages, 0xffffffffu, -7, "codes needs");
+    CHECK(cache_rows_check("x", 12, 4, false, 0, 0, msg, sizeof msg) == 0 && cache_rows_check("x", 13, 4, false, 0, 0, msg, sizeof msg) == -3);
+    CHECK(cache_rows_check("x", 13, 4, true, 20, 0, msg, sizeof msg) == 0 && cache_rows_check("x", 13, 4, true, 19, 0, msg, sizeof msg) == -7 && cache_rows_check("x", 13, 4, true, 20, 2, msg, sizeof msg) == -5);
+    CHECK(cache_heads_check("x", "k", 3, 5, 7, 19 * 256, 0, msg, sizeof msg) == 0 && cache_heads_check("x", "k", 3, 5, 7, 19 * 256 - 1, 0, msg, sizeof msg) == -7);
+    CHECK(cache_heads_check("x", "k", 3, 5, 4, 1 << 20, 0, msg, sizeof msg) == -5 && cache_heads_check("x", "k", 3, 5, 5, 1 << 20, 8, msg, sizeof msg) == -5);
+  }
+  printf("fine\n");
+  return 0;
+}
+"""
+
+
+def test_cache_plan(tmp_path):
+    src, exe = tmp_path / "plan.cpp", tmp_path / "plan"
+    src.write_text(PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-Wall", "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                    "-I", os.path.join(ROOT, "p0pc0rn_kernels_b200", "csrc"), str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
+
+
+def test_code_rounding_is_exact(tmp_path):
+    """the two-step rounding of cacheWrite (fused multiply by the reciprocal plus 768, then plus a constant), for every fp16 magnitude under a sweep of
+    scales: equal to the quotient in 64 bits rounded to the nearest, ties to even; and no code exceeds 127"""
+    src, exe = tmp_path / "code.cpp", tmp_path / "code"
+    src.write_text(r"""
+#include <cmath>
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+static float h2f(uint32_t h) { const int e = (h >> 10) & 31, m = h & 1023; return e ? std::ldexp((float)(1024 + m), e - 25) : std::ldexp((float)m, -24); }
+static uint32_t bits(float f) { uint32_t u; memcpy(&u, &f, 4); return u; }
+int main() {
+  for (uint32_t a = 1; a < 0x7c00; a += a < 2048 ? 1 : 37) {
+    const float amax = h2f(a);
+    uint32_t b = (bits(amax / 127.0f) + 4095u) & ~4095u; float s; memcpy(&s, &b, 4);
+    int e; const double fr = std::frexp((double)amax / 127.0, &e), up = std::ldexp(std::ceil(fr * 4096.0), e - 12);
+    if ((double)s != up) { printf("scale %a %a\n", (double)s, up); return 1; }
+    const float inv = 1.0f / s;
+    for (uint32_t x = 0; x <= a; x += x + 3000 < a && x > 2048 ? 11 : 1) {
+      const float f = h2f(x);
+      volatile float t = fmaf(f, inv, 768.0f);
+      volatile float r = t + (12582912.0f + 128.0f - 768.0f);
+      const int got = (int)(bits(r) & 255u) - 128;
+      const double want = std::nearbyint((double)f / (double)s);
+      if ((double)got != want || got > 127) { printf("%a / %a: %d, %g\n", (double)f, (double)s, got, want); return 1; }
+      volatile float tn = fmaf(-f, inv, 768.0f);
+      volatile float rn = tn + (12582912.0f + 128.0f - 768.0f);
+      if ((int)(bits(rn) & 255u) - 128 != -got) { printf("sign\n"); return 1; }
+    }
+  }
+  printf("fine\n");
+}
+""")
+    subprocess.run(["g++", "-O2", "-mfma", str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
+
+
+def test_argument_blocks_match_the_header(tmp_path):
+    """the ctypes transcriptions have the header's sizes and field offsets"""
+    import ctypes as C
+
+    from p0pc0rn_kernels_b200._lib import Cache, CacheArgs, CacheAttnArgs, RopeArgs
+    blocks = {"p0p_cache": Cache, "p0p_cache_args": CacheArgs, "p0p_cache_attn_args": CacheAttnArgs, "p0p_rope_args": RopeArgs}
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    lines = "".join(f'printf("%zu\\n", sizeof({n}));' + "".join(f'printf("%zu\\n", offsetof({n}, {f[0]}));' for f in t._fields_) for n, t in blocks.items())
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "p0p.h"\nint main(void){' + lines + "return 0;}\n")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    want = [v for t in blocks.values() for v in [C.sizeof(t)] + [getattr(t, f[0]).offset for f in t._fields_]]
+    assert got == want
