@@ -119,6 +119,62 @@ struct CacheCursor {
   P0P_HD bool tail() const { return page() == s.L / CACHE_PAGE; }
 };
 
+// The tensor-memory attention's work: an item = up to 2 * qpt queries of a sequence (qpt: those whose heads of one kv head fill a tile of 128
+// rows) and one kv head, a unit = two visible pages of it.  Per sequence [block of queries][kv head][pair of pages].
+struct CacheTcGeo { uint32_t Hkv, group, seqs, window, sinks, qpt, min_rows; };      // sequences with at most min_rows rows per kv head are the other kernel's
+P0P_HD uint32_t cache_tc_blocks(const CacheSeq& s, const CacheTcGeo& g) {
+  return s.n && (uint64_t)s.n * g.group > g.min_rows ? (s.n - 1u) / (2u * g.qpt) + 1u : 0u;
+}
+// the queries of block x, as a sequence that ends with them
+P0P_HD CacheSeq cache_tc_part(const CacheSeq& s, const CacheTcGeo& g, uint32_t x) {
+  CacheSeq p;
+  const uint32_t q0 = x * 2u * g.qpt;
+  p.r0 = s.r0 + q0; p.n = s.n - q0 < 2u * g.qpt ? s.n - q0 : 2u * g.qpt; p.L = s.L - s.n + q0 + p.n;
+  return p;
+}
+P0P_HD uint32_t cache_tc_units(const CacheSeq& part, const CacheTcGeo& g) { return (cache_visible(part, g.window, g.sinks).np + 1u) / 2u; }
+// the key of column c of a page's 64 score columns (the order in which a lane's V elements lie)
+P0P_HD constexpr uint32_t cache_col_key(uint32_t c) { return 16u * ((c >> 2) & 3u) + 4u * (c >> 4) + (c & 3u); }
+// What a block does next: units [t, t + cnt) of an item.  Every role of the block walks the same list by itself.  get(b): sequence b.
+struct CacheTcWalk {
+  CacheSeq s, part; CacheVis v;
+  uint32_t b, x, hk, t, units, cnt, left;
+  P0P_HD void item(const CacheTcGeo& g) {
+    part = cache_tc_part(s, g, x);
+    v = cache_visible(part, g.window, g.sinks);
+    units = (v.np + 1u) / 2u;
+  }
+  template <class Get>
+  P0P_HD void begin(const CacheTcGeo& g, uint32_t b_, uint32_t x_, uint32_t hk_, uint32_t t_, uint32_t left_, Get get) {
+    b = b_; x = x_; hk = hk_; t = t_; left = left_; cnt = 0u;
+    if (!left) return;
+    s = get(b);
+    item(g);
+    cnt = units - t < left ? units - t : left;
+  }
+  template <class Get>
+  P0P_HD void next(const CacheTcGeo& g, Get get) {
+    left -= cnt; t = 0u; cnt = 0u;
+    if (!left) return;
+    if (++hk == g.Hkv) {
+      hk = 0u;
+      if (++x == cache_tc_blocks(s, g)) {
+        x = 0u;
+        do { b++; s = get(b); } while (b + 1u < g.seqs && cache_tc_blocks(s, g) == 0u);
+      }
+      item(g);
+    }
+    cnt = units < left ? units : left;
+  }
+  P0P_HD bool two(const CacheTcGeo& g) const { return part.n > g.qpt; }      // both tiles of rows hold queries
+};
+// how many blocks share U units: at least four units each, but no fewer blocks than items
+P0P_HD uint64_t cache_tc_workers(uint64_t U, uint64_t items, uint64_t most) {
+  uint64_t g = U / 4u > items ? U / 4u : items;
+  if (g > most) g = most;
+  return g > U ? U : g;
+}
+
 // ---- arguments.  Sizes are the bytes from the given offset to the buffer's end (0: no buffer).
 struct CacheShape {
   uint32_t Hkv, pages, seqs, max_pages;

@@ -1,0 +1,503 @@
+// Attention over the 8-bit cache for many new tokens per sequence (prompts), on the 5th-generation tensor cores.  The products, the running maximum
+// and tensor memory are those of k_attn_tc.cuh (S = Q K^T, O += P V, two tiles of 128 rows that share every K / V tile, lane = row); what differs:
+//   rows    a tile's rows are the queries of ALL heads that share a kv head, query by query (row = query * group + head), so a page is read
+//           and converted once for them
+//   K, V    arrive as codes (bulk copies into a ring of 16-KB slots: K or V of two pages) and are turned into fp16 whole numbers - exact - by four
+//           warps, into the swizzled tiles that the multiplies read.  The cache's order makes a lane's 16 codes 32 consecutive bytes of a tile: for K 16 d of
+//           one key, for V 16 keys of one d (so V's tile is K-major).  The keys stand in the order of V's elements in both (cache_col_key).
+//   scales  a thread's 64 scores belong to one page: its K scale joins the softmax scale, its V scale the exponent (w = 2^(score + log2 vs - m),
+//           and the sum of the weights is weighted with 1 / vs), as in k_cache_attn.cuh
+//   work    the pairs of visible pages of all items (block of queries, kv head) in one row are dealt out evenly to one block per SM, from the
+//           numbers on the device; an item that crosses blocks leaves partial results that k_cache_merge adds up, in order
+// Roles: warp 0 loads, warp 1 multiplies, warps 4-7 convert, warps 8-15 and 16-23 are the softmax of the two tiles, two threads per row.  The softmax
+// threads take the registers that the others leave (setmaxnreg; per scheduler 4 x 104 + 2 x 32 = the 6 x 80 of the launch).
+// Bound: instruction issue (softmax and conversion) and the tensor cores, in that order.
+#pragma once
+#include <cuda.h>
+
+#include "attn_tc.cuh"
+#include "cache_dev.cuh"
+#include "epilogue.cuh"
+#include "umma.cuh"
+
+namespace p0p {
+
+struct CacheTcDesc { uint32_t on, row0, q, hk, c1; };      // an item that begins in this block and goes on: its first row, its queries, its last block
+struct CacheTcP {
+  CacheP c;
+  __half* O;
+  uint32_t ldo;
+  CacheTcGeo geo;
+  float scale_log2;
+  float4* part;          // [block][2][32 groups of 4 columns][256 rows] unnormalised O
+  float2* part_ml;       // [block][2][256 rows] (maximum, sum)
+  CacheTcDesc* desc;     // [block]
+};
+
+constexpr uint32_t CTC_THREADS = 768u, CTC_SLOTS = 3u, CTC_STAGES = 3u, CTC_STAGE = 2u * CACHE_BLOCK;
+constexpr int CTC_REGS = 16 * 104 + 8 * 32;      // registers per lane of all warps, after setmaxnreg
+constexpr uint32_t CTC_SCL = 8u;       // tiles whose scales are kept: the loads are at most three tiles ahead of the softmax
+constexpr uint32_t CTC_SMEM = 1024u + (2u + CTC_SLOTS) * ATC_TILE + CTC_STAGES * CTC_STAGE + 256u + 4096u + CTC_SCL * 16u + 64u;
+static_assert(CTC_SMEM <= 232448u, "shared memory");
+static_assert(CTC_STAGES * CTC_STAGE >= CACHE_MAX_SEQS * 8u, "the sequences' unit counts fit the staging ring while nothing is in it");
+
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// 16 codes (code + 128) -> 16 fp16 whole numbers: a byte behind 0x64 is 1024 + code + 128
+__device__ __forceinline__ void ctc_convert(uint4 w, uint4& a, uint4& b) {
+  const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
+  auto two = [&](uint32_t v, uint32_t sel) { const uint32_t r = __byte_perm(v, 0x64646464u, sel); const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&r), off); return *reinterpret_cast<const uint32_t*>(&h); };
+  a = make_uint4(two(w.x, 0x4140), two(w.x, 0x4342), two(w.y, 0x4140), two(w.y, 0x4342));
+  b = make_uint4(two(w.z, 0x4140), two(w.z, 0x4342), two(w.w, 0x4140), two(w.w, 0x4342));
+}
+__device__ __forceinline__ void ctc_sts(uint32_t a, uint4 v) { asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
+__device__ __forceinline__ uint4 ctc_lds(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+__global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP p, const __grid_constant__ CUtensorMap mapQ) {
+  extern __shared__ unsigned char ctc_raw[];
+  const uint32_t base = (smem_u32(ctc_raw) + 1023u) & ~1023u;
+  unsigned char* gbase = ctc_raw + (base - smem_u32(ctc_raw));
+  const uint32_t q_sm = base, kv_sm = base + 2u * ATC_TILE, st_sm = kv_sm + CTC_SLOTS * ATC_TILE, bars = st_sm + CTC_STAGES * CTC_STAGE;
+  const uint32_t q_full = bars, q_empty = bars + 8u, st_full = bars + 16u, st_empty = st_full + 8u * CTC_STAGES, kv_full = st_empty + 8u * CTC_STAGES, kv_empty = kv_full + 8u * CTC_SLOTS;
+  const uint32_t s_full = kv_empty + 8u * CTC_SLOTS, p_full = s_full + 16u, o_full = p_full + 16u, tmem_slot = o_full + 16u;
+  float* xch = reinterpret_cast<float*>(gbase + (bars + 256u - base));
+  float2* scl = reinterpret_cast<float2*>(xch + 1024);                  // [tile][page of the pair] (K scale, V scale)
+  volatile uint32_t* at = reinterpret_cast<volatile uint32_t*>(scl + 2u * CTC_SCL);
+  const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
+  if (tid == 0) {
+    mbar_init(q_full, 1u); mbar_init(q_empty, 1u);
+    for (uint32_t s = 0; s < CTC_STAGES; s++) { mbar_init(st_full + 8u * s, 1u); mbar_init(st_empty + 8u * s, 4u); }
+    for (uint32_t s = 0; s < CTC_SLOTS; s++) { mbar_init(kv_full + 8u * s, 4u); mbar_init(kv_empty + 8u * s, 1u); }
+    for (uint32_t t = 0; t < 2u; t++) { mbar_init(s_full + 8u * t, 1u); mbar_init(p_full + 8u * t, 8u); mbar_init(o_full + 8u * t, 1u); }
+    fence_mbar_init();
+  }
+  if (warp == 1) { tmem_alloc(tmem_slot, 512u); tmem_relinquish(); }
+  tc_fence_before();
+  grid_dependency_wait();
+  grid_launch_dependents();
+  // ---- this block's share of the work: units per sequence, their sum, then where the share begins
+  {
+    uint64_t* per_seq = reinterpret_cast<uint64_t*>(gbase + (st_sm - base));
+    uint32_t items = 0u;
+    for (uint32_t b = warp; b < p.geo.seqs; b += CTC_THREADS / 32u) {
+      const CacheSeq s = cache_seq(p.c, b);
+      const uint32_t n = cache_tc_blocks(s, p.geo);
+      uint64_t u = 0u;
+      for (uint32_t x = lane; x < n; x += 32u) u += cache_tc_units(cache_tc_part(s, p.geo, x), p.geo);
+#pragma unroll
+      for (uint32_t o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+      items += n;
+      if (lane == 0u) per_seq[b] = u * p.geo.Hkv;
+    }
+    if (tid == 0) at[5] = 0u;
+    __syncthreads();
+    if (lane == 0u && items) atomicAdd(const_cast<uint32_t*>(at) + 5, items);
+    __syncthreads();
+    if (warp == 0u) {
+      auto scan = [&](uint64_t v) {
+#pragma unroll
+        for (uint32_t o = 1; o < 32u; o <<= 1) { const uint64_t w = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += w; }
+        return v;
+      };
+      uint64_t U = 0u;
+      for (uint32_t b = 0; b < p.geo.seqs; b += 32u) U += __shfl_sync(0xffffffffu, scan(b + lane < p.geo.seqs ? per_seq[b + lane] : 0u), 31);
+      const uint64_t G = cache_tc_workers(U, (uint64_t)at[5] * p.geo.Hkv, gridDim.x);
+      uint64_t u0 = 0u, u1 = 0u;
+      if (blockIdx.x < G) { u0 = deal_first(blockIdx.x, U, G); u1 = deal_first(blockIdx.x + 1u, U, G); }
+      if (lane == 0u) {
+        at[4] = (uint32_t)(u1 - u0);
+        at[6] = (uint32_t)U; at[7] = (uint32_t)(U >> 32); at[8] = (uint32_t)G; at[9] = (uint32_t)u0; at[10] = (uint32_t)(u0 >> 32);
+        p.desc[blockIdx.x].on = 0u;
+      }
+      if (u1 > u0) {
+        uint64_t r = u0;                                                  // units before ours, from here on within a sequence, then a block of queries
+        uint32_t b = 0u;
+        for (uint32_t b0 = 0; b0 < p.geo.seqs; b0 += 32u) {
+          const uint64_t mine = b0 + lane < p.geo.seqs ? per_seq[b0 + lane] : 0u, inc = scan(mine), all = __shfl_sync(0xffffffffu, inc, 31);
+          const uint32_t hit = __ballot_sync(0xffffffffu, inc > r);
+          if (hit) { const uint32_t l = __ffs(hit) - 1u; b = b0 + l; r -= __shfl_sync(0xffffffffu, inc - mine, l); break; }
+          r -= all;
+        }
+        const CacheSeq s = cache_seq(p.c, b);
+        const uint32_t n = cache_tc_blocks(s, p.geo);
+        for (uint32_t x0 = 0; x0 < n; x0 += 32u) {
+          const uint32_t u = x0 + lane < n ? cache_tc_units(cache_tc_part(s, p.geo, x0 + lane), p.geo) : 0u;
+          const uint64_t mine = (uint64_t)u * p.geo.Hkv, inc = scan(mine), all = __shfl_sync(0xffffffffu, inc, 31);
+          const uint32_t hit = __ballot_sync(0xffffffffu, inc > r);
+          if (hit) {
+            const uint32_t l = __ffs(hit) - 1u;
+            if (lane == l) { r -= inc - mine; at[0] = b; at[1] = x0 + l; at[2] = (uint32_t)(r / u); at[3] = (uint32_t)(r % u); }
+            break;
+          }
+          r -= all;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t*>(gbase + (tmem_slot - base)), 0);
+  CacheTcWalk w;
+  const auto seq = [&](uint32_t b) { return cache_seq(p.c, b); };
+  w.begin(p.geo, at[0], at[1], at[2], at[3], at[4], seq);
+
+  if (warp < 4u) {
+    regs_down<32>();
+    if (warp == 0u) {
+      // ================================================================= loads: lane l holds page and scales of the l-th of 32 visible pages
+      uint32_t i = 0u, tile = 0u, seg = 0u;
+      bool ok = true;
+      fence_proxy_async();                                                // (the staging ring held the unit counts)
+      for (; w.left && ok; w.next(p.geo, seq), seg++) {
+        if (seg > 0u) { if (!__all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1u) & 1u, p.c.status, 621, 100u))) { ok = false; break; } }
+        if (lane == 0u) {
+          const uint32_t nt = w.two(p.geo) ? 2u : 1u;
+          mbar_expect_tx(q_full, nt * 2u * p.geo.qpt * p.geo.group * 128u);
+          for (uint32_t t = 0; t < nt; t++)
+            for (uint32_t c = 0; c < 2u; c++) tma_load_4d(q_sm + t * ATC_TILE + c * 16384u, &mapQ, (int)(c * 64u), 0, (int)(w.part.r0 + t * p.geo.qpt), (int)w.hk, q_full);
+        }
+        uint32_t mine = 0u;
+        float2 xsc = make_float2(1.0f, 1.0f);
+        for (uint32_t j = 0; j < w.cnt && ok; j++, tile++) {
+          const uint32_t k0 = 2u * (w.t + j), l0 = (2u * j) & 31u;
+          if (l0 == 0u) {
+            const uint32_t k = k0 + lane;
+            xsc = make_float2(1.0f, 1.0f);
+            mine = 0xffffffffu;                                           // no page, or the tail: nothing to load
+            if (k < w.v.np && cache_vis_page(w.v, k) < w.s.L / CACHE_PAGE) {
+              mine = ld_now(p.c.table + (size_t)w.b * p.c.max_pages + cache_vis_page(w.v, k));
+              if (mine >= p.c.pages) { cache_tell(p.c.status, CACHE_BAD_PAGE); mine = 0u; }
+              xsc = ld_now(p.c.scales + (size_t)mine * p.c.Hkv + w.hk);
+            }
+          }
+          const uint32_t pa = __shfl_sync(0xffffffffu, mine, l0), pb = __shfl_sync(0xffffffffu, mine, l0 + 1u);
+          for (uint32_t kind = 0; kind < 2u; kind++, i++) {
+            const uint32_t st = i % CTC_STAGES, use = i / CTC_STAGES, bar = st_full + 8u * st;
+            if (use > 0u && !__all_sync(0xffffffffu, mbar_wait(st_empty + 8u * st, (use - 1u) & 1u, p.c.status, 622, 50u))) { ok = false; break; }
+            if (kind == 0u && (lane == l0 || lane == l0 + 1u)) scl[(tile % CTC_SCL) * 2u + (lane - l0)] = xsc;
+            __syncwarp();
+            if (lane == 0u) {
+              const uint32_t n = (pa != 0xffffffffu ? 1u : 0u) + (pb != 0xffffffffu ? 1u : 0u), dst = st_sm + st * CTC_STAGE;
+              if (n) {
+                mbar_expect_tx(bar, n * CACHE_BLOCK);
+                if (pa != 0xffffffffu) bulk_g2s(dst, p.c.codes + (((size_t)pa * p.c.Hkv + w.hk) * 2u + kind) * CACHE_BLOCK, CACHE_BLOCK, bar);
+                if (pb != 0xffffffffu) bulk_g2s(dst + CACHE_BLOCK, p.c.codes + (((size_t)pb * p.c.Hkv + w.hk) * 2u + kind) * CACHE_BLOCK, CACHE_BLOCK, bar);
+              } else mbar_arrive(bar);
+            }
+          }
+        }
+      }
+    } else if (warp == 1u) {
+      // ================================================================= multiplies (the whole warp walks the loop, one lane issues)
+      const uint32_t idesc = umma_idesc_f16(128u, 128u);
+      const uint64_t qd[2] = {umma_desc_sw128(q_sm), umma_desc_sw128(q_sm + ATC_TILE)};
+      uint32_t i = 0u, seg = 0u, np[2] = {0u, 0u};                        // ring steps, items, weights consumed per tile of rows
+      bool ok = true;
+      for (; w.left && ok; w.next(p.geo, seq), seg++) {
+        const uint32_t nt = w.two(p.geo) ? 2u : 1u;
+        ok = __all_sync(0xffffffffu, mbar_wait(q_full, seg & 1u, p.c.status, 623) && mbar_wait(kv_full + 8u * (i % CTC_SLOTS), (i / CTC_SLOTS) & 1u, p.c.status, 624));
+        if (!ok) break;
+        tc_fence_after();
+        {
+          const uint64_t kd = umma_desc_sw128(kv_sm + (i % CTC_SLOTS) * ATC_TILE);
+          if (elect_one()) {
+            for (uint32_t t = 0; t < nt; t++) {
+#pragma unroll
+              for (uint32_t kk = 0; kk < 8u; kk++) umma_f16_ss(tmem_base + t * 128u, qd[t] + (kk >> 2) * 1024u + 2u * (kk & 3u), kd + (kk >> 2) * 1024u + 2u * (kk & 3u), idesc, kk);
+              umma_commit(s_full + 8u * t);
+            }
+            umma_commit(kv_empty + 8u * (i % CTC_SLOTS));
+            if (w.cnt == 1u) umma_commit(q_empty);
+          }
+          __syncwarp();
+        }
+        for (uint32_t j = 0; j < w.cnt && ok; j++, i += 2u) {
+          const uint32_t iv = i + 1u, sv = iv % CTC_SLOTS, ik = i + 2u, sk = ik % CTC_SLOTS;
+          const bool more = j + 1u < w.cnt;
+          bool rdy = mbar_wait(kv_full + 8u * sv, (iv / CTC_SLOTS) & 1u, p.c.status, 625);
+          if (more) rdy = rdy && mbar_wait(kv_full + 8u * sk, (ik / CTC_SLOTS) & 1u, p.c.status, 626);
+          if (!__all_sync(0xffffffffu, rdy)) { ok = false; break; }
+          const uint64_t vd = umma_desc_sw128(kv_sm + sv * ATC_TILE), kd = umma_desc_sw128(kv_sm + sk * ATC_TILE);
+          for (uint32_t t = 0; t < nt; t++) {
+            if (!__all_sync(0xffffffffu, mbar_spin(p_full + 8u * t, np[t] & 1u, p.c.status, 627))) { ok = false; break; }
+            np[t]++;
+            tc_fence_after();
+            const uint32_t s_col = tmem_base + t * 128u, o_col = tmem_base + 256u + t * 128u;
+            const uint64_t qdt = qd[t];
+            if (elect_one()) {
+#pragma unroll
+              for (uint32_t kk = 0; kk < 8u; kk++) umma_f16_ts(o_col, s_col + 8u * kk, vd + (kk >> 2) * 1024u + 2u * (kk & 3u), idesc, j | kk);
+              if (more) {
+#pragma unroll
+                for (uint32_t kk = 0; kk < 8u; kk++) umma_f16_ss(s_col, qdt + (kk >> 2) * 1024u + 2u * (kk & 3u), kd + (kk >> 2) * 1024u + 2u * (kk & 3u), idesc, kk);
+                umma_commit(s_full + 8u * t);
+              } else
+                umma_commit(o_full + 8u * t);
+            }
+            __syncwarp();
+          }
+          if (ok && elect_one()) {
+            umma_commit(kv_empty + 8u * sv);
+            if (more) umma_commit(kv_empty + 8u * sk);
+            if (j + 2u == w.cnt) umma_commit(q_empty);                    // the item's last scores are under way
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else if (warp < 8u) {
+    // ================================================================= codes (or the tail's fp16) -> fp16 tiles
+    regs_down<32>();
+    const uint32_t ct = tid - 128u;
+    uint32_t i = 0u;
+    bool ok = true;
+    for (; w.left && ok; w.next(p.geo, seq)) {
+      for (uint32_t j = 0; j < w.cnt && ok; j++) {
+        for (uint32_t kind = 0; kind < 2u; kind++, i++) {
+          const uint32_t st = i % CTC_STAGES, slot = i % CTC_SLOTS, src = st_sm + st * CTC_STAGE, dst = kv_sm + slot * ATC_TILE;
+          if (!mbar_wait(st_full + 8u * st, (i / CTC_STAGES) & 1u, p.c.status, 628)) ok = false;
+          if (i >= CTC_SLOTS && ok && !mbar_wait(kv_empty + 8u * slot, (i / CTC_SLOTS - 1u) & 1u, p.c.status, 629)) ok = false;
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          for (uint32_t half = 0; half < 2u; half++) {
+            const uint32_t k = 2u * (w.t + j) + half, page = cache_vis_page(w.v, k), full = w.s.L / CACHE_PAGE;
+            const uint32_t what = k >= w.v.np ? 2u : page < full ? 0u : 1u;      // a page of codes, the tail, nothing
+            const uint4* tl = reinterpret_cast<const uint4*>(p.c.tail + (((size_t)w.b * p.c.Hkv + w.hk) * 2u + kind) * CACHE_BLOCK);
+#pragma unroll 1
+            for (uint32_t it = 0; it < 4u; it++) {
+              const uint32_t u = it * 128u + ct;
+              uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+              if (what == 0u) ctc_convert(ctc_lds(src + half * CACHE_BLOCK + u * 16u), a, b);
+              else if (what == 1u) {
+                a = ld_now(tl + 2u * u); b = ld_now(tl + 2u * u + 1u);
+                if (kind) {                                               // keys behind the sequence's end may hold anything: they weigh nothing, but 0 * NaN would count
+                  const int have = (int)(w.s.L - page * CACHE_PAGE) - (int)(4u * (u & 3u));
+                  auto keep = [&](uint32_t v, int at) { return have >= at + 2 ? v : have == at + 1 ? v & 0xffffu : 0u; };
+                  a.x = keep(a.x, 0); a.y = keep(a.y, 2); a.z = keep(a.z, 16); a.w = keep(a.w, 18);
+                  b.x = keep(b.x, 32); b.y = keep(b.y, 34); b.z = keep(b.z, 48); b.w = keep(b.w, 50);
+                }
+              }
+              uint32_t row, sub, ch;                                      // 128-byte row, 16-KB half of the tile, first 16-byte piece
+              if (kind == 0u) {
+                row = half * 64u + ((u >> 3) & 3u) * 16u + (u >> 7) * 4u + ((u >> 6) & 1u) * 2u + ((u >> 2) & 1u); sub = (u >> 5) & 1u;
+              } else { row = u >> 2; sub = half; }
+              ch = 2u * (u & 3u);
+              const uint32_t to = dst + sub * 16384u + row * 128u, x = row & 7u;
+              ctc_sts(to + ((ch ^ x) << 4), a);
+              ctc_sts(to + (((ch + 1u) ^ x) << 4), b);
+            }
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0u) { mbar_arrive(kv_full + 8u * slot); mbar_arrive(st_empty + 8u * st); }
+        }
+      }
+    }
+  } else {
+    // ================================================================= softmax of one tile: two threads per row, one page of a pair each
+    regs_up<104>();
+    const uint32_t t = (warp - 8u) >> 3, half = ((warp - 8u) >> 2) & 1u, row = (warp & 3u) * 32u + lane;
+    const uint32_t lane_addr = tmem_base + (((warp & 3u) * 32u) << 16), s_addr = lane_addr + t * 128u + half * 64u, p_addr = lane_addr + t * 128u + half * 32u;
+    const uint32_t o_addr = lane_addr + 256u + t * 128u + half * 64u, pair_bar = 1u + t * 4u + (warp & 3u);
+    float* mine = xch + (t * 2u + half) * 128u + row; const float* other = xch + (t * 2u + (half ^ 1u)) * 128u + row;
+    const uint32_t qi = row / p.geo.group, hh = row - qi * p.geo.group;
+    uint32_t n = 0u, tile = 0u, seg = 0u, xp = 0u;                        // this tile's scores so far, the block's key tiles and items, parity of the exchange
+    bool ok = true;
+    uint64_t u = (uint64_t)at[9] | (uint64_t)at[10] << 32;
+    for (; w.left; u += w.cnt, w.next(p.geo, seq)) {
+      if (t == 1u && !w.two(p.geo)) { tile += w.cnt; continue; }
+      const uint32_t q = t * p.geo.qpt + qi;                              // the row's query within the block
+      const bool live = qi < p.geo.qpt && q < w.part.n;
+      const uint32_t p0 = w.part.L - w.part.n, pos = p0 + min(q, w.part.n - 1u);
+      float m_used = -INFINITY, l = 0.0f;
+      for (uint32_t j = 0; j < w.cnt; j++, n++, tile++) {
+        // (a wait that ran out: the thread goes on without it, so that its partner is not left at the barrier; the status word is set)
+        if (ok && !mbar_spin(s_full + 8u * t, n & 1u, p.c.status, 630)) ok = false;
+        tc_fence_after();
+        uint32_t s[64];
+#pragma unroll
+        for (int c = 0; c < 4; c++) tmem_ld16(s_addr + 16u * c, *reinterpret_cast<uint32_t(*)[16]>(&s[16 * c]));
+        const float2 ks = scl[(tile % CTC_SCL) * 2u + half];
+        const float sc = p.scale_log2 * ks.x;
+        float lv;
+        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lv) : "f"(ks.y));
+        const uint32_t k = 2u * (w.t + j) + half, page = cache_vis_page(w.v, k);
+        tmem_ld_wait();
+        if (k >= w.v.np || cache_page_masked(page, p0, w.part.L - 1u, p.geo.window, p.geo.sinks)) {
+          // columns whose key is visible: at most hi, and at least lo or below sk (all relative to the page)
+          const int k0 = (int)(page * CACHE_PAGE);
+          const int hi = k >= w.v.np ? -1 : (int)min(pos - min(pos, (uint32_t)k0), 64u) - (pos < (uint32_t)k0 ? 1 : 0);
+          int lo = 0, sk = 0;
+          if (p.geo.window && pos >= p.geo.window) {
+            const uint32_t first = pos - p.geo.window + 1u;
+            lo = (int)min(first - min(first, (uint32_t)k0), 64u); sk = (int)min(p.geo.sinks - min(p.geo.sinks, (uint32_t)k0), 64u);
+          }
+#pragma unroll
+          for (int c = 0; c < 64; c++) {
+            const int key = (int)cache_col_key(c);
+            s[c] = key <= hi && (key >= lo || key < sk) ? s[c] : 0xff800000u;
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          mx[0] = fmaxf(mx[0], __uint_as_float(s[c])); mx[1] = fmaxf(mx[1], __uint_as_float(s[c + 1]));
+          mx[2] = fmaxf(mx[2], __uint_as_float(s[c + 2])); mx[3] = fmaxf(mx[3], __uint_as_float(s[c + 3]));
+        }
+        float mts = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sc, lv);
+        mine[xp * 512u] = mts;
+        tc_fence_before();                   // this warp's reads of S end before its partner writes P over columns 32..63 of them
+        bar_sync_named((int)pair_bar, 64);
+        tc_fence_after();
+        mts = fmaxf(mts, other[xp * 512u]);
+        xp ^= 1u;
+        if (__any_sync(0xffffffffu, mts > m_used + 8.0f || (m_used == -INFINITY && mts > -INFINITY))) {
+          const float m_new = fmaxf(m_used, mts);
+          const float alpha = m_new == -INFINITY ? 1.0f : atc_ex2(m_used - m_new);
+          l *= alpha;
+          if (j > 0u) {
+#pragma unroll 1
+            for (uint32_t c = 0; c < 4u; c++) {
+              uint32_t o[16];
+              tmem_ld16(o_addr + 16u * c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st16(o_addr + 16u * c, o);
+            }
+          }
+          m_used = m_new;
+        }
+        float2 ls[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        const float nm = m_used == -INFINITY ? 0.0f : lv - m_used;       // (a row that has seen no key yet: all its weights are 0)
+        const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[32 * c + 2 * e]), __uint_as_float(s[32 * c + 2 * e + 1])), sc2, nm2);
+            float2 pr;
+            if ((e * ATC_EMU) % 16 < ATC_EMU) pr = atc_ex2_poly2(x);
+            else pr = make_float2(atc_ex2(x.x), atc_ex2(x.y));
+            ls[e & 1] = __fadd2_rn(ls[e & 1], pr);
+            const __half2 hp = __floats2half2_rn(pr.x, pr.y);
+            pk[e] = *reinterpret_cast<const uint32_t*>(&hp);
+          }
+          tmem_st16(p_addr + 16u * c, pk);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 8u * t);
+        l = fmaf((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y), __fdividef(1.0f, ks.y), l);
+      }
+      mine[xp * 512u] = l;
+      bar_sync_named((int)pair_bar, 64);
+      l += other[xp * 512u];
+      xp ^= 1u;
+      // ---- the item's end: O / l, or this block's partial result
+      if (ok && !mbar_wait(o_full + 8u * t, seg & 1u, p.c.status, 631)) ok = false;
+      seg++;
+      tc_fence_after();
+      const bool whole = w.t == 0u && w.cnt == w.units;
+      const uint32_t slot = w.t > 0u ? 0u : 1u;
+      const float inv = l > 0.0f ? 1.0f / l : l;
+      __half* dst = p.O + (size_t)(w.part.r0 + q) * p.ldo + (size_t)(w.hk * p.geo.group + hh) * 128u + half * 64u;
+      const bool vec = ((reinterpret_cast<uintptr_t>(p.O) | ((uintptr_t)p.ldo * 2u)) & 15u) == 0u;
+      float4* pt = p.part + ((size_t)(blockIdx.x * 2u + slot) * 32u + half * 16u) * 256u + t * 128u + row;
+#pragma unroll 1
+      for (uint32_t c = 0; c < 4u; c++) {
+        uint32_t o[16];
+        tmem_ld16(o_addr + 16u * c, o);
+        tmem_ld_wait();
+        if (!live || !ok) continue;
+        if (whole) {
+          uint32_t v[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const __half2 hp = __floats2half2_rn(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            v[e] = *reinterpret_cast<const uint32_t*>(&hp);
+          }
+          if (vec) {
+            *reinterpret_cast<uint4*>(dst + 16u * c) = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(dst + 16u * c + 8u) = make_uint4(v[4], v[5], v[6], v[7]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) *reinterpret_cast<uint32_t*>(dst + 16u * c + 2 * e) = v[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) pt[(4u * c + e) * 256u] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+        }
+      }
+      tc_fence_before();                     // (the reads of O end before the next item's weights are handed over)
+      if (!whole) {
+        if (half == 0u) p.part_ml[(size_t)(blockIdx.x * 2u + slot) * 256u + t * 128u + row] = make_float2(m_used, l);
+        if (slot == 1u && t == 0u && half == 0u && row == 0u) {
+          const uint64_t U = (uint64_t)at[6] | (uint64_t)at[7] << 32;
+          p.desc[blockIdx.x] = CacheTcDesc{1u, w.part.r0, w.part.n, w.hk, (uint32_t)deal_owner(u + w.units - 1u, U, at[8])};
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1u) { tc_fence_after(); tmem_dealloc(tmem_base, 512u); }
+}
+
+// ---- items that cross blocks: (maximum, sum, O) of their blocks added up in block order.  A block takes 32 rows of one item's 256.
+struct CacheMergeP {
+  const float4* part; const float2* part_ml; const CacheTcDesc* desc;
+  __half* O;
+  uint32_t ldo, group, qpt;
+};
+__global__ void __launch_bounds__(256) k_cache_merge(const CacheMergeP p) {
+  __shared__ float tile[32][132];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const uint32_t c0 = blockIdx.x, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, row = blockIdx.y * 32u + lane;
+  const CacheTcDesc d = p.desc[c0];
+  if (!d.on) return;
+  auto live = [&](uint32_t r) { const uint32_t x = r & 127u, q = (r >> 7) * p.qpt + x / p.group; return x < p.qpt * p.group && q < d.q; };
+  if (__syncthreads_or(live(row)) == 0) return;
+  auto slab = [&](uint32_t c) { return (size_t)c * 2u + (c == c0 ? 1u : 0u); };
+  float M = -INFINITY;
+  if (live(row)) for (uint32_t c = c0; c <= d.c1; c++) M = fmaxf(M, p.part_ml[slab(c) * 256u + row].x);
+  float L = 0.0f;
+  float4 acc[4];
+#pragma unroll
+  for (int k = 0; k < 4; k++) acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (live(row)) {
+#pragma unroll 2
+    for (uint32_t c = c0; c <= d.c1; c++) {
+      const float2 ml = p.part_ml[slab(c) * 256u + row];
+      const float f = ml.x == -INFINITY ? 0.0f : atc_ex2(ml.x - M);
+      L = fmaf(f, ml.y, L);
+#pragma unroll
+      for (uint32_t k = 0; k < 4u; k++) {
+        const float4 v = p.part[(slab(c) * 32u + warp + 8u * k) * 256u + row];
+        acc[k].x = fmaf(f, v.x, acc[k].x); acc[k].y = fmaf(f, v.y, acc[k].y); acc[k].z = fmaf(f, v.z, acc[k].z); acc[k].w = fmaf(f, v.w, acc[k].w);
+      }
+    }
+  }
+  const float inv = L > 0.0f ? 1.0f / L : L;
+#pragma unroll
+  for (uint32_t k = 0; k < 4u; k++) *reinterpret_cast<float4*>(&tile[lane][(warp + 8u * k) * 4u]) = make_float4(acc[k].x * inv, acc[k].y * inv, acc[k].z * inv, acc[k].w * inv);
+  __syncthreads();
+#pragma unroll
+  for (uint32_t k = 0; k < 4u; k++) {
+    const uint32_t r = blockIdx.y * 32u + warp * 4u + k;
+    if (!live(r)) continue;
+    const uint32_t x = r & 127u, q = (r >> 7) * p.qpt + x / p.group, h = d.hk * p.group + x % p.group;
+    const float4 v = *reinterpret_cast<const float4*>(&tile[r & 31u][lane * 4u]);
+    __half2* o = reinterpret_cast<__half2*>(p.O + (size_t)(d.row0 + q) * p.ldo + h * 128u + 4u * lane);
+    o[0] = __floats2half2_rn(v.x, v.y); o[1] = __floats2half2_rn(v.z, v.w);
+  }
+}
+
+}  // namespace p0p

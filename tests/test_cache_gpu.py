@@ -254,12 +254,30 @@ def _att_cache(P, gpu, c):
     return cache
 
 
-@pytest.mark.parametrize("c", ATT, ids=lambda c: c["label"])
-def test_attention(gpu, c):
+PROMPTS = [
+    dict(label="a block of queries exactly", Hkv=1, group=4, lens=[64], news=[64]),
+    dict(label="one query more than a tile", Hkv=2, group=4, lens=[33], news=[33]),
+    dict(label="an odd number of pages, history that ends in one", Hkv=2, group=4, lens=[700], news=[130]),
+    dict(label="few queries over a long context: items that cross many blocks", Hkv=2, group=4, lens=[20000], news=[70]),
+    dict(label="a long prompt: blocks with several items", Hkv=4, group=4, lens=[1500], news=[1500]),
+    dict(label="groups that do not divide a tile", Hkv=2, group=7, lens=[600, 300], news=[200, 300]),
+    dict(label="one head per kv head", Hkv=5, group=1, lens=[1000], news=[400]),
+    dict(label="many heads per kv head", Hkv=1, group=100, lens=[200], news=[70]),
+    dict(label="128 heads per kv head", Hkv=1, group=128, lens=[300], news=[3]),
+    dict(label="long window over long contexts", Hkv=2, group=4, lens=[9000, 4000], news=[300, 1000], window=700, sinks=70),
+    dict(label="wide scores: the maximum moves by more than the lazy threshold", Hkv=2, group=4, lens=[2000], news=[200], qstd=6.0),
+    dict(label="steps and prompts in one batch", Hkv=2, group=4, lens=[5000, 300, 2000, 64, 900], news=[1, 300, 2, 64, 500], extra=1),
+]
+
+
+@pytest.mark.parametrize("kernel", [None, "split", "tmem"])
+@pytest.mark.parametrize("c", ATT + PROMPTS, ids=lambda c: c["label"])
+def test_attention(gpu, c, kernel):
     import p0pc0rn_kernels_b200 as P
     cache = _att_cache(P, gpu, c)
     try:
         kw = {k: c[k] for k in ("window", "sinks", "scale", "qstd", "extra", "ldo") if k in c}
+        kw["kernel"] = kernel
         for _ in range(2): _check(cache, c["news"], c["group"], **kw)                          # (twice: a counter left over would show)
         if len(set(c["news"])) == 1: _check(cache, c["news"], c["group"], rows=False, new=c["news"][0], **{k: v for k, v in kw.items() if k != "extra"})
     finally:
@@ -275,8 +293,10 @@ def test_attention_scales_far_apart(gpu):
     v[:, :64] *= 2.0 ** -14; v[:, 64:128] = 0; v[:, 128:192] *= 2.0 ** 6; k[:, 192:256] *= 2.0 ** -10; k[0, 256:320] = 0; v[1, 300, :] = 60000.0
     try:
         cache.write([400], [k.astype(np.float16)], [v.astype(np.float16)], rows=False)
-        _check(cache, [2], 4)
-        _check(cache, [2], 4, window=330)
+        for kernel in ("split", "tmem"):
+            _check(cache, [2], 4, kernel=kernel)
+            _check(cache, [2], 4, window=330, kernel=kernel)
+            _check(cache, [200], 4, window=330, kernel=kernel)
     finally:
         cache.free()
 
@@ -286,7 +306,7 @@ def test_attention_nan_query_stays_in_its_row(gpu):
     cache = Cache(P, gpu, 2, 2, 10)
     cache.fill([500, 200])
     try:
-        for kernel in (None, "split"):
+        for kernel in ("split", "tmem"):
             out, q, offs = _attend(cache, [3, 2], 4, nan_row=(5, 1), kernel=kernel)
             bad = np.zeros(out.shape[:2], bool); bad[1, 5] = True
             assert np.isnan(out[bad]).all() and np.isfinite(out[~bad]).all()
@@ -303,10 +323,11 @@ def test_attention_of_a_later_token_does_not_reach_back(gpu):
     v[0, 69] = np.inf; k[0, 69] = np.nan
     try:
         cache.write([70], [k], [v], rows=False)
-        out, q, offs = _attend(cache, [4], 2)
-        want = _attn_want(q[0][:, :3], *(x[:, :69] for x in cache.held(0)), 0, 0)
-        top = np.abs(v[0, :69].astype(np.float64)).max()
-        assert np.abs(out[:3] - want).max() <= top * (2 * (2.0 ** -11 + 1e-4) + 2.0 ** -11 + 70 * 2.0 ** -25)
+        for kernel in ("split", "tmem"):
+            out, q, offs = _attend(cache, [4], 2, kernel=kernel)
+            want = _attn_want(q[0][:, :3], *(x[:, :69] for x in cache.held(0)), 0, 0)
+            top = np.abs(v[0, :69].astype(np.float64)).max()
+            assert np.abs(out[:3] - want).max() <= top * (2 * (2.0 ** -11 + 1e-4) + 2.0 ** -11 + 70 * 2.0 ** -25)
     finally:
         cache.free()
 
@@ -480,6 +501,7 @@ def test_refusals(gpu):
             no(op, a, "rows needs", rows={"buf": gpu.bufs and b, "off": (1 << 20) - 8})
         no(P.cacheWrite, kv, "k needs", M=3000); no(P.cacheWrite, kv, "v.ld", v={"buf": b, "ld": 5}); no(P.cacheWrite, kv, "multiple of 16", k={"buf": b, "off": 4})
         no(P.cacheAttention, at, "multiple of Hkv", Hq=3); no(P.cacheAttention, at, "o needs", o={"buf": b, "ld": 1 << 18}); no(P.cacheAttention, at, "o.ld", o={"buf": b, "ld": 511})
+        no(P.cacheAttention, dict(at, Hq=2 * 130), "128 heads", kernel="tmem", q={"buf": b}, o={"buf": b})
         no(P.cacheAttention, at, "finite", scale=float("nan")); no(P.cacheAttention, at, "q needs", M=3000)
         no(P.rope, ro, "even", rot=7); no(P.rope, ro, "even", rot=130); no(P.rope, ro, "unknown mode", mode="x"); no(P.rope, ro, "positive", theta=-1.0); no(P.rope, ro, "fast above slow", fast=1.0, slow=2.0)
         no(P.rope, ro, "multiple of seqs", M=7); no(P.rope, ro, "x needs", M=3000); no(P.rope, ro, "sequences", seqs=0); no(P.rope, ro, "multiple of 16", x={"buf": b, "off": 2})

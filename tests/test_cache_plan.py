@@ -104,6 +104,48 @@ int main() {
       }
     }
   }
+  {   // score columns: every key of a page once, in the order of a lane's V elements
+    std::vector<int> seen(64, 0);
+    for (uint32_t c = 0; c < 64; c++) { seen[cache_col_key(c)]++; CHECK(cache_v_off(cache_col_key(c), 0) == c); }
+    for (int x : seen) CHECK(x == 1);
+  }
+  for (int it = 0; it < 1500; it++) {   // the tensor-memory kernel's units: every block's walk
+    const uint32_t seqs = 1 + rnd(rnd(2) ? 3 : 40), group = 1 + rnd(rnd(2) ? 8 : 128);
+    const CacheTcGeo g{1 + rnd(5), group, seqs, rnd(2) ? 1 + rnd(300) : 0, rnd(70), 128 / group, rnd(2) ? rnd(100) : 0};
+    std::vector<CacheSeq> seq(seqs);
+    struct Unit { uint32_t b, x, hk, t, units; };
+    std::vector<Unit> all;
+    uint64_t items = 0;
+    for (uint32_t b = 0; b < seqs; b++) {
+      seq[b] = CacheSeq{0, rnd(3) ? rnd(3) : rnd(200), 0};
+      seq[b].L = seq[b].n + rnd(900);
+      if ((uint64_t)seq[b].n * group <= g.min_rows) continue;
+      for (uint32_t q0 = 0, x = 0; q0 < seq[b].n; q0 += 2 * g.qpt, x++) {
+        const CacheSeq part = cache_tc_part(seq[b], g, x);
+        CHECK(part.r0 == seq[b].r0 + q0 && part.n == (seq[b].n - q0 < 2 * g.qpt ? seq[b].n - q0 : 2 * g.qpt) && part.L - part.n == seq[b].L - seq[b].n + q0);
+        const uint32_t np = cache_visible(part, g.window, g.sinks).np;
+        CHECK(cache_tc_units(part, g) == (np + 1) / 2 && (part.n <= g.qpt || part.n * group <= 2 * 128));
+        for (uint32_t h = 0; h < g.Hkv; h++) { items++; for (uint32_t t = 0; t < (np + 1) / 2; t++) all.push_back({b, x, h, t, (np + 1) / 2}); }
+      }
+    }
+    const uint64_t U = all.size();
+    if (!U) continue;
+    const uint64_t G = cache_tc_workers(U, items, 148);
+    CHECK(G >= 1 && G <= U && G <= 148);
+    const auto get = [&](uint32_t b) { CHECK(b < seqs); return seq[b]; };
+    for (uint64_t c = 0; c < G; c++) {
+      const uint64_t u0 = deal_first(c, U, G), u1 = deal_first(c + 1, U, G);
+      uint64_t u = u0;
+      CacheTcWalk w;
+      for (w.begin(g, all[u].b, all[u].x, all[u].hk, all[u].t, (uint32_t)(u1 - u0), get); w.left; u += w.cnt, w.next(g, get)) {
+        CHECK(w.cnt > 0 && u + w.cnt <= u1 && w.t + w.cnt <= w.units);
+        for (uint32_t k = 0; k < w.cnt; k++) CHECK(all[u + k].b == w.b && all[u + k].x == w.x && all[u + k].hk == w.hk && all[u + k].t == w.t + k && all[u + k].units == w.units);
+        if (w.t + w.cnt < w.units) CHECK(u + w.cnt == u1);
+        CHECK(deal_owner(u, U, G) == c && deal_owner(u + w.cnt - 1, U, G) == c);
+      }
+      CHECK(u == u1);
+    }
+  }
   {   // refusals
     char msg[256];
     CacheShape ok{8, 10, 4, 5, 10 * 8 * 16384, 10 * 8 * 8, 4 * 8 * 32768, 4 * 5 * 4, 16, 0, 0, 0, 0, 0};
