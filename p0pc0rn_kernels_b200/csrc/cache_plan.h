@@ -135,42 +135,54 @@ P0P_HD CacheSeq cache_tc_part(const CacheSeq& s, const CacheTcGeo& g, uint32_t x
 P0P_HD uint32_t cache_tc_units(const CacheSeq& part, const CacheTcGeo& g) { return (cache_visible(part, g.window, g.sinks).np + 1u) / 2u; }
 // the key of column c of a page's 64 score columns (the order in which a lane's V elements lie)
 P0P_HD constexpr uint32_t cache_col_key(uint32_t c) { return 16u * ((c >> 2) & 3u) + 4u * (c >> 4) + (c & 3u); }
-// What a block does next: units [t, t + cnt) of an item.  Every role of the block walks the same list by itself.  get(b): sequence b.
+// The work is dealt out by cost: an item costs CACHE_TC_ITEM units (its queries arrive, its result leaves, the pipeline fills) and then its own.
+// (Dealt out by units alone, a block at the start of a prompt, with many items of one unit or two, took 1.7 times as long as the others.)
+constexpr uint32_t CACHE_TC_ITEM = 2u;
+P0P_HD uint32_t cache_tc_cost(const CacheSeq& part, const CacheTcGeo& g) { return CACHE_TC_ITEM + cache_tc_units(part, g); }
+// What a block does next: units [t, t + cnt) of an item; cnt 0: nothing more.  Every role of the block walks the same list by itself.  get(b): sequence b.
 struct CacheTcWalk {
   CacheSeq s, part; CacheVis v;
-  uint32_t b, x, hk, t, units, cnt, left;
+  uint32_t b, x, blocks, hk, t, units, cnt, left, spent;      // spent: the cost, from the beginning of the block's share, of unit t
   P0P_HD void item(const CacheTcGeo& g) {
     part = cache_tc_part(s, g, x);
     v = cache_visible(part, g.window, g.sinks);
     units = (v.np + 1u) / 2u;
   }
+  // the share begins `at` into item (b_, x_, hk_) and costs left_
   template <class Get>
-  P0P_HD void begin(const CacheTcGeo& g, uint32_t b_, uint32_t x_, uint32_t hk_, uint32_t t_, uint32_t left_, Get get) {
-    b = b_; x = x_; hk = hk_; t = t_; left = left_; cnt = 0u;
+  P0P_HD void begin(const CacheTcGeo& g, uint32_t b_, uint32_t x_, uint32_t hk_, uint32_t at, uint32_t left_, Get get) {
+    b = b_; x = x_; hk = hk_; left = left_; cnt = 0u; spent = 0u; t = 0u;
     if (!left) return;
     s = get(b);
+    blocks = cache_tc_blocks(s, g);
     item(g);
-    cnt = units - t < left ? units - t : left;
+    if (at < CACHE_TC_ITEM) enter(CACHE_TC_ITEM - at);
+    else { t = at - CACHE_TC_ITEM; cnt = units - t < left ? units - t : left; }
+  }
+  P0P_HD void enter(uint32_t first) {
+    if (left <= first) { left = 0u; cnt = 0u; return; }
+    left -= first; spent += first;
+    cnt = units < left ? units : left;
   }
   template <class Get>
   P0P_HD void next(const CacheTcGeo& g, Get get) {
-    left -= cnt; t = 0u; cnt = 0u;
+    left -= cnt; spent += cnt; t = 0u; cnt = 0u;
     if (!left) return;
     if (++hk == g.Hkv) {
       hk = 0u;
-      if (++x == cache_tc_blocks(s, g)) {
+      if (++x == blocks) {
         x = 0u;
-        do { b++; s = get(b); } while (b + 1u < g.seqs && cache_tc_blocks(s, g) == 0u);
+        do { b++; s = get(b); blocks = cache_tc_blocks(s, g); } while (b + 1u < g.seqs && blocks == 0u);
       }
       item(g);
     }
-    cnt = units < left ? units : left;
+    enter(CACHE_TC_ITEM);
   }
   P0P_HD bool two(const CacheTcGeo& g) const { return part.n > g.qpt; }      // both tiles of rows hold queries
 };
-// how many blocks share U units: at least four units each, but no fewer blocks than items
+// how many blocks share a cost of U: six each at least, but no fewer blocks than items
 P0P_HD uint64_t cache_tc_workers(uint64_t U, uint64_t items, uint64_t most) {
-  uint64_t g = U / 4u > items ? U / 4u : items;
+  uint64_t g = U / 6u > items ? U / 6u : items;
   if (g > most) g = most;
   return g > U ? U : g;
 }

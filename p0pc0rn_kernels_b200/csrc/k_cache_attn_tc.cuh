@@ -35,9 +35,17 @@ struct CacheTcP {
 };
 
 constexpr uint32_t CTC_THREADS = 768u, CTC_SLOTS = 3u, CTC_STAGES = 3u, CTC_STAGE = 2u * CACHE_BLOCK;
+// of every 16 pairs of scores, how many take their exponential on the FMA pipe: with the conversion in the same issue slots fewer than in k_attn_tc
+// (2000 tokens over 6100, four prompts under a window: 6 260, 148 us; 5 258, 146.8; 4 256, 146.2)
+constexpr int CTC_EMU = 4;
 constexpr int CTC_REGS = 16 * 104 + 8 * 32;      // registers per lane of all warps, after setmaxnreg
-constexpr uint32_t CTC_SCL = 8u;       // tiles whose scales are kept: the loads are at most three tiles ahead of the softmax
-constexpr uint32_t CTC_SMEM = 1024u + (2u + CTC_SLOTS) * ATC_TILE + CTC_STAGES * CTC_STAGE + 256u + 4096u + CTC_SCL * 16u + 64u;
+constexpr uint32_t CTC_SCL = 8u;       // tiles whose pages are described: the loads are at most three tiles ahead of the softmax
+constexpr uint32_t CTC_SEGS = 4u;      // items that the loads may be ahead of the slowest reader
+// an item's share as the loads announce it
+struct CtcSeg { uint32_t cnt, t, units, r0, n, L, hk, b, seq_L, spent; };
+// what a page of a tile means for the softmax: scale_log2 * K scale, log2 and reciprocal of the V scale, its first key | 1 where some key is hidden from some row
+struct CtcPage { float f, lv, inv_v; uint32_t key0; };
+constexpr uint32_t CTC_SMEM = 1024u + (2u + CTC_SLOTS) * ATC_TILE + CTC_STAGES * CTC_STAGE + 256u + 4096u + CTC_SCL * 2u * (uint32_t)sizeof(CtcPage) + CTC_SEGS * (uint32_t)sizeof(CtcSeg) + 64u;
 static_assert(CTC_SMEM <= 232448u, "shared memory");
 static_assert(CTC_STAGES * CTC_STAGE >= CACHE_MAX_SEQS * 8u, "the sequences' unit counts fit the staging ring while nothing is in it");
 
@@ -58,29 +66,39 @@ __device__ __forceinline__ uint4 ctc_lds(uint32_t a) {
   return v;
 }
 
+// a named barrier of 64 threads at which all learn whether all are fine
+__device__ __forceinline__ bool ctc_agree(int bar, bool fine) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.and.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"(bar), "r"(fine ? 1u : 0u) : "memory");
+  return r != 0u;
+}
+
 __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP p, const __grid_constant__ CUtensorMap mapQ) {
   extern __shared__ unsigned char ctc_raw[];
   const uint32_t base = (smem_u32(ctc_raw) + 1023u) & ~1023u;
   unsigned char* gbase = ctc_raw + (base - smem_u32(ctc_raw));
   const uint32_t q_sm = base, kv_sm = base + 2u * ATC_TILE, st_sm = kv_sm + CTC_SLOTS * ATC_TILE, bars = st_sm + CTC_STAGES * CTC_STAGE;
   const uint32_t q_full = bars, q_empty = bars + 8u, st_full = bars + 16u, st_empty = st_full + 8u * CTC_STAGES, kv_full = st_empty + 8u * CTC_STAGES, kv_empty = kv_full + 8u * CTC_SLOTS;
-  const uint32_t s_full = kv_empty + 8u * CTC_SLOTS, p_full = s_full + 16u, o_full = p_full + 16u, tmem_slot = o_full + 16u;
+  const uint32_t s_full = kv_empty + 8u * CTC_SLOTS, p_full = s_full + 16u, o_full = p_full + 16u, seg_full = o_full + 16u, seg_empty = seg_full + 8u * CTC_SEGS, tmem_slot = seg_empty + 8u * CTC_SEGS;
   float* xch = reinterpret_cast<float*>(gbase + (bars + 256u - base));
-  float2* scl = reinterpret_cast<float2*>(xch + 1024);                  // [tile][page of the pair] (K scale, V scale)
-  volatile uint32_t* at = reinterpret_cast<volatile uint32_t*>(scl + 2u * CTC_SCL);
+  CtcPage* scl = reinterpret_cast<CtcPage*>(xch + 1024);                // [tile][page of the pair]
+  volatile CtcSeg* segs = reinterpret_cast<volatile CtcSeg*>(scl + 2u * CTC_SCL);
+  volatile uint32_t* at = reinterpret_cast<volatile uint32_t*>(const_cast<CtcSeg*>(segs) + CTC_SEGS);
+  volatile uint32_t* what = at + 12;                                    // [stage] what its two pages are: codes 0, the tail 1, nothing 2 (the second << 2)
   const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
   if (tid == 0) {
     mbar_init(q_full, 1u); mbar_init(q_empty, 1u);
     for (uint32_t s = 0; s < CTC_STAGES; s++) { mbar_init(st_full + 8u * s, 1u); mbar_init(st_empty + 8u * s, 4u); }
     for (uint32_t s = 0; s < CTC_SLOTS; s++) { mbar_init(kv_full + 8u * s, 4u); mbar_init(kv_empty + 8u * s, 1u); }
     for (uint32_t t = 0; t < 2u; t++) { mbar_init(s_full + 8u * t, 1u); mbar_init(p_full + 8u * t, 8u); mbar_init(o_full + 8u * t, 1u); }
+    for (uint32_t s = 0; s < CTC_SEGS; s++) { mbar_init(seg_full + 8u * s, 1u); mbar_init(seg_empty + 8u * s, 21u); }
     fence_mbar_init();
   }
   if (warp == 1) { tmem_alloc(tmem_slot, 512u); tmem_relinquish(); }
   tc_fence_before();
   grid_dependency_wait();
   grid_launch_dependents();
-  // ---- this block's share of the work: units per sequence, their sum, then where the share begins
+  // ---- this block's share of the work: cost per sequence, their sum, then where the share begins
   {
     uint64_t* per_seq = reinterpret_cast<uint64_t*>(gbase + (st_sm - base));
     uint32_t items = 0u;
@@ -88,7 +106,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
       const CacheSeq s = cache_seq(p.c, b);
       const uint32_t n = cache_tc_blocks(s, p.geo);
       uint64_t u = 0u;
-      for (uint32_t x = lane; x < n; x += 32u) u += cache_tc_units(cache_tc_part(s, p.geo, x), p.geo);
+      for (uint32_t x = lane; x < n; x += 32u) u += cache_tc_cost(cache_tc_part(s, p.geo, x), p.geo);
 #pragma unroll
       for (uint32_t o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
       items += n;
@@ -115,7 +133,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
         p.desc[blockIdx.x].on = 0u;
       }
       if (u1 > u0) {
-        uint64_t r = u0;                                                  // units before ours, from here on within a sequence, then a block of queries
+        uint64_t r = u0;                                                  // cost before ours, from here on within a sequence, then a block of queries
         uint32_t b = 0u;
         for (uint32_t b0 = 0; b0 < p.geo.seqs; b0 += 32u) {
           const uint64_t mine = b0 + lane < p.geo.seqs ? per_seq[b0 + lane] : 0u, inc = scan(mine), all = __shfl_sync(0xffffffffu, inc, 31);
@@ -126,7 +144,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
         const CacheSeq s = cache_seq(p.c, b);
         const uint32_t n = cache_tc_blocks(s, p.geo);
         for (uint32_t x0 = 0; x0 < n; x0 += 32u) {
-          const uint32_t u = x0 + lane < n ? cache_tc_units(cache_tc_part(s, p.geo, x0 + lane), p.geo) : 0u;
+          const uint32_t u = x0 + lane < n ? cache_tc_cost(cache_tc_part(s, p.geo, x0 + lane), p.geo) : 0u;
           const uint64_t mine = (uint64_t)u * p.geo.Hkv, inc = scan(mine), all = __shfl_sync(0xffffffffu, inc, 31);
           const uint32_t hit = __ballot_sync(0xffffffffu, inc > r);
           if (hit) {
@@ -142,55 +160,77 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t*>(gbase + (tmem_slot - base)), 0);
-  CacheTcWalk w;
-  const auto seq = [&](uint32_t b) { return cache_seq(p.c, b); };
-  w.begin(p.geo, at[0], at[1], at[2], at[3], at[4], seq);
+  // an item's share, to the other roles: they wait for it here and give it back when they are done with it (every warp of them)
+  auto seg_wait = [&](uint32_t seg) { return mbar_wait(seg_full + 8u * (seg % CTC_SEGS), (seg / CTC_SEGS) & 1u, p.c.status, 620, 50u); };
+  auto seg_done = [&](uint32_t seg) { __syncwarp(); if (lane == 0u) mbar_arrive(seg_empty + 8u * (seg % CTC_SEGS)); };
 
   if (warp < 4u) {
     regs_down<32>();
     if (warp == 0u) {
-      // ================================================================= loads: lane l holds page and scales of the l-th of 32 visible pages
+      // ================================================================= loads: lane l looks after the l-th of 32 visible pages
       uint32_t i = 0u, tile = 0u, seg = 0u;
       bool ok = true;
-      fence_proxy_async();                                                // (the staging ring held the unit counts)
-      for (; w.left && ok; w.next(p.geo, seq), seg++) {
-        if (seg > 0u) { if (!__all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1u) & 1u, p.c.status, 621, 100u))) { ok = false; break; } }
+      fence_proxy_async();                                                // (the staging ring held the costs)
+      CacheTcWalk w;
+      const auto seq = [&](uint32_t b) { return cache_seq(p.c, b); };
+      w.begin(p.geo, at[0], at[1], at[2], at[3], at[4], seq);
+      for (;; w.next(p.geo, seq), seg++) {
+        if (seg >= CTC_SEGS && !__all_sync(0xffffffffu, mbar_wait(seg_empty + 8u * (seg % CTC_SEGS), (seg / CTC_SEGS - 1u) & 1u, p.c.status, 632, 50u))) break;
+        if (lane == 0u) {
+          volatile CtcSeg& g = segs[seg % CTC_SEGS];
+          g.cnt = w.cnt; g.t = w.t; g.units = w.units; g.r0 = w.part.r0; g.n = w.part.n; g.L = w.part.L; g.hk = w.hk; g.b = w.b; g.seq_L = w.s.L; g.spent = w.spent;
+          mbar_arrive(seg_full + 8u * (seg % CTC_SEGS));
+        }
+        __syncwarp();
+        if (!w.cnt) break;
+        if (seg > 0u && !__all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1u) & 1u, p.c.status, 621, 50u))) break;
         if (lane == 0u) {
           const uint32_t nt = w.two(p.geo) ? 2u : 1u;
           mbar_expect_tx(q_full, nt * 2u * p.geo.qpt * p.geo.group * 128u);
           for (uint32_t t = 0; t < nt; t++)
             for (uint32_t c = 0; c < 2u; c++) tma_load_4d(q_sm + t * ATC_TILE + c * 16384u, &mapQ, (int)(c * 64u), 0, (int)(w.part.r0 + t * p.geo.qpt), (int)w.hk, q_full);
         }
-        uint32_t mine = 0u;
-        float2 xsc = make_float2(1.0f, 1.0f);
+        uint32_t mine = 0u, kind_of = 2u;
+        CtcPage pg{1.0f, 0.0f, 1.0f, 0xffffffffu};
         for (uint32_t j = 0; j < w.cnt && ok; j++, tile++) {
-          const uint32_t k0 = 2u * (w.t + j), l0 = (2u * j) & 31u;
+          const uint32_t l0 = (2u * j) & 31u;
           if (l0 == 0u) {
-            const uint32_t k = k0 + lane;
-            xsc = make_float2(1.0f, 1.0f);
-            mine = 0xffffffffu;                                           // no page, or the tail: nothing to load
-            if (k < w.v.np && cache_vis_page(w.v, k) < w.s.L / CACHE_PAGE) {
-              mine = ld_now(p.c.table + (size_t)w.b * p.c.max_pages + cache_vis_page(w.v, k));
-              if (mine >= p.c.pages) { cache_tell(p.c.status, CACHE_BAD_PAGE); mine = 0u; }
-              xsc = ld_now(p.c.scales + (size_t)mine * p.c.Hkv + w.hk);
+            const uint32_t k = 2u * (w.t + j) + lane, page = cache_vis_page(w.v, k);
+            pg = CtcPage{1.0f, 0.0f, 1.0f, 0xffffffffu};                  // no page: every key hidden
+            mine = 0u; kind_of = 2u;
+            if (k < w.v.np) {
+              float2 sc = make_float2(1.0f, 1.0f);
+              kind_of = 1u;
+              if (page < w.s.L / CACHE_PAGE) {
+                kind_of = 0u;
+                mine = ld_now(p.c.table + (size_t)w.b * p.c.max_pages + page);
+                if (mine >= p.c.pages) { cache_tell(p.c.status, CACHE_BAD_PAGE); mine = 0u; }
+                sc = ld_now(p.c.scales + (size_t)mine * p.c.Hkv + w.hk);
+              }
+              pg.f = p.scale_log2 * sc.x; pg.inv_v = __fdividef(1.0f, sc.y);
+              asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(pg.lv) : "f"(sc.y));
+              pg.key0 = page * CACHE_PAGE | (cache_page_masked(page, w.part.L - w.part.n, w.part.L - 1u, p.geo.window, p.geo.sinks) ? 1u : 0u);
             }
           }
           const uint32_t pa = __shfl_sync(0xffffffffu, mine, l0), pb = __shfl_sync(0xffffffffu, mine, l0 + 1u);
+          const uint32_t ka = __shfl_sync(0xffffffffu, kind_of, l0), kb = __shfl_sync(0xffffffffu, kind_of, l0 + 1u);
           for (uint32_t kind = 0; kind < 2u; kind++, i++) {
             const uint32_t st = i % CTC_STAGES, use = i / CTC_STAGES, bar = st_full + 8u * st;
             if (use > 0u && !__all_sync(0xffffffffu, mbar_wait(st_empty + 8u * st, (use - 1u) & 1u, p.c.status, 622, 50u))) { ok = false; break; }
-            if (kind == 0u && (lane == l0 || lane == l0 + 1u)) scl[(tile % CTC_SCL) * 2u + (lane - l0)] = xsc;
+            if (kind == 0u && (lane == l0 || lane == l0 + 1u)) scl[(tile % CTC_SCL) * 2u + (lane - l0)] = pg;
             __syncwarp();
             if (lane == 0u) {
-              const uint32_t n = (pa != 0xffffffffu ? 1u : 0u) + (pb != 0xffffffffu ? 1u : 0u), dst = st_sm + st * CTC_STAGE;
+              const uint32_t n = (ka == 0u ? 1u : 0u) + (kb == 0u ? 1u : 0u), dst = st_sm + st * CTC_STAGE;
+              what[st] = ka | kb << 2;
               if (n) {
                 mbar_expect_tx(bar, n * CACHE_BLOCK);
-                if (pa != 0xffffffffu) bulk_g2s(dst, p.c.codes + (((size_t)pa * p.c.Hkv + w.hk) * 2u + kind) * CACHE_BLOCK, CACHE_BLOCK, bar);
-                if (pb != 0xffffffffu) bulk_g2s(dst + CACHE_BLOCK, p.c.codes + (((size_t)pb * p.c.Hkv + w.hk) * 2u + kind) * CACHE_BLOCK, CACHE_BLOCK, bar);
+                if (ka == 0u) bulk_g2s(dst, p.c.codes + (((size_t)pa * p.c.Hkv + w.hk) * 2u + kind) * CACHE_BLOCK, CACHE_BLOCK, bar);
+                if (kb == 0u) bulk_g2s(dst + CACHE_BLOCK, p.c.codes + (((size_t)pb * p.c.Hkv + w.hk) * 2u + kind) * CACHE_BLOCK, CACHE_BLOCK, bar);
               } else mbar_arrive(bar);
             }
           }
         }
+        if (!ok) break;
       }
     } else if (warp == 1u) {
       // ================================================================= multiplies (the whole warp walks the loop, one lane issues)
@@ -198,8 +238,11 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
       const uint64_t qd[2] = {umma_desc_sw128(q_sm), umma_desc_sw128(q_sm + ATC_TILE)};
       uint32_t i = 0u, seg = 0u, np[2] = {0u, 0u};                        // ring steps, items, weights consumed per tile of rows
       bool ok = true;
-      for (; w.left && ok; w.next(p.geo, seq), seg++) {
-        const uint32_t nt = w.two(p.geo) ? 2u : 1u;
+      for (; ok; seg++) {
+        if (!__all_sync(0xffffffffu, seg_wait(seg))) break;
+        const uint32_t cnt = segs[seg % CTC_SEGS].cnt, nt = segs[seg % CTC_SEGS].n > p.geo.qpt ? 2u : 1u;
+        seg_done(seg);
+        if (!cnt) break;
         ok = __all_sync(0xffffffffu, mbar_wait(q_full, seg & 1u, p.c.status, 623) && mbar_wait(kv_full + 8u * (i % CTC_SLOTS), (i / CTC_SLOTS) & 1u, p.c.status, 624));
         if (!ok) break;
         tc_fence_after();
@@ -212,19 +255,19 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
               umma_commit(s_full + 8u * t);
             }
             umma_commit(kv_empty + 8u * (i % CTC_SLOTS));
-            if (w.cnt == 1u) umma_commit(q_empty);
+            if (cnt == 1u) umma_commit(q_empty);
           }
           __syncwarp();
         }
-        for (uint32_t j = 0; j < w.cnt && ok; j++, i += 2u) {
+        for (uint32_t j = 0; j < cnt && ok; j++, i += 2u) {
           const uint32_t iv = i + 1u, sv = iv % CTC_SLOTS, ik = i + 2u, sk = ik % CTC_SLOTS;
-          const bool more = j + 1u < w.cnt;
+          const bool more = j + 1u < cnt;
           bool rdy = mbar_wait(kv_full + 8u * sv, (iv / CTC_SLOTS) & 1u, p.c.status, 625);
           if (more) rdy = rdy && mbar_wait(kv_full + 8u * sk, (ik / CTC_SLOTS) & 1u, p.c.status, 626);
           if (!__all_sync(0xffffffffu, rdy)) { ok = false; break; }
           const uint64_t vd = umma_desc_sw128(kv_sm + sv * ATC_TILE), kd = umma_desc_sw128(kv_sm + sk * ATC_TILE);
           for (uint32_t t = 0; t < nt; t++) {
-            if (!__all_sync(0xffffffffu, mbar_spin(p_full + 8u * t, np[t] & 1u, p.c.status, 627))) { ok = false; break; }
+                        if (!__all_sync(0xffffffffu, mbar_wait(p_full + 8u * t, np[t] & 1u, p.c.status, 627))) { ok = false; break; }
             np[t]++;
             tc_fence_after();
             const uint32_t s_col = tmem_base + t * 128u, o_col = tmem_base + 256u + t * 128u;
@@ -244,7 +287,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
           if (ok && elect_one()) {
             umma_commit(kv_empty + 8u * sv);
             if (more) umma_commit(kv_empty + 8u * sk);
-            if (j + 2u == w.cnt) umma_commit(q_empty);                    // the item's last scores are under way
+            if (j + 2u == cnt) umma_commit(q_empty);                    // the item's last scores are under way
           }
           __syncwarp();
         }
@@ -253,42 +296,64 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
   } else if (warp < 8u) {
     // ================================================================= codes (or the tail's fp16) -> fp16 tiles
     regs_down<32>();
-    const uint32_t ct = tid - 128u;
+    // unit u = 128 e + ct of a page's 512 (16 elements each): its 32 bytes go to row r of the tile's half h, pieces 2 (u % 4) and the next, swizzled
+    //   K: r = 64 page + 16 (u / 8 % 4) + 4 e + 2 (u / 64 % 2) + u / 4 % 2 (the key's column), h = u / 32 % 2 (which 64 of d);   V: r = u / 4 (d), h = page
+    const uint32_t ct = tid - 128u, ch = 2u * (ct & 3u), kx = ((ct >> 6) & 1u) * 2u + ((ct >> 2) & 1u), vx = (ct >> 2) & 7u;
+    const uint32_t k_to = ((ct >> 5) & 1u) * 16384u + (((ct >> 3) & 3u) * 16u + kx) * 128u, v_to = (ct >> 2) * 128u;
+    const uint32_t k_c0 = (ch ^ kx) << 4, k_c1 = ((ch + 1u) ^ kx) << 4, v_c0 = (ch ^ vx) << 4, v_c1 = ((ch + 1u) ^ vx) << 4;
     uint32_t i = 0u;
     bool ok = true;
-    for (; w.left && ok; w.next(p.geo, seq)) {
-      for (uint32_t j = 0; j < w.cnt && ok; j++) {
+    for (uint32_t seg = 0u; ok; seg++) {
+      if (!__all_sync(0xffffffffu, seg_wait(seg))) break;
+      const uint32_t cnt = segs[seg % CTC_SEGS].cnt;
+      if (!cnt) { seg_done(seg); break; }
+      for (uint32_t j = 0; j < cnt && ok; j++) {
         for (uint32_t kind = 0; kind < 2u; kind++, i++) {
           const uint32_t st = i % CTC_STAGES, slot = i % CTC_SLOTS, src = st_sm + st * CTC_STAGE, dst = kv_sm + slot * ATC_TILE;
           if (!mbar_wait(st_full + 8u * st, (i / CTC_STAGES) & 1u, p.c.status, 628)) ok = false;
           if (i >= CTC_SLOTS && ok && !mbar_wait(kv_empty + 8u * slot, (i / CTC_SLOTS - 1u) & 1u, p.c.status, 629)) ok = false;
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          for (uint32_t half = 0; half < 2u; half++) {
-            const uint32_t k = 2u * (w.t + j) + half, page = cache_vis_page(w.v, k), full = w.s.L / CACHE_PAGE;
-            const uint32_t what = k >= w.v.np ? 2u : page < full ? 0u : 1u;      // a page of codes, the tail, nothing
-            const uint4* tl = reinterpret_cast<const uint4*>(p.c.tail + (((size_t)w.b * p.c.Hkv + w.hk) * 2u + kind) * CACHE_BLOCK);
+          const uint32_t pages = what[st];
+          if (pages == 0u) {
+            if (kind == 0u) {
+#pragma unroll
+              for (uint32_t e = 0; e < 8u; e++) {                         // (4 rows further: the other value of the swizzle's upper bit)
+                uint4 a, b;
+                ctc_convert(ctc_lds(src + ct * 16u + e * 2048u), a, b);
+                const uint32_t to = dst + k_to + (e >> 2) * 8192u + (e & 3u) * 512u;
+                ctc_sts(to + (k_c0 ^ ((e & 1u) << 6)), a);
+                ctc_sts(to + (k_c1 ^ ((e & 1u) << 6)), b);
+              }
+            } else {
+#pragma unroll
+              for (uint32_t e = 0; e < 8u; e++) {
+                uint4 a, b;
+                ctc_convert(ctc_lds(src + ct * 16u + e * 2048u), a, b);
+                const uint32_t to = dst + v_to + (e >> 2) * 16384u + (e & 3u) * 4096u;
+                ctc_sts(to + v_c0, a);
+                ctc_sts(to + v_c1, b);
+              }
+            }
+          } else {
 #pragma unroll 1
-            for (uint32_t it = 0; it < 4u; it++) {
-              const uint32_t u = it * 128u + ct;
+            for (uint32_t e = 0; e < 8u; e++) {
+              const uint32_t half = e >> 2, u = (e & 3u) * 128u + ct, is = (pages >> (2u * half)) & 3u;
               uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
-              if (what == 0u) ctc_convert(ctc_lds(src + half * CACHE_BLOCK + u * 16u), a, b);
-              else if (what == 1u) {
+              if (is == 0u) ctc_convert(ctc_lds(src + ct * 16u + e * 2048u), a, b);
+              else if (is == 1u) {
+                volatile CtcSeg& g = segs[seg % CTC_SEGS];
+                const uint4* tl = reinterpret_cast<const uint4*>(p.c.tail + (((size_t)g.b * p.c.Hkv + g.hk) * 2u + kind) * CACHE_BLOCK);
                 a = ld_now(tl + 2u * u); b = ld_now(tl + 2u * u + 1u);
                 if (kind) {                                               // keys behind the sequence's end may hold anything: they weigh nothing, but 0 * NaN would count
-                  const int have = (int)(w.s.L - page * CACHE_PAGE) - (int)(4u * (u & 3u));
+                  const int have = (int)(g.seq_L & (CACHE_PAGE - 1u)) - (int)(4u * (u & 3u));
                   auto keep = [&](uint32_t v, int at) { return have >= at + 2 ? v : have == at + 1 ? v & 0xffffu : 0u; };
                   a.x = keep(a.x, 0); a.y = keep(a.y, 2); a.z = keep(a.z, 16); a.w = keep(a.w, 18);
                   b.x = keep(b.x, 32); b.y = keep(b.y, 34); b.z = keep(b.z, 48); b.w = keep(b.w, 50);
                 }
               }
-              uint32_t row, sub, ch;                                      // 128-byte row, 16-KB half of the tile, first 16-byte piece
-              if (kind == 0u) {
-                row = half * 64u + ((u >> 3) & 3u) * 16u + (u >> 7) * 4u + ((u >> 6) & 1u) * 2u + ((u >> 2) & 1u); sub = (u >> 5) & 1u;
-              } else { row = u >> 2; sub = half; }
-              ch = 2u * (u & 3u);
-              const uint32_t to = dst + sub * 16384u + row * 128u, x = row & 7u;
-              ctc_sts(to + ((ch ^ x) << 4), a);
-              ctc_sts(to + (((ch + 1u) ^ x) << 4), b);
+              const uint32_t flip = kind ? 0u : (e & 1u) << 6, to = dst + (kind ? v_to + half * 16384u + (e & 3u) * 4096u : k_to + half * 8192u + (e & 3u) * 512u);
+              ctc_sts(to + ((kind ? v_c0 : k_c0) ^ flip), a);
+              ctc_sts(to + ((kind ? v_c1 : k_c1) ^ flip), b);
             }
           }
           fence_proxy_async();
@@ -296,6 +361,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
           if (lane == 0u) { mbar_arrive(kv_full + 8u * slot); mbar_arrive(st_empty + 8u * st); }
         }
       }
+      seg_done(seg);
     }
   } else {
     // ================================================================= softmax of one tile: two threads per row, one page of a pair each
@@ -305,36 +371,35 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
     const uint32_t o_addr = lane_addr + 256u + t * 128u + half * 64u, pair_bar = 1u + t * 4u + (warp & 3u);
     float* mine = xch + (t * 2u + half) * 128u + row; const float* other = xch + (t * 2u + (half ^ 1u)) * 128u + row;
     const uint32_t qi = row / p.geo.group, hh = row - qi * p.geo.group;
-    uint32_t n = 0u, tile = 0u, seg = 0u, xp = 0u;                        // this tile's scores so far, the block's key tiles and items, parity of the exchange
+    uint32_t n = 0u, tile = 0u, items = 0u, xp = 0u;                      // this tile's scores and items so far, the block's key tiles, parity of the exchange
     bool ok = true;
-    uint64_t u = (uint64_t)at[9] | (uint64_t)at[10] << 32;
-    for (; w.left; u += w.cnt, w.next(p.geo, seq)) {
-      if (t == 1u && !w.two(p.geo)) { tile += w.cnt; continue; }
-      const uint32_t q = t * p.geo.qpt + qi;                              // the row's query within the block
-      const bool live = qi < p.geo.qpt && q < w.part.n;
-      const uint32_t p0 = w.part.L - w.part.n, pos = p0 + min(q, w.part.n - 1u);
+    for (uint32_t seg = 0u;; seg++) {
+      if (ok && !seg_wait(seg)) ok = false;
+      volatile CtcSeg& g = segs[seg % CTC_SEGS];
+      ok = ctc_agree((int)pair_bar, ok);                                  // (the two warps of a row meet at barriers: both go on, or neither)
+      const uint32_t cnt = ok ? g.cnt : 0u;
+      if (!cnt) break;
+      if (t == 1u && g.n <= p.geo.qpt) { tile += cnt; seg_done(seg); continue; }
+      const uint32_t pos = g.L - g.n + min(t * p.geo.qpt + qi, g.n - 1u);
       float m_used = -INFINITY, l = 0.0f;
-      for (uint32_t j = 0; j < w.cnt; j++, n++, tile++) {
+      for (uint32_t j = 0; j < cnt; j++, n++, tile++) {
         // (a wait that ran out: the thread goes on without it, so that its partner is not left at the barrier; the status word is set)
-        if (ok && !mbar_spin(s_full + 8u * t, n & 1u, p.c.status, 630)) ok = false;
+                if (ok && !mbar_wait(s_full + 8u * t, n & 1u, p.c.status, 630)) ok = false;
         tc_fence_after();
         uint32_t s[64];
 #pragma unroll
         for (int c = 0; c < 4; c++) tmem_ld16(s_addr + 16u * c, *reinterpret_cast<uint32_t(*)[16]>(&s[16 * c]));
-        const float2 ks = scl[(tile % CTC_SCL) * 2u + half];
-        const float sc = p.scale_log2 * ks.x;
-        float lv;
-        asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lv) : "f"(ks.y));
-        const uint32_t k = 2u * (w.t + j) + half, page = cache_vis_page(w.v, k);
+        const CtcPage pg = scl[(tile % CTC_SCL) * 2u + half];
+        const float sc = pg.f, lv = pg.lv;
         tmem_ld_wait();
-        if (k >= w.v.np || cache_page_masked(page, p0, w.part.L - 1u, p.geo.window, p.geo.sinks)) {
+        if (pg.key0 & 1u) {
           // columns whose key is visible: at most hi, and at least lo or below sk (all relative to the page)
-          const int k0 = (int)(page * CACHE_PAGE);
-          const int hi = k >= w.v.np ? -1 : (int)min(pos - min(pos, (uint32_t)k0), 64u) - (pos < (uint32_t)k0 ? 1 : 0);
+          const uint32_t k0 = pg.key0 & ~1u;
+          const int hi = (int)min(pos - min(pos, k0), 64u) - (pos < k0 ? 1 : 0);
           int lo = 0, sk = 0;
           if (p.geo.window && pos >= p.geo.window) {
             const uint32_t first = pos - p.geo.window + 1u;
-            lo = (int)min(first - min(first, (uint32_t)k0), 64u); sk = (int)min(p.geo.sinks - min(p.geo.sinks, (uint32_t)k0), 64u);
+            lo = (int)min(first - min(first, k0), 64u); sk = (int)min(p.geo.sinks - min(p.geo.sinks, k0), 64u);
           }
 #pragma unroll
           for (int c = 0; c < 64; c++) {
@@ -344,9 +409,9 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          mx[0] = fmaxf(mx[0], __uint_as_float(s[c])); mx[1] = fmaxf(mx[1], __uint_as_float(s[c + 1]));
-          mx[2] = fmaxf(mx[2], __uint_as_float(s[c + 2])); mx[3] = fmaxf(mx[3], __uint_as_float(s[c + 3]));
+        for (int c = 0; c < 64; c += 8) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(s[c + 2 * e])), __uint_as_float(s[c + 2 * e + 1]));      // (one instruction: the maximum of three)
         }
         float mts = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sc, lv);
         mine[xp * 512u] = mts;
@@ -382,7 +447,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
           for (int e = 0; e < 16; e++) {
             const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[32 * c + 2 * e]), __uint_as_float(s[32 * c + 2 * e + 1])), sc2, nm2);
             float2 pr;
-            if ((e * ATC_EMU) % 16 < ATC_EMU) pr = atc_ex2_poly2(x);
+            if ((e * CTC_EMU) % 16 < CTC_EMU) pr = atc_ex2_poly2(x);
             else pr = make_float2(atc_ex2(x.x), atc_ex2(x.y));
             ls[e & 1] = __fadd2_rn(ls[e & 1], pr);
             const __half2 hp = __floats2half2_rn(pr.x, pr.y);
@@ -394,45 +459,68 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + 8u * t);
-        l = fmaf((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y), __fdividef(1.0f, ks.y), l);
+        l = fmaf((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y), pg.inv_v, l);
       }
       mine[xp * 512u] = l;
       bar_sync_named((int)pair_bar, 64);
       l += other[xp * 512u];
       xp ^= 1u;
       // ---- the item's end: O / l, or this block's partial result
-      if (ok && !mbar_wait(o_full + 8u * t, seg & 1u, p.c.status, 631)) ok = false;
-      seg++;
+      if (ok && !mbar_wait(o_full + 8u * t, items & 1u, p.c.status, 631)) ok = false;
+      items++;
       tc_fence_after();
-      const bool whole = w.t == 0u && w.cnt == w.units;
-      const uint32_t slot = w.t > 0u ? 0u : 1u;
+      const uint32_t q = t * p.geo.qpt + qi, gt = g.t;                    // the row's query within the block
+      const bool live = qi < p.geo.qpt && q < g.n, whole = gt == 0u && cnt == g.units;
+      const uint32_t slot = gt > 0u ? 0u : 1u;
       const float inv = l > 0.0f ? 1.0f / l : l;
-      __half* dst = p.O + (size_t)(w.part.r0 + q) * p.ldo + (size_t)(w.hk * p.geo.group + hh) * 128u + half * 64u;
+      const int64_t at_o = live && ok ? (int64_t)(g.r0 + q) * p.ldo + (g.hk * p.geo.group + hh) * 128u + half * 64u : -1;      // the row's half columns in O; -1: not stored
       const bool vec = ((reinterpret_cast<uintptr_t>(p.O) | ((uintptr_t)p.ldo * 2u)) & 15u) == 0u;
-      float4* pt = p.part + ((size_t)(blockIdx.x * 2u + slot) * 32u + half * 16u) * 256u + t * 128u + row;
 #pragma unroll 1
-      for (uint32_t c = 0; c < 4u; c++) {
-        uint32_t o[16];
-        tmem_ld16(o_addr + 16u * c, o);
+      for (uint32_t c = 0; c < 2u; c++) {                                 // 32 columns at a time
+        uint32_t o[32];
+        tmem_ld16(o_addr + 32u * c, *reinterpret_cast<uint32_t(*)[16]>(&o[0]));
+        tmem_ld16(o_addr + 32u * c + 16u, *reinterpret_cast<uint32_t(*)[16]>(&o[16]));
         tmem_ld_wait();
-        if (!live || !ok) continue;
-        if (whole) {
-          uint32_t v[8];
+        if (!whole) {
+          float4* pt = p.part + ((size_t)(blockIdx.x * 2u + slot) * 32u + half * 16u + 8u * c) * 256u + t * 128u + row;
+          if (at_o >= 0) {
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const __half2 hp = __floats2half2_rn(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-            v[e] = *reinterpret_cast<const uint32_t*>(&hp);
+            for (int e = 0; e < 8; e++) pt[e * 256] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
           }
-          if (vec) {
-            *reinterpret_cast<uint4*>(dst + 16u * c) = make_uint4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<uint4*>(dst + 16u * c + 8u) = make_uint4(v[4], v[5], v[6], v[7]);
-          } else {
+          continue;
+        }
+        uint32_t v[4][4];                                                 // four pieces of 8 columns
 #pragma unroll
-            for (int e = 0; e < 8; e++) *reinterpret_cast<uint32_t*>(dst + 16u * c + 2 * e) = v[e];
+        for (int e = 0; e < 16; e++) {
+          const __half2 hp = __floats2half2_rn(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+          v[e >> 2][e & 3] = *reinterpret_cast<const uint32_t*>(&hp);
+        }
+        if (!vec) {
+          if (at_o >= 0) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) *reinterpret_cast<uint32_t*>(p.O + at_o + 32u * c + 2 * e) = v[e >> 2][e & 3];
           }
-        } else {
+          continue;
+        }
+        // Four lanes swap pieces (a 4 x 4 transposition), so that a store writes 64 consecutive bytes of each of 8 rows: with a row per lane every
+        // store touched 32 lines, and nothing else got through to shared memory for 8000 cycles an item.
 #pragma unroll
-          for (int e = 0; e < 4; e++) pt[(4u * c + e) * 256u] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+        for (int x = 1; x < 4; x += x) {
+          const bool up = (lane & x) != 0u;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            if (i & x) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? v[i][e] : v[i + x][e], x);
+              if (up) v[i][e] = got; else v[i + x][e] = got;
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {                                     // this lane's piece of the row of lane r of the four
+          const int64_t to = __shfl_sync(0xffffffffu, at_o, (int)((lane & 28u) + r));
+          if (to >= 0) *reinterpret_cast<uint4*>(p.O + to + 32u * c + 8u * (lane & 3u)) = make_uint4(v[r][0], v[r][1], v[r][2], v[r][3]);
         }
       }
       tc_fence_before();                     // (the reads of O end before the next item's weights are handed over)
@@ -440,9 +528,11 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
         if (half == 0u) p.part_ml[(size_t)(blockIdx.x * 2u + slot) * 256u + t * 128u + row] = make_float2(m_used, l);
         if (slot == 1u && t == 0u && half == 0u && row == 0u) {
           const uint64_t U = (uint64_t)at[6] | (uint64_t)at[7] << 32;
-          p.desc[blockIdx.x] = CacheTcDesc{1u, w.part.r0, w.part.n, w.hk, (uint32_t)deal_owner(u + w.units - 1u, U, at[8])};
+          const uint64_t u0 = (uint64_t)at[9] | (uint64_t)at[10] << 32;
+          p.desc[blockIdx.x] = CacheTcDesc{1u, g.r0, g.n, g.hk, (uint32_t)deal_owner(u0 + g.spent + g.units - 1u, U, at[8])};
         }
       }
+      seg_done(seg);
     }
   }
   tc_fence_before();

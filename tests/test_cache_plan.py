@@ -113,9 +113,9 @@ int main() {
     const uint32_t seqs = 1 + rnd(rnd(2) ? 3 : 40), group = 1 + rnd(rnd(2) ? 8 : 128);
     const CacheTcGeo g{1 + rnd(5), group, seqs, rnd(2) ? 1 + rnd(300) : 0, rnd(70), 128 / group, rnd(2) ? rnd(100) : 0};
     std::vector<CacheSeq> seq(seqs);
-    struct Unit { uint32_t b, x, hk, t, units; };
-    std::vector<Unit> all;
-    uint64_t items = 0;
+    struct Cost { uint32_t b, x, hk, at, units; };
+    std::vector<Cost> all;
+    uint64_t items = 0, work = 0, done = 0;
     for (uint32_t b = 0; b < seqs; b++) {
       seq[b] = CacheSeq{0, rnd(3) ? rnd(3) : rnd(200), 0};
       seq[b].L = seq[b].n + rnd(900);
@@ -123,9 +123,9 @@ int main() {
       for (uint32_t q0 = 0, x = 0; q0 < seq[b].n; q0 += 2 * g.qpt, x++) {
         const CacheSeq part = cache_tc_part(seq[b], g, x);
         CHECK(part.r0 == seq[b].r0 + q0 && part.n == (seq[b].n - q0 < 2 * g.qpt ? seq[b].n - q0 : 2 * g.qpt) && part.L - part.n == seq[b].L - seq[b].n + q0);
-        const uint32_t np = cache_visible(part, g.window, g.sinks).np;
-        CHECK(cache_tc_units(part, g) == (np + 1) / 2 && (part.n <= g.qpt || part.n * group <= 2 * 128));
-        for (uint32_t h = 0; h < g.Hkv; h++) { items++; for (uint32_t t = 0; t < (np + 1) / 2; t++) all.push_back({b, x, h, t, (np + 1) / 2}); }
+        const uint32_t np = cache_visible(part, g.window, g.sinks).np, units = (np + 1) / 2;
+        CHECK(cache_tc_units(part, g) == units && cache_tc_cost(part, g) == CACHE_TC_ITEM + units && (part.n <= g.qpt || part.n * group <= 2 * 128));
+        for (uint32_t h = 0; h < g.Hkv; h++) { items++; work += units; for (uint32_t c = 0; c < CACHE_TC_ITEM + units; c++) all.push_back({b, x, h, c, units}); }
       }
     }
     const uint64_t U = all.size();
@@ -135,16 +135,19 @@ int main() {
     const auto get = [&](uint32_t b) { CHECK(b < seqs); return seq[b]; };
     for (uint64_t c = 0; c < G; c++) {
       const uint64_t u0 = deal_first(c, U, G), u1 = deal_first(c + 1, U, G);
-      uint64_t u = u0;
       CacheTcWalk w;
-      for (w.begin(g, all[u].b, all[u].x, all[u].hk, all[u].t, (uint32_t)(u1 - u0), get); w.left; u += w.cnt, w.next(g, get)) {
-        CHECK(w.cnt > 0 && u + w.cnt <= u1 && w.t + w.cnt <= w.units);
-        for (uint32_t k = 0; k < w.cnt; k++) CHECK(all[u + k].b == w.b && all[u + k].x == w.x && all[u + k].hk == w.hk && all[u + k].t == w.t + k && all[u + k].units == w.units);
-        if (w.t + w.cnt < w.units) CHECK(u + w.cnt == u1);
-        CHECK(deal_owner(u, U, G) == c && deal_owner(u + w.cnt - 1, U, G) == c);
+      for (w.begin(g, all[u0].b, all[u0].x, all[u0].hk, all[u0].at, (uint32_t)(u1 - u0), get); w.cnt; w.next(g, get)) {
+        const uint64_t u = u0 + w.spent;                  // the cost of unit t lies here
+        CHECK(u + w.cnt <= u1 && w.t + w.cnt <= w.units);
+        for (uint32_t k = 0; k < w.cnt; k++, done++) CHECK(all[u + k].b == w.b && all[u + k].x == w.x && all[u + k].hk == w.hk && all[u + k].at == CACHE_TC_ITEM + w.t + k && all[u + k].units == w.units);
+        if (w.t + w.cnt < w.units) {                      // goes on in the next block, which begins with it; the last block of it is the owner of its last unit
+          CHECK(u + w.cnt == u1);
+          CHECK(deal_owner(u + (w.units - 1 - w.t), U, G) > c);
+        }
+        if (w.t > 0) CHECK(u == u0);
       }
-      CHECK(u == u1);
     }
+    CHECK(done == work);
   }
   {   // refusals
     char msg[256];
