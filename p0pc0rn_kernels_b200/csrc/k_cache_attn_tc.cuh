@@ -2,8 +2,8 @@
 // and tensor memory are those of k_attn_tc.cuh (S = Q K^T, O += P V, two tiles of 128 rows that share every K / V tile, lane = row); what differs:
 //   rows    a tile's rows are the queries of ALL heads that share a kv head, query by query (row = query * group + head), so a page is read
 //           and converted once for them
-//   K, V    arrive as codes (bulk copies into a ring of 16-KB slots: K or V of two pages) and are turned into fp16 whole numbers - exact - by four
-//           warps, into the swizzled tiles that the multiplies read.  The cache's order makes a lane's 16 codes 32 consecutive bytes of a tile: for K 16 d of
+//   K, V    arrive as codes (bulk copies) and are turned into fp16 whole numbers - exact - by two
+//           warps for K and two for V, into the swizzled tiles that the multiplies read.  The cache's order makes a lane's 16 codes 32 consecutive bytes of a tile: for K 16 d of
 //           one key, for V 16 keys of one d (so V's tile is K-major).  The keys stand in the order of V's elements in both (cache_col_key).
 //   scales  a thread's 64 scores belong to one page: its K scale joins the softmax scale, its V scale the exponent (w = 2^(score + log2 vs - m),
 //           and the sum of the weights is weighted with 1 / vs), as in k_cache_attn.cuh
@@ -34,20 +34,24 @@ struct CacheTcP {
   CacheTcDesc* desc;     // [block]
 };
 
-constexpr uint32_t CTC_THREADS = 768u, CTC_SLOTS = 3u, CTC_STAGES = 3u, CTC_STAGE = 2u * CACHE_BLOCK;
+// Four slots of tiles: with three the K tile two pairs ahead takes the V tile's place, and its conversion waits for that product.  What is left of
+// shared memory holds one pair's codes: 4 KB of each page for each converting warp, which asks for the next ones itself as soon as it has read them (one
+// warp loading for all four, or a lane for each of the eight, came late: 4000 cycles from the last read to the next codes).
+constexpr uint32_t CTC_THREADS = 768u, CTC_SLOTS = 4u, CTC_STAGE = CACHE_BLOCK / 2u;
 // of every 16 pairs of scores, how many take their exponential on the FMA pipe: with the conversion in the same issue slots fewer than in k_attn_tc
 // (2000 tokens over 6100, four prompts under a window: 6 260, 148 us; 5 258, 146.8; 4 256, 146.2)
-constexpr int CTC_EMU = 4;
+constexpr int CTC_EMU = 2;
 constexpr int CTC_REGS = 16 * 104 + 8 * 32;      // registers per lane of all warps, after setmaxnreg
-constexpr uint32_t CTC_SCL = 8u;       // tiles whose pages are described: the loads are at most three tiles ahead of the softmax
-constexpr uint32_t CTC_SEGS = 4u;      // items that the loads may be ahead of the slowest reader
-// an item's share as the loads announce it
-struct CtcSeg { uint32_t cnt, t, units, r0, n, L, hk, b, seq_L, spent; };
-// what a page of a tile means for the softmax: scale_log2 * K scale, log2 and reciprocal of the V scale, its first key | 1 where some key is hidden from some row
-struct CtcPage { float f, lv, inv_v; uint32_t key0; };
-constexpr uint32_t CTC_SMEM = 1024u + (2u + CTC_SLOTS) * ATC_TILE + CTC_STAGES * CTC_STAGE + 256u + 4096u + CTC_SCL * 2u * (uint32_t)sizeof(CtcPage) + CTC_SEGS * (uint32_t)sizeof(CtcSeg) + 64u;
+constexpr uint32_t CTC_PAIRS = 4u;     // pairs of pages that are described ahead
+constexpr uint32_t CTC_SEGS = 4u;      // items that are announced ahead
+// an item's share
+struct CtcSeg { uint32_t cnt, t, units, r0, n, L, hk, spent; };
+// a page of a pair.  For the softmax: scale_log2 * K scale, log2 and reciprocal of the V scale, its first key | 1 where some key is hidden from some row.
+// For the conversion: what it is (codes 0, the tail 1 | its tokens << 8, nothing 2, the end of the work 3), and which block of codes or of the tail.
+struct CtcPage { float f, lv, inv_v; uint32_t key0, is, block, pad[2]; };
+constexpr uint32_t CTC_SMEM = (2u + CTC_SLOTS) * ATC_TILE + 8u * CTC_STAGE + 512u + 2048u + CTC_PAIRS * 2u * (uint32_t)sizeof(CtcPage) + CTC_SEGS * (uint32_t)sizeof(CtcSeg) + 64u;
 static_assert(CTC_SMEM <= 232448u, "shared memory");
-static_assert(CTC_STAGES * CTC_STAGE >= CACHE_MAX_SEQS * 8u, "the sequences' unit counts fit the staging ring while nothing is in it");
+static_assert(8u * CTC_STAGE >= CACHE_MAX_SEQS * 8u, "the sequences' costs fit the codes' place while nothing is in it");
 
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -74,24 +78,26 @@ __device__ __forceinline__ bool ctc_agree(int bar, bool fine) {
 }
 
 __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP p, const __grid_constant__ CUtensorMap mapQ) {
-  extern __shared__ unsigned char ctc_raw[];
-  const uint32_t base = (smem_u32(ctc_raw) + 1023u) & ~1023u;
-  unsigned char* gbase = ctc_raw + (base - smem_u32(ctc_raw));
-  const uint32_t q_sm = base, kv_sm = base + 2u * ATC_TILE, st_sm = kv_sm + CTC_SLOTS * ATC_TILE, bars = st_sm + CTC_STAGES * CTC_STAGE;
-  const uint32_t q_full = bars, q_empty = bars + 8u, st_full = bars + 16u, st_empty = st_full + 8u * CTC_STAGES, kv_full = st_empty + 8u * CTC_STAGES, kv_empty = kv_full + 8u * CTC_SLOTS;
-  const uint32_t s_full = kv_empty + 8u * CTC_SLOTS, p_full = s_full + 16u, o_full = p_full + 16u, seg_full = o_full + 16u, seg_empty = seg_full + 8u * CTC_SEGS, tmem_slot = seg_empty + 8u * CTC_SEGS;
-  float* xch = reinterpret_cast<float*>(gbase + (bars + 256u - base));
-  CtcPage* scl = reinterpret_cast<CtcPage*>(xch + 1024);                // [tile][page of the pair]
-  volatile CtcSeg* segs = reinterpret_cast<volatile CtcSeg*>(scl + 2u * CTC_SCL);
+  extern __shared__ __align__(1024) unsigned char ctc_raw[];             // (the swizzled tiles; there is no room to align them by hand, and no static shared memory before them)
+  const uint32_t base = smem_u32(ctc_raw);
+  unsigned char* gbase = ctc_raw;
+  if (base & 1023u) { cache_tell(p.c.status, 633); return; }
+  const uint32_t q_sm = base, kv_sm = base + 2u * ATC_TILE, st_sm = kv_sm + CTC_SLOTS * ATC_TILE, bars = st_sm + 8u * CTC_STAGE;
+  const uint32_t q_full = bars, q_empty = bars + 8u, st_full = bars + 16u, kv_full = st_full + 64u, kv_empty = kv_full + 8u * CTC_SLOTS, s_full = kv_empty + 8u * CTC_SLOTS, p_full = s_full + 16u;
+  const uint32_t o_full = p_full + 16u, seg_full = o_full + 16u, seg_empty = seg_full + 8u * CTC_SEGS, pair_full = seg_empty + 8u * CTC_SEGS, pair_empty = pair_full + 8u * CTC_PAIRS;
+  const uint32_t tmem_slot = pair_empty + 8u * CTC_PAIRS;
+  float* xch = reinterpret_cast<float*>(gbase + (bars + 512u - base));
+  CtcPage* scl = reinterpret_cast<CtcPage*>(xch + 512);                   // [pair][page of it]
+  volatile CtcSeg* segs = reinterpret_cast<volatile CtcSeg*>(scl + 2u * CTC_PAIRS);
   volatile uint32_t* at = reinterpret_cast<volatile uint32_t*>(const_cast<CtcSeg*>(segs) + CTC_SEGS);
-  volatile uint32_t* what = at + 12;                                    // [stage] what its two pages are: codes 0, the tail 1, nothing 2 (the second << 2)
   const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
   if (tid == 0) {
     mbar_init(q_full, 1u); mbar_init(q_empty, 1u);
-    for (uint32_t s = 0; s < CTC_STAGES; s++) { mbar_init(st_full + 8u * s, 1u); mbar_init(st_empty + 8u * s, 4u); }
-    for (uint32_t s = 0; s < CTC_SLOTS; s++) { mbar_init(kv_full + 8u * s, 4u); mbar_init(kv_empty + 8u * s, 1u); }
+    for (uint32_t s = 0; s < 8u; s++) mbar_init(st_full + 8u * s, 1u);
+    for (uint32_t s = 0; s < CTC_SLOTS; s++) { mbar_init(kv_full + 8u * s, 2u); mbar_init(kv_empty + 8u * s, 1u); }
     for (uint32_t t = 0; t < 2u; t++) { mbar_init(s_full + 8u * t, 1u); mbar_init(p_full + 8u * t, 8u); mbar_init(o_full + 8u * t, 1u); }
-    for (uint32_t s = 0; s < CTC_SEGS; s++) { mbar_init(seg_full + 8u * s, 1u); mbar_init(seg_empty + 8u * s, 21u); }
+    for (uint32_t s = 0; s < CTC_SEGS; s++) { mbar_init(seg_full + 8u * s, 1u); mbar_init(seg_empty + 8u * s, 18u); }      // (queries, multiplies, softmax)
+    for (uint32_t s = 0; s < CTC_PAIRS; s++) { mbar_init(pair_full + 8u * s, 1u); mbar_init(pair_empty + 8u * s, 1u); }
     fence_mbar_init();
   }
   if (warp == 1) { tmem_alloc(tmem_slot, 512u); tmem_relinquish(); }
@@ -167,76 +173,71 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
   if (warp < 4u) {
     regs_down<32>();
     if (warp == 0u) {
-      // ================================================================= loads: lane l looks after the l-th of 32 visible pages
-      uint32_t i = 0u, tile = 0u, seg = 0u;
-      bool ok = true;
-      fence_proxy_async();                                                // (the staging ring held the costs)
+      // ================================================================= the list of work: items, and page by page what the others need to know.  Lane l looks
+      // after the l-th of 32 visible pages
+      uint32_t pair = 0u, seg = 0u;
       CacheTcWalk w;
       const auto seq = [&](uint32_t b) { return cache_seq(p.c, b); };
       w.begin(p.geo, at[0], at[1], at[2], at[3], at[4], seq);
-      for (;; w.next(p.geo, seq), seg++) {
-        if (seg >= CTC_SEGS && !__all_sync(0xffffffffu, mbar_wait(seg_empty + 8u * (seg % CTC_SEGS), (seg / CTC_SEGS - 1u) & 1u, p.c.status, 632, 50u))) break;
+      bool ok = true;
+      for (; ok; w.next(p.geo, seq), seg++) {
+        if (seg >= CTC_SEGS) ok = __all_sync(0xffffffffu, mbar_wait(seg_empty + 8u * (seg % CTC_SEGS), (seg / CTC_SEGS - 1u) & 1u, p.c.status, 632, 50u));
+        if (!ok) break;
         if (lane == 0u) {
           volatile CtcSeg& g = segs[seg % CTC_SEGS];
-          g.cnt = w.cnt; g.t = w.t; g.units = w.units; g.r0 = w.part.r0; g.n = w.part.n; g.L = w.part.L; g.hk = w.hk; g.b = w.b; g.seq_L = w.s.L; g.spent = w.spent;
+          g.cnt = w.cnt; g.t = w.t; g.units = w.units; g.r0 = w.part.r0; g.n = w.part.n; g.L = w.part.L; g.hk = w.hk; g.spent = w.spent;
           mbar_arrive(seg_full + 8u * (seg % CTC_SEGS));
         }
         __syncwarp();
-        if (!w.cnt) break;
-        if (seg > 0u && !__all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1u) & 1u, p.c.status, 621, 50u))) break;
-        if (lane == 0u) {
-          const uint32_t nt = w.two(p.geo) ? 2u : 1u;
-          mbar_expect_tx(q_full, nt * 2u * p.geo.qpt * p.geo.group * 128u);
-          for (uint32_t t = 0; t < nt; t++)
-            for (uint32_t c = 0; c < 2u; c++) tma_load_4d(q_sm + t * ATC_TILE + c * 16384u, &mapQ, (int)(c * 64u), 0, (int)(w.part.r0 + t * p.geo.qpt), (int)w.hk, q_full);
-        }
-        uint32_t mine = 0u, kind_of = 2u;
-        CtcPage pg{1.0f, 0.0f, 1.0f, 0xffffffffu};
-        for (uint32_t j = 0; j < w.cnt && ok; j++, tile++) {
+        CtcPage pg{1.0f, 0.0f, 1.0f, 0xffffffffu, 2u, 0u, {0u, 0u}};
+        for (uint32_t j = 0; j < max(w.cnt, 1u) && ok; j++, pair++) {
           const uint32_t l0 = (2u * j) & 31u;
           if (l0 == 0u) {
             const uint32_t k = 2u * (w.t + j) + lane, page = cache_vis_page(w.v, k);
-            pg = CtcPage{1.0f, 0.0f, 1.0f, 0xffffffffu};                  // no page: every key hidden
-            mine = 0u; kind_of = 2u;
-            if (k < w.v.np) {
+            pg = CtcPage{1.0f, 0.0f, 1.0f, 0xffffffffu, w.cnt ? 2u : 3u, 0u, {0u, 0u}};      // no page: every key hidden
+            if (w.cnt && k < w.v.np) {
               float2 sc = make_float2(1.0f, 1.0f);
-              kind_of = 1u;
               if (page < w.s.L / CACHE_PAGE) {
-                kind_of = 0u;
-                mine = ld_now(p.c.table + (size_t)w.b * p.c.max_pages + page);
-                if (mine >= p.c.pages) { cache_tell(p.c.status, CACHE_BAD_PAGE); mine = 0u; }
-                sc = ld_now(p.c.scales + (size_t)mine * p.c.Hkv + w.hk);
+                uint32_t at_page = ld_now(p.c.table + (size_t)w.b * p.c.max_pages + page);
+                if (at_page >= p.c.pages) { cache_tell(p.c.status, CACHE_BAD_PAGE); at_page = 0u; }
+                pg.block = at_page * p.c.Hkv + w.hk; pg.is = 0u;
+                sc = ld_now(p.c.scales + pg.block);
+              } else {
+                pg.block = w.b * p.c.Hkv + w.hk; pg.is = 1u | (w.s.L & (CACHE_PAGE - 1u)) << 8;
               }
               pg.f = p.scale_log2 * sc.x; pg.inv_v = __fdividef(1.0f, sc.y);
               asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(pg.lv) : "f"(sc.y));
               pg.key0 = page * CACHE_PAGE | (cache_page_masked(page, w.part.L - w.part.n, w.part.L - 1u, p.geo.window, p.geo.sinks) ? 1u : 0u);
             }
           }
-          const uint32_t pa = __shfl_sync(0xffffffffu, mine, l0), pb = __shfl_sync(0xffffffffu, mine, l0 + 1u);
-          const uint32_t ka = __shfl_sync(0xffffffffu, kind_of, l0), kb = __shfl_sync(0xffffffffu, kind_of, l0 + 1u);
-          for (uint32_t kind = 0; kind < 2u; kind++, i++) {
-            const uint32_t st = i % CTC_STAGES, use = i / CTC_STAGES, bar = st_full + 8u * st;
-            if (use > 0u && !__all_sync(0xffffffffu, mbar_wait(st_empty + 8u * st, (use - 1u) & 1u, p.c.status, 622, 50u))) { ok = false; break; }
-            if (kind == 0u && (lane == l0 || lane == l0 + 1u)) scl[(tile % CTC_SCL) * 2u + (lane - l0)] = pg;
-            __syncwarp();
-            if (lane == 0u) {
-              const uint32_t n = (ka == 0u ? 1u : 0u) + (kb == 0u ? 1u : 0u), dst = st_sm + st * CTC_STAGE;
-              what[st] = ka | kb << 2;
-              if (n) {
-                mbar_expect_tx(bar, n * CACHE_BLOCK);
-                if (ka == 0u) bulk_g2s(dst, p.c.codes + (((size_t)pa * p.c.Hkv + w.hk) * 2u + kind) * CACHE_BLOCK, CACHE_BLOCK, bar);
-                if (kb == 0u) bulk_g2s(dst + CACHE_BLOCK, p.c.codes + (((size_t)pb * p.c.Hkv + w.hk) * 2u + kind) * CACHE_BLOCK, CACHE_BLOCK, bar);
-              } else mbar_arrive(bar);
-            }
-          }
+          if (pair >= CTC_PAIRS) ok = __all_sync(0xffffffffu, mbar_wait(pair_empty + 8u * (pair % CTC_PAIRS), (pair / CTC_PAIRS - 1u) & 1u, p.c.status, 622, 20u));
+          if (!ok) break;
+          if (lane == l0 || lane == l0 + 1u) scl[(pair % CTC_PAIRS) * 2u + (lane - l0)] = pg;
+          __syncwarp();
+          if (lane == 0u) mbar_arrive(pair_full + 8u * (pair % CTC_PAIRS));
         }
-        if (!ok) break;
+        if (!w.cnt) break;
+      }
+    } else if (warp == 2u) {
+      // ================================================================= queries
+      for (uint32_t seg = 0u;; seg++) {
+        if (!__all_sync(0xffffffffu, seg_wait(seg))) break;
+        volatile CtcSeg& g = segs[seg % CTC_SEGS];
+        if (!g.cnt) break;
+        const uint32_t r0 = g.r0, hk = g.hk, nt = g.n > p.geo.qpt ? 2u : 1u;
+        seg_done(seg);
+        if (seg > 0u && !__all_sync(0xffffffffu, mbar_wait(q_empty, (seg - 1u) & 1u, p.c.status, 621, 20u))) break;
+        if (lane == 0u) {
+          mbar_expect_tx(q_full, nt * 2u * p.geo.qpt * p.geo.group * 128u);
+          for (uint32_t t = 0; t < nt; t++)
+            for (uint32_t c = 0; c < 2u; c++) tma_load_4d(q_sm + t * ATC_TILE + c * 16384u, &mapQ, (int)(c * 64u), 0, (int)(r0 + t * p.geo.qpt), (int)hk, q_full);
+        }
       }
     } else if (warp == 1u) {
       // ================================================================= multiplies (the whole warp walks the loop, one lane issues)
       const uint32_t idesc = umma_idesc_f16(128u, 128u);
       const uint64_t qd[2] = {umma_desc_sw128(q_sm), umma_desc_sw128(q_sm + ATC_TILE)};
-      uint32_t i = 0u, seg = 0u, np[2] = {0u, 0u};                        // ring steps, items, weights consumed per tile of rows
+      uint32_t i = 0u, seg = 0u, np[2] = {0u, 0u};                        // tiles of K and V, items, weights consumed per tile of rows
       bool ok = true;
       for (; ok; seg++) {
         if (!__all_sync(0xffffffffu, seg_wait(seg))) break;
@@ -288,6 +289,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
             umma_commit(kv_empty + 8u * sv);
             if (more) umma_commit(kv_empty + 8u * sk);
             if (j + 2u == cnt) umma_commit(q_empty);                    // the item's last scores are under way
+            mbar_arrive(pair_empty + 8u * ((i >> 1) % CTC_PAIRS));      // (converted, and read by the softmax before it handed over the weights)
           }
           __syncwarp();
         }
@@ -296,72 +298,85 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
   } else if (warp < 8u) {
     // ================================================================= codes (or the tail's fp16) -> fp16 tiles
     regs_down<32>();
-    // unit u = 128 e + ct of a page's 512 (16 elements each): its 32 bytes go to row r of the tile's half h, pieces 2 (u % 4) and the next, swizzled
-    //   K: r = 64 page + 16 (u / 8 % 4) + 4 e + 2 (u / 64 % 2) + u / 4 % 2 (the key's column), h = u / 32 % 2 (which 64 of d);   V: r = u / 4 (d), h = page
-    const uint32_t ct = tid - 128u, ch = 2u * (ct & 3u), kx = ((ct >> 6) & 1u) * 2u + ((ct >> 2) & 1u), vx = (ct >> 2) & 7u;
-    const uint32_t k_to = ((ct >> 5) & 1u) * 16384u + (((ct >> 3) & 3u) * 16u + kx) * 128u, v_to = (ct >> 2) * 128u;
-    const uint32_t k_c0 = (ch ^ kx) << 4, k_c1 = ((ch + 1u) ^ kx) << 4, v_c0 = (ch ^ vx) << 4, v_c1 = ((ch + 1u) ^ vx) << 4;
-    uint32_t i = 0u;
-    bool ok = true;
-    for (uint32_t seg = 0u; ok; seg++) {
-      if (!__all_sync(0xffffffffu, seg_wait(seg))) break;
-      const uint32_t cnt = segs[seg % CTC_SEGS].cnt;
-      if (!cnt) { seg_done(seg); break; }
-      for (uint32_t j = 0; j < cnt && ok; j++) {
-        for (uint32_t kind = 0; kind < 2u; kind++, i++) {
-          const uint32_t st = i % CTC_STAGES, slot = i % CTC_SLOTS, src = st_sm + st * CTC_STAGE, dst = kv_sm + slot * ATC_TILE;
-          if (!mbar_wait(st_full + 8u * st, (i / CTC_STAGES) & 1u, p.c.status, 628)) ok = false;
-          if (i >= CTC_SLOTS && ok && !mbar_wait(kv_empty + 8u * slot, (i / CTC_SLOTS - 1u) & 1u, p.c.status, 629)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          const uint32_t pages = what[st];
-          if (pages == 0u) {
-            if (kind == 0u) {
+    // Two warps for K, two for V; a warp has half of each page: units 256 part + 32 e + lane of its 512 (16 elements each).  A unit's 32 bytes go to row r of the
+    // tile's half h, pieces 2 (u % 4) and the next, swizzled
+    //   K: r = 64 page + 16 (u / 8 % 4) + 4 (u / 128) + 2 (u / 64 % 2) + u / 4 % 2 (the key's column), h = u / 32 % 2 (which 64 of d);   V: r = u / 4 (d), h = page
+    const uint32_t kind = (warp - 4u) >> 1, part = warp & 1u, ch = 2u * (lane & 3u), x = kind ? lane >> 2 : (lane >> 2) & 1u, c0 = (ch ^ x) << 4, c1 = ((ch + 1u) ^ x) << 4;
+    const uint32_t to = kv_sm + (kind ? (part * 64u + (lane >> 2)) * 128u : ((lane >> 3) * 16u + part * 8u + x) * 128u), stage = st_sm + (warp - 4u) * 2u * CTC_STAGE, bar = st_full + (warp - 4u) * 16u;
+    uint32_t arrived = 0u;                                                // bit h: parity of page h's loads
+    const uint8_t* const codes = p.c.codes + kind * CACHE_BLOCK + part * CTC_STAGE;
+    auto fetch = [&](uint32_t block, uint32_t half) {                     // one lane
+      mbar_expect_tx(bar + 8u * half, CTC_STAGE);
+      bulk_g2s(stage + half * CTC_STAGE, codes + (size_t)block * (2u * CACHE_BLOCK), CTC_STAGE, bar + 8u * half);
+    };
+    auto announced = [&](uint32_t pair) { return __all_sync(0xffffffffu, mbar_wait(pair_full + 8u * (pair % CTC_PAIRS), (pair / CTC_PAIRS) & 1u, p.c.status, 634)); };
+    fence_proxy_async();                                                  // (the codes' place held the costs)
+    bool ok = announced(0u);
+    if (ok && lane < 2u && scl[lane].is == 0u) fetch(scl[lane].block, lane);
+    for (uint32_t pair = 0u; ok; pair++) {
+      const CtcPage* pg = scl + (pair % CTC_PAIRS) * 2u; const CtcPage* nx = scl + ((pair + 1u) % CTC_PAIRS) * 2u;
+      if (pg->is == 3u) break;
+      // (whether the next pair is announced is looked at without waiting: that could wait for this one)
+      const bool known = __all_sync(0xffffffffu, mbar_test(pair_full + 8u * ((pair + 1u) % CTC_PAIRS), ((pair + 1u) / CTC_PAIRS) & 1u));
+      const uint32_t slot = (2u * pair + kind) % CTC_SLOTS, use = (2u * pair + kind) / CTC_SLOTS, dst = to + slot * ATC_TILE;
+      if (use > 0u) ok = __all_sync(0xffffffffu, mbar_wait(kv_empty + 8u * slot, (use - 1u) & 1u, p.c.status, 629));
+      for (uint32_t half = 0; half < 2u && ok; half++) {
+        const uint32_t from = stage + half * CTC_STAGE + lane * 16u, at_h = dst + half * (kind ? 16384u : 8192u), is = pg[half].is;
+        uint32_t next = 0xffffffffu;                                      // the block to ask for (a cache has fewer)
+        if (known && nx[half].is == 0u) next = nx[half].block;
+        if (is == 0u) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bar + 8u * half, (arrived >> half) & 1u, p.c.status, 628));
+          if (!ok) break;
+          arrived ^= 1u << half;
+          if (kind == 0u) {
 #pragma unroll
-              for (uint32_t e = 0; e < 8u; e++) {                         // (4 rows further: the other value of the swizzle's upper bit)
-                uint4 a, b;
-                ctc_convert(ctc_lds(src + ct * 16u + e * 2048u), a, b);
-                const uint32_t to = dst + k_to + (e >> 2) * 8192u + (e & 3u) * 512u;
-                ctc_sts(to + (k_c0 ^ ((e & 1u) << 6)), a);
-                ctc_sts(to + (k_c1 ^ ((e & 1u) << 6)), b);
-              }
-            } else {
-#pragma unroll
-              for (uint32_t e = 0; e < 8u; e++) {
-                uint4 a, b;
-                ctc_convert(ctc_lds(src + ct * 16u + e * 2048u), a, b);
-                const uint32_t to = dst + v_to + (e >> 2) * 16384u + (e & 3u) * 4096u;
-                ctc_sts(to + v_c0, a);
-                ctc_sts(to + v_c1, b);
-              }
+            for (uint32_t e = 0; e < 8u; e++) {                           // e = 4 (u / 128 % 2) + 2 (u / 64 % 2) + h: rows, which turn the swizzle, and the half
+              constexpr uint32_t HALF = 16384u;
+              const uint32_t rows = (e >> 2) * 4u + ((e >> 1) & 1u) * 2u;
+              uint4 a, b;
+              ctc_convert(ctc_lds(from + e * 512u), a, b);
+              ctc_sts(at_h + (e & 1u) * HALF + rows * 128u + (c0 ^ (rows << 4)), a);
+              ctc_sts(at_h + (e & 1u) * HALF + rows * 128u + (c1 ^ (rows << 4)), b);
             }
           } else {
-#pragma unroll 1
+#pragma unroll
             for (uint32_t e = 0; e < 8u; e++) {
-              const uint32_t half = e >> 2, u = (e & 3u) * 128u + ct, is = (pages >> (2u * half)) & 3u;
-              uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
-              if (is == 0u) ctc_convert(ctc_lds(src + ct * 16u + e * 2048u), a, b);
-              else if (is == 1u) {
-                volatile CtcSeg& g = segs[seg % CTC_SEGS];
-                const uint4* tl = reinterpret_cast<const uint4*>(p.c.tail + (((size_t)g.b * p.c.Hkv + g.hk) * 2u + kind) * CACHE_BLOCK);
-                a = ld_now(tl + 2u * u); b = ld_now(tl + 2u * u + 1u);
-                if (kind) {                                               // keys behind the sequence's end may hold anything: they weigh nothing, but 0 * NaN would count
-                  const int have = (int)(g.seq_L & (CACHE_PAGE - 1u)) - (int)(4u * (u & 3u));
-                  auto keep = [&](uint32_t v, int at) { return have >= at + 2 ? v : have == at + 1 ? v & 0xffffu : 0u; };
-                  a.x = keep(a.x, 0); a.y = keep(a.y, 2); a.z = keep(a.z, 16); a.w = keep(a.w, 18);
-                  b.x = keep(b.x, 32); b.y = keep(b.y, 34); b.z = keep(b.z, 48); b.w = keep(b.w, 50);
-                }
-              }
-              const uint32_t flip = kind ? 0u : (e & 1u) << 6, to = dst + (kind ? v_to + half * 16384u + (e & 3u) * 4096u : k_to + half * 8192u + (e & 3u) * 512u);
-              ctc_sts(to + ((kind ? v_c0 : k_c0) ^ flip), a);
-              ctc_sts(to + ((kind ? v_c1 : k_c1) ^ flip), b);
+              uint4 a, b;
+              ctc_convert(ctc_lds(from + e * 512u), a, b);
+              ctc_sts(at_h + e * 1024u + c0, a);
+              ctc_sts(at_h + e * 1024u + c1, b);
             }
           }
-          fence_proxy_async();
-          __syncwarp();
-          if (lane == 0u) { mbar_arrive(kv_full + 8u * slot); mbar_arrive(st_empty + 8u * st); }
+        } else {
+          const uint4* tl = reinterpret_cast<const uint4*>(p.c.tail + ((size_t)pg[half].block * 2u + kind) * CACHE_BLOCK) + part * 512u + 2u * lane;
+#pragma unroll 1
+          for (uint32_t e = 0; e < 8u; e++) {
+            uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+            if (is != 2u) {
+              a = ld_now(tl + e * 64u); b = ld_now(tl + e * 64u + 1u);
+              if (kind) {                                                 // keys behind the sequence's end may hold anything: they weigh nothing, but 0 * NaN would count
+                const int have = (int)(is >> 8) - (int)(4u * (lane & 3u));
+                auto keep = [&](uint32_t v, int at) { return have >= at + 2 ? v : have == at + 1 ? v & 0xffffu : 0u; };
+                a.x = keep(a.x, 0); a.y = keep(a.y, 2); a.z = keep(a.z, 16); a.w = keep(a.w, 18);
+                b.x = keep(b.x, 32); b.y = keep(b.y, 34); b.z = keep(b.z, 48); b.w = keep(b.w, 50);
+              }
+            }
+            const uint32_t rows = (e >> 2) * 4u + ((e >> 1) & 1u) * 2u, flip = kind ? 0u : rows << 4, at_e = at_h + (kind ? e * 1024u : (e & 1u) * 16384u + rows * 128u);
+            ctc_sts(at_e + (c0 ^ flip), a);
+            ctc_sts(at_e + (c1 ^ flip), b);
+          }
+        }
+        if (half) fence_proxy_async();
+        __syncwarp();
+        if (lane == 0u) {
+          if (half) mbar_arrive(kv_full + 8u * slot);
+          if (next != 0xffffffffu) fetch(next, half);
         }
       }
-      seg_done(seg);
+      if (!ok) break;
+      ok = announced(pair + 1u);
+      if (ok && !known && lane < 2u && nx[lane].is == 0u) fetch(nx[lane].block, lane);
+      __syncwarp();
     }
   } else {
     // ================================================================= softmax of one tile: two threads per row, one page of a pair each
@@ -371,7 +386,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
     const uint32_t o_addr = lane_addr + 256u + t * 128u + half * 64u, pair_bar = 1u + t * 4u + (warp & 3u);
     float* mine = xch + (t * 2u + half) * 128u + row; const float* other = xch + (t * 2u + (half ^ 1u)) * 128u + row;
     const uint32_t qi = row / p.geo.group, hh = row - qi * p.geo.group;
-    uint32_t n = 0u, tile = 0u, items = 0u, xp = 0u;                      // this tile's scores and items so far, the block's key tiles, parity of the exchange
+    uint32_t n = 0u, pair = 0u, items = 0u;                               // this tile's scores and items so far, the block's pairs of pages
     bool ok = true;
     for (uint32_t seg = 0u;; seg++) {
       if (ok && !seg_wait(seg)) ok = false;
@@ -379,22 +394,23 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
       ok = ctc_agree((int)pair_bar, ok);                                  // (the two warps of a row meet at barriers: both go on, or neither)
       const uint32_t cnt = ok ? g.cnt : 0u;
       if (!cnt) break;
-      if (t == 1u && g.n <= p.geo.qpt) { tile += cnt; seg_done(seg); continue; }
+      if (t == 1u && g.n <= p.geo.qpt) { pair += cnt; seg_done(seg); continue; }
       const uint32_t pos = g.L - g.n + min(t * p.geo.qpt + qi, g.n - 1u);
       float m_used = -INFINITY, l = 0.0f;
-      for (uint32_t j = 0; j < cnt; j++, n++, tile++) {
+      for (uint32_t j = 0; j < cnt; j++, n++, pair++) {
         // (a wait that ran out: the thread goes on without it, so that its partner is not left at the barrier; the status word is set)
                 if (ok && !mbar_wait(s_full + 8u * t, n & 1u, p.c.status, 630)) ok = false;
         tc_fence_after();
         uint32_t s[64];
 #pragma unroll
         for (int c = 0; c < 4; c++) tmem_ld16(s_addr + 16u * c, *reinterpret_cast<uint32_t(*)[16]>(&s[16 * c]));
-        const CtcPage pg = scl[(tile % CTC_SCL) * 2u + half];
-        const float sc = pg.f, lv = pg.lv;
+        const float4 pg = *reinterpret_cast<const float4*>(&scl[(pair % CTC_PAIRS) * 2u + half]);      // f, lv, inv_v, key0
+        const float sc = pg.x, lv = pg.y;
+        const uint32_t key0 = __float_as_uint(pg.w);
         tmem_ld_wait();
-        if (pg.key0 & 1u) {
+        if (key0 & 1u) {
           // columns whose key is visible: at most hi, and at least lo or below sk (all relative to the page)
-          const uint32_t k0 = pg.key0 & ~1u;
+          const uint32_t k0 = key0 & ~1u;
           const int hi = (int)min(pos - min(pos, k0), 64u) - (pos < k0 ? 1 : 0);
           int lo = 0, sk = 0;
           if (p.geo.window && pos >= p.geo.window) {
@@ -414,12 +430,11 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
           for (int e = 0; e < 4; e++) mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(s[c + 2 * e])), __uint_as_float(s[c + 2 * e + 1]));      // (one instruction: the maximum of three)
         }
         float mts = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sc, lv);
-        mine[xp * 512u] = mts;
+        *mine = mts;                         // (the partner has read the last one: these scores are there because it handed over the weights before them)
         tc_fence_before();                   // this warp's reads of S end before its partner writes P over columns 32..63 of them
         bar_sync_named((int)pair_bar, 64);
         tc_fence_after();
-        mts = fmaxf(mts, other[xp * 512u]);
-        xp ^= 1u;
+        mts = fmaxf(mts, *other);
         if (__any_sync(0xffffffffu, mts > m_used + 8.0f || (m_used == -INFINITY && mts > -INFINITY))) {
           const float m_new = fmaxf(m_used, mts);
           const float alpha = m_new == -INFINITY ? 1.0f : atc_ex2(m_used - m_new);
@@ -459,12 +474,12 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + 8u * t);
-        l = fmaf((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y), pg.inv_v, l);
+        l = fmaf((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y), pg.z, l);
       }
-      mine[xp * 512u] = l;
+      bar_sync_named((int)pair_bar, 64);     // (the partner has read the last maximum)
+      *mine = l;
       bar_sync_named((int)pair_bar, 64);
-      l += other[xp * 512u];
-      xp ^= 1u;
+      l += *other;
       // ---- the item's end: O / l, or this block's partial result
       if (ok && !mbar_wait(o_full + 8u * t, items & 1u, p.c.status, 631)) ok = false;
       items++;
