@@ -76,8 +76,9 @@ P0P_HD bool cache_page_masked(uint32_t page, uint32_t p0, uint32_t p1, uint32_t 
 }
 
 // U units of work in a row are dealt out to G workers, G <= U: worker c has units [deal_first(c), deal_first(c + 1)).
-P0P_HD uint64_t deal_first(uint64_t c, uint64_t U, uint64_t G) { return c * U / G; }
-P0P_HD uint64_t deal_owner(uint64_t u, uint64_t U, uint64_t G) { return ((u + 1u) * G - 1u) / U; }
+P0P_HD uint64_t div_64(uint64_t a, uint64_t b) { return ((a | b) >> 32) ? a / b : (uint32_t)a / (uint32_t)b; }      // (a 64-bit division takes hundreds of cycles)
+P0P_HD uint64_t deal_first(uint64_t c, uint64_t U, uint64_t G) { return div_64(c * U, G); }
+P0P_HD uint64_t deal_owner(uint64_t u, uint64_t U, uint64_t G) { return div_64((u + 1u) * G - 1u, U); }
 
 // The split-key attention's units: per sequence [kv head][block of 16 query rows][visible page], one sequence after the other.  The query rows of
 // the `group` heads that share a kv head are one matrix of n * group rows, query by query.
@@ -99,9 +100,9 @@ struct CacheCursor {
     while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (pre[mid + 1u] > u) hi = mid; else lo = mid + 1u; }
     sequence(g, seq, lo);
     const uint64_t r = u - pre[lo], per = (uint64_t)rbs * v.np;
-    hk = (uint32_t)(r / per);
+    hk = (uint32_t)div_64(r, per);
     const uint64_t x = r - hk * per;
-    rb = (uint32_t)(x / v.np); t = (uint32_t)(x - (uint64_t)rb * v.np);
+    rb = (uint32_t)div_64(x, v.np); t = (uint32_t)(x - (uint64_t)rb * v.np);
   }
   // the next unit, which there has to be
   P0P_HD void next(const CacheGeo& g, const uint64_t* pre, const CacheSeq* seq) {

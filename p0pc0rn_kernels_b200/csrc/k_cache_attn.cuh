@@ -102,78 +102,176 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
   const uint64_t u0 = deal_first(blockIdx.x, U, G), u1 = deal_first(blockIdx.x + 1u, U, G), here = u1 - u0, W = here < CA_WARPS ? here : CA_WARPS;
   if (warp < W) {
     const uint64_t w0 = u0 + deal_first(warp, here, W), w1 = u0 + deal_first(warp + 1u, here, W);
-    CacheCursor cur, nxt;
+    CacheCursor cur;
     cur.seek(geo, sh.pre, sh.seq, w0);
-    nxt = cur;
-    auto table_at = [&](const CacheCursor& c) { return c.tail() ? 0u : ld_now(p.c.table + (size_t)c.b * p.c.max_pages + c.page()); };
-    auto checked = [&](uint32_t page) { if (page < p.c.pages) return page; if (lane == 0u) cache_tell(p.c.status, CACHE_BAD_PAGE); return 0u; };
-    auto codes_at = [&](const CacheCursor& c, uint32_t page, uint32_t w) -> const void* {
-      return c.tail() ? (const void*)(p.c.tail + (((size_t)c.b * p.c.Hkv + c.hk) * 2u + w) * CACHE_BLOCK) : (const void*)(p.c.codes + (((size_t)page * p.c.Hkv + c.hk) * 2u + w) * CACHE_BLOCK);
+    // pages of a row's blocks of codes, by the lane's page of 32: as the table has them, then checked, as blocks (page * Hkv + kv head)
+    auto raw_at = [&](const CacheCursor& c, uint32_t t) {
+      return t >= c.v.np || cache_vis_page(c.v, t) == c.s.L / CACHE_PAGE ? 0u : ld_now(p.c.table + (size_t)c.b * p.c.max_pages + cache_vis_page(c.v, t));
     };
-    auto fetch = [&](const CacheCursor& c, uint32_t page, uint32_t w) {       // one lane: K (w 0) or V of a page; the tail's takes both buffers
-      const uint32_t bytes = c.tail() ? 2u * CACHE_BLOCK : CACHE_BLOCK, bar = w ? bar_v : bar_k;
-      mbar_expect_tx(bar, bytes);
-      bulk_g2s(ring + (w && !c.tail() ? CACHE_BLOCK : 0u), codes_at(c, page, w), bytes, bar);
+    auto block_of = [&](const CacheCursor& c, uint32_t raw) {
+      if (raw >= p.c.pages) { cache_tell(p.c.status, CACHE_BAD_PAGE); raw = 0u; }
+      return raw * p.c.Hkv + c.hk;
     };
-    auto scales_at = [&](const CacheCursor& c, uint32_t page) { return c.tail() ? make_float2(1.0f, 1.0f) : ld_now(p.c.scales + (size_t)page * p.c.Hkv + c.hk); };
-    uint32_t page = checked(table_at(cur)), nxt_raw = 0u;                  // this unit's page; the next one's as read
-    float2 sc = scales_at(cur, page);
-    if (lane == 0u) { fetch(cur, page, 0u); if (!cur.tail()) fetch(cur, page, 1u); }
-    if (w0 + 1u < w1) { nxt.next(geo, sh.pre, sh.seq); nxt_raw = table_at(nxt); }
+    auto fetch = [&](uint32_t block, uint32_t w) {                         // K (w 0) or V of a block of codes
+      if (lane == 0u) {
+        mbar_expect_tx(w ? bar_v : bar_k, CACHE_BLOCK);
+        bulk_g2s(ring + w * CACHE_BLOCK, p.c.codes + ((size_t)block * 2u + w) * CACHE_BLOCK, CACHE_BLOCK, w ? bar_v : bar_k);
+      }
+    };
+    auto fetch_tail = [&](const CacheCursor& c, uint32_t w) {              // of a tail, into both buffers
+      if (lane == 0u) {
+        mbar_expect_tx(w ? bar_v : bar_k, 2u * CACHE_BLOCK);
+        bulk_g2s(ring, p.c.tail + (((size_t)c.b * p.c.Hkv + c.hk) * 2u + w) * CACHE_BLOCK, 2u * CACHE_BLOCK, w ? bar_v : bar_k);
+      }
+    };
     uint32_t ph_k = 0u, ph_v = 0u;
-    uint32_t qa[8][4];
-    float bias[2] = {0.0f, 0.0f};
-    uint32_t pos[2] = {0u, 0u};
-    float o[16][4], m[2], l[2];
-    bool fresh = true, ok = true;
-    uint64_t i0 = 0u;                                                      // the item's first unit
-    for (uint64_t u = w0; u < w1; u++) {
-      const bool tail = cur.tail(), more = u + 1u < w1;
-      const uint32_t kp = cur.page(), rows = cur.s.n * p.group;
-      if (fresh) {
-        // ---- a new item: this thread's two query rows (rows past the end repeat the last one; they are not stored)
-        fresh = false;
-        i0 = u - cur.t;
-        const uint32_t first = cur.s.L - cur.s.n;
+    bool ok = true;
+    auto wait_k = [&] { ok = __all_sync(0xffffffffu, mbar_wait(bar_k, ph_k, p.c.status, 611)); ph_k ^= 1u; return ok; };
+    auto wait_v = [&] { ok = __all_sync(0xffffffffu, mbar_wait(bar_v, ph_v, p.c.status, 612)); ph_v ^= 1u; return ok; };
+    uint32_t qa[8][4], pa[4][4], pos[2];
+    float bias[2], o[16][4], m[2], l[2], s[8][4], zp[4];
+    // scores (scaled, log2) -> weights pa, their sums zp; the running maximum rises only when it grew by more than 2^8 (weights are at most 256 then)
+    auto weigh = [&](uint32_t page, uint32_t p0, uint32_t p1, float f, float lv, float inv_v) {
+      float mx[2] = {-INFINITY, -INFINITY};
+      if (cache_page_masked(page, p0, p1, p.window, p.sinks)) {
+#pragma unroll
+        for (uint32_t n = 0; n < 8u; n++)
+#pragma unroll
+          for (uint32_t e = 0; e < 4u; e++) {
+            const uint32_t key = page * CACHE_PAGE + 16u * (n >> 1) + 4u * t4 + 2u * (n & 1u) + (e & 1u);
+            s[n][e] = cache_key_visible(key, pos[e >> 1], p.window, p.sinks) ? s[n][e] : -INFINITY;
+          }
+      }
+#pragma unroll
+      for (uint32_t n = 0; n < 8u; n++) { mx[0] = fmaxf(fmaxf(mx[0], s[n][0]), s[n][1]); mx[1] = fmaxf(fmaxf(mx[1], s[n][2]), s[n][3]); }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1)); mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+        mx[h] = fmaf(mx[h], f, lv);
+      }
+      if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.0f || mx[1] > m[1] + 8.0f)) {
+        const float n0 = fmaxf(m[0], mx[0]), n1 = fmaxf(m[1], mx[1]);
+        const float a0 = n0 == -INFINITY ? 1.0f : at_ex2(m[0] - n0), a1 = n1 == -INFINITY ? 1.0f : at_ex2(m[1] - n1);
+        m[0] = n0; m[1] = n1; l[0] *= a0; l[1] *= a1;
+#pragma unroll
+        for (int d = 0; d < 16; d++) { o[d][0] *= a0; o[d][1] *= a0; o[d][2] *= a1; o[d][3] *= a1; }
+      }
+      const float e0 = m[0] == -INFINITY ? 0.0f : lv - m[0], e1 = m[1] == -INFINITY ? 0.0f : lv - m[1];      // (a row that has seen no key yet: all its weights are 0)
+      zp[0] = zp[1] = zp[2] = zp[3] = 0.0f;
+#pragma unroll
+      for (uint32_t j = 0; j < 4u; j++) {
 #pragma unroll
         for (uint32_t h = 0; h < 2u; h++) {
-          const uint32_t r = min(cur.rb * 16u + h * 8u + g, rows - 1u), i = r / p.group;
-          pos[h] = first + i;
-          const uint4* q = reinterpret_cast<const uint4*>(p.Q + ((size_t)(cur.hk * p.group + (r - i * p.group)) * p.ldq + cur.s.r0 + i) * 128u + t4 * 16u);
-#pragma unroll
-          for (uint32_t k = 0; k < 2u; k++) {
-            const uint4 a = ld_now(q + k * 8u), c = ld_now(q + k * 8u + 1u);
-            qa[k * 4u][h] = a.x; qa[k * 4u][2u + h] = a.y; qa[k * 4u + 1u][h] = a.z; qa[k * 4u + 1u][2u + h] = a.w;
-            qa[k * 4u + 2u][h] = c.x; qa[k * 4u + 2u][2u + h] = c.y; qa[k * 4u + 3u][h] = c.z; qa[k * 4u + 3u][2u + h] = c.w;
-          }
+          const float* x = s[2u * j + h];
+          const float2 u0 = __ffma2_rn(make_float2(x[0], x[1]), make_float2(f, f), make_float2(e0, e0)), u1 = __ffma2_rn(make_float2(x[2], x[3]), make_float2(f, f), make_float2(e1, e1));
+          pa[j][2u * h] = at_pack(at_ex2(u0.x), at_ex2(u0.y));
+          pa[j][2u * h + 1u] = at_pack(at_ex2(u1.x), at_ex2(u1.y));
         }
+        at_mma(zp, pa[j], 0x3c003c00u, 0x3c003c00u);
+      }
+      l[0] = fmaf(zp[0], inv_v, l[0]); l[1] = fmaf(zp[2], inv_v, l[1]);
+    };
+    // ---- the first page is on its way before anything else
+    uint32_t blk = block_of(cur, raw_at(cur, cur.t + lane));               // this lane's page of the 32 at hand
+    {
+      const uint32_t first = __shfl_sync(0xffffffffu, blk, 0);
+      if (cur.tail()) fetch_tail(cur, 0u);
+      else { fetch(first, 0u); fetch(first, 1u); }
+    }
+    for (uint64_t u = w0; u < w1;) {
+      // ---- an item, or this warp's share of it: pages t .. t + cnt - 1, of which the last may be the tail
+      const uint64_t i0 = u - cur.t;
+      const uint32_t cnt = (uint32_t)min((uint64_t)(cur.v.np - cur.t), w1 - u), rows = cur.s.n * p.group, p0 = cur.s.L - cur.s.n, p1 = cur.s.L - 1u;
+      const bool done = cur.t + cnt == cur.v.np, has_tail = done && (cur.s.L & (CACHE_PAGE - 1u)) != 0u, more = u + cnt < w1;
+      const uint32_t codes = cnt - (has_tail ? 1u : 0u);
+      // (everything that has to come from memory is asked for before any of it is looked at: one after the other these loads took 6000 cycles an item)
+      float2 sc = ld_now(p.c.scales + blk), sc2 = sc;
+      CacheCursor nxt = cur;
+      uint32_t nxt_raw = 0u, nxt_blk = 0u, blk2 = 0u, raw2 = 0u;
+      if (more) { nxt.t = nxt.v.np - 1u; nxt.next(geo, sh.pre, sh.seq); nxt_raw = raw_at(nxt, lane); }
+      const bool nxt_tail = more && nxt.tail();
+      // this thread's two query rows (rows past the end repeat the last one; they are not stored)
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; h++) {
+        const uint32_t r = min(cur.rb * 16u + h * 8u + g, rows - 1u), i = r / p.group;
+        pos[h] = p0 + i;
+        const uint4* q = reinterpret_cast<const uint4*>(p.Q + ((size_t)(cur.hk * p.group + (r - i * p.group)) * p.ldq + cur.s.r0 + i) * 128u + t4 * 16u);
+#pragma unroll
+        for (uint32_t k = 0; k < 2u; k++) {
+          const uint4 a = ld_now(q + k * 8u), c = ld_now(q + k * 8u + 1u);
+          qa[k * 4u][h] = a.x; qa[k * 4u][2u + h] = a.y; qa[k * 4u + 1u][h] = a.z; qa[k * 4u + 1u][2u + h] = a.w;
+          qa[k * 4u + 2u][h] = c.x; qa[k * 4u + 2u][2u + h] = c.y; qa[k * 4u + 3u][h] = c.z; qa[k * 4u + 3u][2u + h] = c.w;
+        }
+      }
+      {
         float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < 8; k++) at_mma(s4, qa[k], 0x80808080u, 0x80808080u);      // -128 * 2^-24 each
         bias[0] = s4[0]; bias[1] = s4[2];
-#pragma unroll
-        for (int d = 0; d < 16; d++) { o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f; }
-        m[0] = m[1] = -INFINITY; l[0] = l[1] = 0.0f;
       }
-      // ---- scores of 64 keys
-      float s[8][4];
-      if (ok && !mbar_wait(bar_k, ph_k, p.c.status, 611)) ok = false;
-      ph_k ^= 1u;
-      if (!__all_sync(0xffffffffu, ok)) { sh.failed = 1u; break; }
-      if (!tail) {
 #pragma unroll
-        for (uint32_t n = 0; n < 8u; n++) {
-          s[n][0] = s[n][1] = bias[0]; s[n][2] = s[n][3] = bias[1];
+      for (int d = 0; d < 16; d++) { o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f; }
+      m[0] = m[1] = -INFINITY; l[0] = l[1] = 0.0f;
+      if (more) nxt_blk = block_of(nxt, nxt_raw);
+      const uint32_t nxt_block = __shfl_sync(0xffffffffu, nxt_blk, 0);
+      for (uint32_t i = 0; i < codes && ok; i++) {
+        const uint32_t at = i & 31u;
+        if (at == 0u) {                                                    // 32 pages at a time: the next ones' numbers are asked for here, their scales half way
+          if (i > 0u) { blk = blk2; sc = sc2; }
+          raw2 = raw_at(cur, cur.t + i + 32u + lane);
+        }
+        if (at == 16u) { blk2 = block_of(cur, raw2); sc2 = ld_now(p.c.scales + blk2); }
+        const float ks = __shfl_sync(0xffffffffu, sc.x, at), vs = __shfl_sync(0xffffffffu, sc.y, at);
+        const bool last = i + 1u == codes;
+        const uint32_t next = last ? nxt_block : __shfl_sync(0xffffffffu, at == 31u ? blk2 : blk, (at + 1u) & 31u);
+        // what follows: a page of codes (of this item or the next) can be asked for buffer by buffer, a tail needs both
+        const bool follows = !last || (!has_tail && more && !nxt_tail), tail_follows = last && (has_tail || nxt_tail);
+        if (!wait_k()) break;
+#pragma unroll
+        for (uint32_t n = 0; n < 8u; n += 4u) {                            // (four sums at a time: a product waits for the one before it on the same sum)
+#pragma unroll
+          for (uint32_t h = 0; h < 4u; h++) { s[n + h][0] = s[n + h][1] = bias[0]; s[n + h][2] = s[n + h][3] = bias[1]; }
 #pragma unroll
           for (uint32_t k = 0; k < 2u; k++) {
-            const uint4 w = ca_lds(ring + n * 1024u + k * 512u + lane * 16u);
-            at_mma(s[n], qa[k * 4u], __byte_perm(w.x, 0u, 0x4140), __byte_perm(w.x, 0u, 0x4342));
-            at_mma(s[n], qa[k * 4u + 1u], __byte_perm(w.y, 0u, 0x4140), __byte_perm(w.y, 0u, 0x4342));
-            at_mma(s[n], qa[k * 4u + 2u], __byte_perm(w.z, 0u, 0x4140), __byte_perm(w.z, 0u, 0x4342));
-            at_mma(s[n], qa[k * 4u + 3u], __byte_perm(w.w, 0u, 0x4140), __byte_perm(w.w, 0u, 0x4342));
+            uint32_t w[4][4];
+#pragma unroll
+            for (uint32_t h = 0; h < 4u; h++) { const uint4 v = ca_lds(ring + (n + h) * 1024u + k * 512u + lane * 16u); w[h][0] = v.x; w[h][1] = v.y; w[h][2] = v.z; w[h][3] = v.w; }
+#pragma unroll
+            for (uint32_t j = 0; j < 4u; j++)
+#pragma unroll
+              for (uint32_t h = 0; h < 4u; h++) at_mma(s[n + h], qa[k * 4u + j], __byte_perm(w[h][j], 0u, 0x4140), __byte_perm(w[h][j], 0u, 0x4342));
           }
         }
-      } else {
+        __syncwarp();                                                      // the K buffer is read
+        if (follows) fetch(next, 0u);
+        weigh(cache_vis_page(cur.v, cur.t + i), p0, p1, p.scale_log2 * ks * 16777216.0f, ca_lg2(vs), __fdividef(1.0f, vs));
+        const float c0 = -0x1p-17f * zp[0], c1 = -0x1p-17f * zp[2];        // -128 * 2^-24 each
+        if (!wait_v()) break;
+#pragma unroll
+        for (uint32_t d = 0; d < 16u; d += 4u) {
+          uint32_t w[4][4];
+#pragma unroll
+          for (uint32_t h = 0; h < 4u; h++) { const uint4 v = ca_lds(ring + CACHE_BLOCK + (d + h) * 512u + lane * 16u); w[h][0] = v.x; w[h][1] = v.y; w[h][2] = v.z; w[h][3] = v.w; }
+#pragma unroll
+          for (uint32_t h = 0; h < 4u; h++) {
+            const float2 y = __fadd2_rn(make_float2(o[d + h][0], o[d + h][1]), make_float2(c0, c0)), v = __fadd2_rn(make_float2(o[d + h][2], o[d + h][3]), make_float2(c1, c1));
+            o[d + h][0] = y.x; o[d + h][1] = y.y; o[d + h][2] = v.x; o[d + h][3] = v.y;
+          }
+#pragma unroll
+          for (uint32_t j = 0; j < 4u; j++)
+#pragma unroll
+            for (uint32_t h = 0; h < 4u; h++) at_mma(o[d + h], pa[j], __byte_perm(w[h][j], 0u, 0x4140), __byte_perm(w[h][j], 0u, 0x4342));
+        }
+        __syncwarp();                                                      // the V buffer is read
+        if (follows) fetch(next, 1u);
+        if (tail_follows) fetch_tail(has_tail ? cur : nxt, 0u);
+      }
+      if (!ok) { sh.failed = 1u; break; }
+      // from here on O is in real units
+#pragma unroll
+      for (int d = 0; d < 16; d++) { o[d][0] *= 16777216.0f; o[d][1] *= 16777216.0f; o[d][2] *= 16777216.0f; o[d][3] *= 16777216.0f; }
+      if (has_tail) {
+        if (!wait_k()) { sh.failed = 1u; break; }
 #pragma unroll
         for (uint32_t n = 0; n < 8u; n++) {
           s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
@@ -186,92 +284,17 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
             at_mma(s[n], qa[k * 4u + 3u], x.z, x.w);
           }
         }
-      }
-      __syncwarp();                                                        // the K buffer is read
-      uint32_t nxt_page = 0u;
-      float2 nxt_sc = make_float2(1.0f, 1.0f);
-      if (tail) { if (lane == 0u) fetch(cur, 0u, 1u); }                    // the tail's V, into both buffers
-      if (more) {
-        nxt_page = checked(nxt_raw);
-        if (lane == 0u && !tail && !nxt.tail()) fetch(nxt, nxt_page, 0u);
-        nxt_sc = scales_at(nxt, nxt_page);
-      }
-      CacheCursor aft = nxt;                                                  // the unit after the next: its table entry is asked for now
-      uint32_t aft_raw = 0u;
-      if (u + 2u < w1) { aft.next(geo, sh.pre, sh.seq); aft_raw = table_at(aft); }
-      // ---- masks, maximum, weights
-      const float f = p.scale_log2 * sc.x * (tail ? 1.0f : 16777216.0f), lv = tail ? 0.0f : ca_lg2(sc.y), inv_v = tail ? 1.0f : __fdividef(1.0f, sc.y);
-      const uint32_t p0 = cur.s.L - cur.s.n, p1 = cur.s.L - 1u;
-      float mx[2] = {-INFINITY, -INFINITY};
-      if (cache_page_masked(kp, p0, p1, p.window, p.sinks)) {
-#pragma unroll
-        for (uint32_t n = 0; n < 8u; n++)
-#pragma unroll
-          for (uint32_t e = 0; e < 4u; e++) {
-            const uint32_t key = kp * CACHE_PAGE + 16u * (n >> 1) + 4u * t4 + 2u * (n & 1u) + (e & 1u);
-            s[n][e] = cache_key_visible(key, pos[e >> 1], p.window, p.sinks) ? fmaf(s[n][e], f, lv) : -INFINITY;
-            mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-          }
-      } else {
-#pragma unroll
-        for (uint32_t n = 0; n < 8u; n++)
-#pragma unroll
-          for (uint32_t e = 0; e < 4u; e++) { s[n][e] = fmaf(s[n][e], f, lv); mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]); }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; h++) { mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1)); mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)); }
-      if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-        const float n0 = fmaxf(m[0], mx[0]), n1 = fmaxf(m[1], mx[1]);
-        const float a0 = n0 == -INFINITY ? 1.0f : at_ex2(m[0] - n0), a1 = n1 == -INFINITY ? 1.0f : at_ex2(m[1] - n1);
-        m[0] = n0; m[1] = n1; l[0] *= a0; l[1] *= a1;
-#pragma unroll
-        for (int d = 0; d < 16; d++) { o[d][0] *= a0; o[d][1] *= a0; o[d][2] *= a1; o[d][3] *= a1; }
-      }
-      const float e0 = m[0] == -INFINITY ? 0.0f : m[0], e1 = m[1] == -INFINITY ? 0.0f : m[1];
-      uint32_t pa[4][4];
-      float zp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (uint32_t j = 0; j < 4u; j++) {
-#pragma unroll
-        for (uint32_t h = 0; h < 2u; h++) {
-          const float* x = s[2u * j + h];
-          pa[j][2u * h] = at_pack(at_ex2(x[0] - e0), at_ex2(x[1] - e0));
-          pa[j][2u * h + 1u] = at_pack(at_ex2(x[2] - e1), at_ex2(x[3] - e1));
-        }
-        at_mma(zp, pa[j], 0x3c003c00u, 0x3c003c00u);
-      }
-      l[0] = fmaf(zp[0], inv_v, l[0]); l[1] = fmaf(zp[2], inv_v, l[1]);
-      // (the tail is the last page of its item: from there on O is in real units)
-#pragma unroll
-      for (int d = 0; d < 16; d++) {
-        if (tail) { o[d][0] *= 16777216.0f; o[d][1] *= 16777216.0f; o[d][2] *= 16777216.0f; o[d][3] *= 16777216.0f; }
-        else {
-          const float c0 = -0x1p-17f * zp[0], c1 = -0x1p-17f * zp[2];      // -128 * 2^-24 each
-          const float2 x = __fadd2_rn(make_float2(o[d][0], o[d][1]), make_float2(c0, c0)), y = __fadd2_rn(make_float2(o[d][2], o[d][3]), make_float2(c1, c1));
-          o[d][0] = x.x; o[d][1] = x.y; o[d][2] = y.x; o[d][3] = y.y;
-        }
-      }
-      // ---- weights times values
-      if (ok && !mbar_wait(bar_v, ph_v, p.c.status, 612)) ok = false;
-      ph_v ^= 1u;
-      if (!__all_sync(0xffffffffu, ok)) { sh.failed = 1u; break; }
-      if (!tail) {
-#pragma unroll
-        for (uint32_t d = 0; d < 16u; d++) {
-          const uint4 w = ca_lds(ring + CACHE_BLOCK + d * 512u + lane * 16u);
-          at_mma(o[d], pa[0], __byte_perm(w.x, 0u, 0x4140), __byte_perm(w.x, 0u, 0x4342));
-          at_mma(o[d], pa[1], __byte_perm(w.y, 0u, 0x4140), __byte_perm(w.y, 0u, 0x4342));
-          at_mma(o[d], pa[2], __byte_perm(w.z, 0u, 0x4140), __byte_perm(w.z, 0u, 0x4342));
-          at_mma(o[d], pa[3], __byte_perm(w.w, 0u, 0x4140), __byte_perm(w.w, 0u, 0x4342));
-        }
-      } else {
+        __syncwarp();
+        fetch_tail(cur, 1u);
+        weigh(cur.s.L / CACHE_PAGE, p0, p1, p.scale_log2, 0.0f, 1.0f);
         // (behind the sequence's end the tail may hold anything: those values weigh nothing, but 0 * NaN would count)
-        const int have = (int)(cur.s.L - kp * CACHE_PAGE) - (int)(4u * t4);
+        const int have = (int)(cur.s.L & (CACHE_PAGE - 1u)) - (int)(4u * t4);
         uint32_t keep[4][2];
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
           for (int h = 0; h < 2; h++) { const int r = have - 16 * j - 2 * h; keep[j][h] = r >= 2 ? 0xffffffffu : r == 1 ? 0xffffu : 0u; }
+        if (!wait_v()) { sh.failed = 1u; break; }
 #pragma unroll
         for (uint32_t d = 0; d < 16u; d++) {
           const uint4 w = ca_lds(ring + d * 1024u + lane * 32u), x = ca_lds(ring + d * 1024u + lane * 32u + 16u);
@@ -280,47 +303,37 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
           at_mma(o[d], pa[2], x.x & keep[2][0], x.y & keep[2][1]);
           at_mma(o[d], pa[3], x.z & keep[3][0], x.w & keep[3][1]);
         }
-      }
-      __syncwarp();                                                        // the V buffer is read
-      if (more && lane == 0u) {
-        if (tail || nxt.tail()) fetch(nxt, nxt_page, 0u);
-        if (!nxt.tail()) fetch(nxt, nxt_page, 1u);
+        __syncwarp();
+        if (nxt_tail) fetch_tail(nxt, 0u);
+        else if (more) { fetch(nxt_block, 0u); fetch(nxt_block, 1u); }
       }
       // ---- the end of the item, or of this warp's share
-      const bool done = cur.t + 1u == cur.v.np;
-      if (done || !more) {
-        fresh = true;
-        if (!tail) {
+      if (done && i0 >= w0) {
+        const float inv[2] = {l[0] > 0.0f ? 1.0f / l[0] : l[0], l[1] > 0.0f ? 1.0f / l[1] : l[1]};
 #pragma unroll
-          for (int d = 0; d < 16; d++) { o[d][0] *= 16777216.0f; o[d][1] *= 16777216.0f; o[d][2] *= 16777216.0f; o[d][3] *= 16777216.0f; }
-        }
-        if (done && i0 >= w0) {
-          const float inv[2] = {l[0] > 0.0f ? 1.0f / l[0] : l[0], l[1] > 0.0f ? 1.0f / l[1] : l[1]};      // (a row that saw only pages that do not exist: 0)
+        for (uint32_t h = 0; h < 2u; h++) {
+          const uint32_t r = cur.rb * 16u + h * 8u + g, i = r / p.group;
+          if (r < rows) {
+            __half2* dst = reinterpret_cast<__half2*>(p.O + (size_t)(cur.s.r0 + i) * p.ldo + (cur.hk * p.group + (r - i * p.group)) * 128u + 2u * t4);
 #pragma unroll
-          for (uint32_t h = 0; h < 2u; h++) {
-            const uint32_t r = cur.rb * 16u + h * 8u + g, i = r / p.group;
-            if (r < rows) {
-              __half2* dst = reinterpret_cast<__half2*>(p.O + (size_t)(cur.s.r0 + i) * p.ldo + (cur.hk * p.group + (r - i * p.group)) * 128u + 2u * t4);
-#pragma unroll
-              for (int d = 0; d < 16; d++) dst[4 * d] = __floats2half2_rn(o[d][2 * h] * inv[h], o[d][2 * h + 1] * inv[h]);
-            }
+            for (int d = 0; d < 16; d++) dst[4 * d] = __floats2half2_rn(o[d][2 * h] * inv[h], o[d][2 * h + 1] * inv[h]);
           }
-        } else {
-          // a share of an item: the warp's first item goes to a place of its own, its last one over its buffers (nothing is in flight then)
-          const uint32_t which = i0 < w0 ? 0u : 1u;
-          float* dst = which ? tailp : headp;
-#pragma unroll
-          for (int d = 0; d < 16; d++) {
-            *reinterpret_cast<float2*>(dst + g * CA_LD + d * 8 + 2 * t4) = make_float2(o[d][0], o[d][1]);
-            *reinterpret_cast<float2*>(dst + (g + 8u) * CA_LD + d * 8 + 2 * t4) = make_float2(o[d][2], o[d][3]);
-          }
-          if (t4 == 0u) { sh.ml[warp][which][g] = make_float2(m[0], l[0]); sh.ml[warp][which][g + 8u] = make_float2(m[1], l[1]); }
-          if (lane == 0u) { CaEntry& e = sh.ent[warp * 2u + which]; e.i0 = i0; e.i1 = i0 + cur.v.np; e.b = cur.b; e.hk = cur.hk; e.rb = cur.rb; e.on = 1u; }
         }
+      } else {
+        // a share of an item: the warp's first item goes to a place of its own, its last one over its buffers (nothing is in flight then)
+        const uint32_t which = i0 < w0 ? 0u : 1u;
+        float* dst = which ? tailp : headp;
+#pragma unroll
+        for (int d = 0; d < 16; d++) {
+          *reinterpret_cast<float2*>(dst + g * CA_LD + d * 8 + 2 * t4) = make_float2(o[d][0], o[d][1]);
+          *reinterpret_cast<float2*>(dst + (g + 8u) * CA_LD + d * 8 + 2 * t4) = make_float2(o[d][2], o[d][3]);
+        }
+        if (t4 == 0u) { sh.ml[warp][which][g] = make_float2(m[0], l[0]); sh.ml[warp][which][g + 8u] = make_float2(m[1], l[1]); }
+        if (lane == 0u) { CaEntry& e = sh.ent[warp * 2u + which]; e.i0 = i0; e.i1 = i0 + cur.v.np; e.b = cur.b; e.hk = cur.hk; e.rb = cur.rb; e.on = 1u; }
       }
-      cur = nxt; nxt = aft; page = nxt_page; sc = nxt_sc; nxt_raw = aft_raw;
+      u += cnt;
+      cur = nxt; blk = nxt_blk;
     }
-    (void)page;
   }
   __syncthreads();
   // ---- the warps' shares of one item, merged in order; an item that is all here is finished, another one's partial result goes to memory
@@ -333,20 +346,20 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
   auto rows_of = [&](const CaEntry& e) { return min(16u, sh.seq[e.b].n * p.group - e.rb * 16u); };
   CaEntry open[2];                                                         // items that other blocks share: the one that began before, the one that goes on
   open[0].on = open[1].on = 0u;
-  for (uint32_t e0 = 0; e0 < CA_WARPS * 2u;) {
-    if (!sh.ent[e0].on) { e0++; continue; }
+  const uint64_t my_i0 = lane < CA_WARPS * 2u && sh.ent[lane].on ? sh.ent[lane].i0 : ~0ull;
+  for (uint32_t left = __ballot_sync(0xffffffffu, my_i0 != ~0ull); left;) {
+    const uint32_t e0 = __ffs(left) - 1u, run = __ballot_sync(0xffffffffu, my_i0 == __shfl_sync(0xffffffffu, my_i0, e0)) & left;      // (shares of one item stand together, in order)
+    left &= ~run;
     const CaEntry it = sh.ent[e0];
-    uint32_t e1 = e0 + 1u;
-    while (e1 < CA_WARPS * 2u && (!sh.ent[e1].on || sh.ent[e1].i0 == it.i0)) e1++;
     const bool whole = it.i0 >= u0 && it.i1 <= u1;
     const uint32_t slot = it.i0 < u0 ? 0u : 1u, n = rows_of(it);
-    if (!whole) open[slot] = it;
+    if (!whole) { if (slot) open[1] = it; else open[0] = it; }
     for (uint32_t r = warp; r < n; r += CA_WARPS) {
       float M = -INFINITY, L = 0.0f;
-      for (uint32_t e = e0; e < e1; e++) if (sh.ent[e].on) M = fmaxf(M, sh.ml[e >> 1][e & 1u][r].x);
+      for (uint32_t k = run; k; k &= k - 1u) { const uint32_t e = __ffs(k) - 1u; M = fmaxf(M, sh.ml[e >> 1][e & 1u][r].x); }
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (uint32_t e = e0; e < e1; e++) {
-        if (!sh.ent[e].on) continue;
+      for (uint32_t k = run; k; k &= k - 1u) {
+        const uint32_t e = __ffs(k) - 1u;
         const float2 ml = sh.ml[e >> 1][e & 1u][r];
         const float f = ml.x == -INFINITY ? 0.0f : at_ex2(ml.x - M);
         const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(gbase + ((e & 1u) ? (e >> 1) * CA_RING : CA_WARPS * CA_RING + (e >> 1) * CA_PART)) + r * CA_LD + 4u * lane);
@@ -360,7 +373,6 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
         if (lane == 0u) p.part_ml[at] = make_float2(M, L);
       }
     }
-    e0 = e1;
   }
   if (sh.failed) {                                                         // a wait ran out: the arrivals still have to be told, or the counters would not return to zero
     auto shared = [&](uint64_t u, uint32_t slot) {
@@ -369,21 +381,24 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
       CaEntry e;
       e.i0 = u - x.t; e.i1 = e.i0 + x.v.np; e.b = x.b; e.hk = x.hk; e.rb = x.rb;
       e.on = (e.i0 < u0 || e.i1 > u1) && slot == (e.i0 < u0 ? 0u : 1u) ? 1u : 0u;
-      open[slot] = e;
+      if (slot) open[1] = e; else open[0] = e;
     };
     shared(u0, 0u); shared(u1 - 1u, 1u);
   }
   if (!open[0].on && !open[1].on) return;
   // ---- items that cross blocks: the last of their blocks merges them, in block order
+  uint32_t own0 = 0u, own1 = 0u;                                           // thread k < 2: the first and the last block of open item k
+  if (tid < 2u) {
+    const uint64_t a = tid ? open[1].i0 : open[0].i0, b = tid ? open[1].i1 : open[0].i1;
+    if (tid ? open[1].on : open[0].on) { own0 = (uint32_t)deal_owner(a, U, G); own1 = (uint32_t)deal_owner(b - 1u, U, G); }
+  }
   __threadfence();
   __syncthreads();
   if (tid < 2u) {
     uint32_t mine = 0u;
-    const CaEntry it = open[tid];
-    if (it.on) {
-      const uint64_t c0 = deal_owner(it.i0, U, G), c1 = deal_owner(it.i1 - 1u, U, G);
-      mine = atomicAdd(p.count + c0, 1u) == (uint32_t)(c1 - c0) ? 1u : 0u;
-      if (mine) p.count[c0] = 0u;
+    if (tid ? open[1].on : open[0].on) {
+      mine = atomicAdd(p.count + own0, 1u) == own1 - own0 ? 1u : 0u;
+      if (mine) p.count[own0] = 0u;
     }
     sh.last[tid] = mine;
   }
@@ -391,7 +406,7 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
   __threadfence();
   for (uint32_t k = 0; k < 2u; k++) {
     if (!sh.last[k]) continue;
-    const CaEntry it = open[k];
+    const CaEntry it = k ? open[1] : open[0];
     const uint32_t c0 = (uint32_t)deal_owner(it.i0, U, G), c1 = (uint32_t)deal_owner(it.i1 - 1u, U, G), n = rows_of(it);
     auto at = [&](uint32_t c, uint32_t r) { return ((size_t)c * 2u + (c == c0 ? 1u : 0u)) * 16u + r; };      // (in the item's first block it is the item that goes on)
     for (uint32_t r = warp; r < n; r += CA_WARPS) {
