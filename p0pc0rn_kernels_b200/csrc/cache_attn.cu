@@ -88,7 +88,7 @@ extern "C" int p0p_cache_attention(p0p_ctx* c, const p0p_cache_attn_args* a) {
   if ((uint64_t)M * p.group > 0x7fffffffu) return fail(c, -5, "cacheAttention: too many rows for one call");
   p.scale_log2 = (a->scale > 0.0f ? a->scale : 1.0f / std::sqrt(128.0f)) * 1.4426950408889634f;
   DeviceGuard g(c->device);
-  const uint32_t G = std::min<uint32_t>((uint32_t)c->prop.multiProcessorCount, c->n_counters);
+  const uint32_t G = std::min<uint32_t>((uint32_t)c->prop.multiProcessorCount, c->n_counters / 16u);
   // Which kernel a sequence is for depends on its number of new tokens.  Without row offsets the host knows it; with them it knows the most any
   // sequence has, if the caller says so, and where that is many, both kernels run, each for its sequences.
   const uint64_t most = (uint64_t)p.group * (p.c.rows ? (a->max_new ? std::min(a->max_new, M) : M) : p.c.each);

@@ -81,15 +81,27 @@ P0P_HD uint64_t deal_first(uint64_t c, uint64_t U, uint64_t G) { return div_64(c
 P0P_HD uint64_t deal_owner(uint64_t u, uint64_t U, uint64_t G) { return div_64((u + 1u) * G - 1u, U); }
 
 // The split-key attention's units: per sequence [kv head][block of 16 query rows][visible page], one sequence after the other.  The query rows of
-// the `group` heads that share a kv head are one matrix of n * group rows, query by query.
+// the `group` heads that share a kv head are one matrix of n * group rows, query by query.  An item (all pages of a kv head and row block) costs one
+// unit before its pages: its queries and page numbers arrive, its result leaves.
 struct CacheGeo { uint32_t Hkv, group, seqs, window, sinks; };
 P0P_HD uint64_t cache_units(const CacheSeq& s, const CacheGeo& g) {
-  return s.n ? (uint64_t)g.Hkv * ((s.n * g.group + 15u) >> 4) * cache_visible(s, g.window, g.sinks).np : 0u;
+  return s.n ? (uint64_t)g.Hkv * ((s.n * g.group + 15u) >> 4) * (1u + cache_visible(s, g.window, g.sinks).np) : 0u;
+}
+// how many blocks share U units of `items` items: all, unless that cuts items that few blocks (of 8 warps) would do.  Where there are fewer items than blocks
+// each gets the same number of them, so that items of one length are cut between blocks as little as can be.
+P0P_HD uint64_t cache_workers(uint64_t U, uint64_t items, uint64_t most) {
+  uint64_t g = most;
+  if (items && items <= most) {
+    const uint64_t fit = most / items, per = div_64(U, items), want = per / 9u + (per % 9u ? 1u : 0u);      // (an item's cost: a warp's page each, and the unit before them)
+    g = items * (want < fit ? want : fit);
+  }
+  if (g > most) g = most;
+  return g > U ? U : g;
 }
 // where a warp stands.  pre[b]: units before sequence b; seq[b]: the sequences.
 struct CacheCursor {
   CacheSeq s; CacheVis v;
-  uint32_t b, hk, rb, rbs, t;
+  uint32_t b, hk, rb, rbs, at;      // at 0: before the item's first page; at k > 0: at page k - 1
   P0P_HD void sequence(const CacheGeo& g, const CacheSeq* seq, uint32_t b_) {
     b = b_; s = seq[b];
     v = cache_visible(s, g.window, g.sinks);
@@ -99,15 +111,13 @@ struct CacheCursor {
     uint32_t lo = 0u, hi = g.seqs - 1u;                                   // the first sequence that ends behind u: it is not empty
     while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (pre[mid + 1u] > u) hi = mid; else lo = mid + 1u; }
     sequence(g, seq, lo);
-    const uint64_t r = u - pre[lo], per = (uint64_t)rbs * v.np;
-    hk = (uint32_t)div_64(r, per);
-    const uint64_t x = r - hk * per;
-    rb = (uint32_t)div_64(x, v.np); t = (uint32_t)(x - (uint64_t)rb * v.np);
+    const uint64_t item = div_64(u - pre[lo], v.np + 1u);
+    at = (uint32_t)(u - pre[lo] - item * (v.np + 1u));
+    hk = (uint32_t)div_64(item, rbs); rb = (uint32_t)(item - (uint64_t)hk * rbs);
   }
-  // the next unit, which there has to be
-  P0P_HD void next(const CacheGeo& g, const uint64_t* pre, const CacheSeq* seq) {
-    if (++t < v.np) return;
-    t = 0u;
+  // the beginning of the next item, which there has to be
+  P0P_HD void next_item(const CacheGeo& g, const uint64_t* pre, const CacheSeq* seq) {
+    at = 0u;
     if (++rb < rbs) return;
     rb = 0u;
     if (++hk < g.Hkv) return;
@@ -116,8 +126,8 @@ struct CacheCursor {
     while (n + 1u < g.seqs && pre[n + 1u] == pre[n]) n++;
     if (n < g.seqs) sequence(g, seq, n);
   }
-  P0P_HD uint32_t page() const { return cache_vis_page(v, t); }
-  P0P_HD bool tail() const { return page() == s.L / CACHE_PAGE; }
+  P0P_HD uint32_t t() const { return at ? at - 1u : 0u; }
+  P0P_HD bool tail(uint32_t k) const { return cache_vis_page(v, k) == s.L / CACHE_PAGE; }      // is visible page k the unfinished one?
 };
 
 // The tensor-memory attention's work: an item = up to 2 * qpt queries of a sequence (qpt: those whose heads of one kv head fill a tile of 128

@@ -14,8 +14,8 @@
 // contexts of any mix of lengths fill the machine, and the numbers on the device decide how: nothing but the launch is fixed on the host.
 // A warp streams its pages through two 8-KB buffers of its own (K, V) by bulk copies, one page ahead.  An item (all pages of a
 // sequence, kv head and row block) that lies within one warp's share is finished there; otherwise partial results (maximum, sum, O)
-// are merged in the block, and across blocks by the one that arrives last (a counter per item that crosses blocks; it resets it), in
-// order: deterministic, one launch.
+// are merged in the block, and across blocks by the warp that arrives last (a counter per row of an item that crosses blocks; it resets
+// it), in order: deterministic, one launch.
 // Bound: one pass over the visible codes (HBM).
 #pragma once
 #include <cuda_fp16.h>
@@ -23,6 +23,7 @@
 
 #include "cache_dev.cuh"
 #include "k_attn.cuh"
+#include "umma.cuh"
 
 namespace p0p {
 
@@ -34,11 +35,11 @@ struct CacheAttnP {
   float scale_log2;      // scale * log2(e)
   float* part;           // [block][2][16][128] unnormalised O, then (maximum, sum) [block][2][16]
   float2* part_ml;
-  uint32_t* count;       // [block] arrivals, zero between calls
+  uint32_t* count;       // [block][16] arrivals, zero between calls
 };
 
 constexpr uint32_t CA_WARPS = 8u, CA_LD = 132u, CA_RING = 2u * CACHE_BLOCK, CA_PART = 16u * CA_LD * 4u;
-struct CaEntry { uint64_t i0, i1; uint32_t b, hk, rb, on; };              // a partial result of a warp: its item's units, the item
+struct CaEntry { uint64_t i0, i1; uint32_t b, hk, rb, on; };              // a partial result of a warp: the units of its item's pages, the item
 struct CaShared {
   uint64_t pre[CACHE_MAX_SEQS + 1];                                       // units before each sequence
   CacheSeq seq[CACHE_MAX_SEQS];
@@ -46,7 +47,7 @@ struct CaShared {
   CaEntry ent[CA_WARPS * 2];
   uint64_t bars[CA_WARPS][2];
   uint64_t warp_sum[CA_WARPS];
-  uint32_t last[2], failed;
+  uint32_t items, failed;
 };
 constexpr uint32_t CA_SMEM = CA_WARPS * (CA_RING + CA_PART) + (uint32_t)sizeof(CaShared) + 128u;
 static_assert(CA_SMEM <= 232448u, "shared memory");
@@ -72,7 +73,8 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
   const uint32_t bar_k = smem_u32(&sh.bars[warp][0]), bar_v = smem_u32(&sh.bars[warp][1]);
   if (lane == 0u) { mbar_init(bar_k, 1u); mbar_init(bar_v, 1u); }
   if (tid < CA_WARPS * 2u) sh.ent[tid].on = 0u;
-  if (tid == 0u) sh.failed = 0u;
+  if (tid == 0u) { sh.failed = 0u; sh.items = 0u; }
+  __syncthreads();
   fence_mbar_init();
   grid_dependency_wait();
   grid_launch_dependents();
@@ -84,7 +86,7 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
     if (b < p.c.seqs) {
       const CacheSeq s = cache_seq(p.c, b);
       sh.seq[b] = s;
-      if (s.n && (uint64_t)s.n * p.group <= p.max_rows) c = cache_units(s, geo);
+      if (s.n && (uint64_t)s.n * p.group <= p.max_rows) { c = cache_units(s, geo); atomicAdd(&sh.items, (uint32_t)min((uint64_t)p.c.Hkv * ((s.n * p.group + 15u) >> 4), (uint64_t)1u << 20)); }
     }
     uint64_t inc = c;
 #pragma unroll
@@ -97,11 +99,13 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
     if (b < p.c.seqs) { sh.pre[b + 1u] = before + inc; if (b == 0u) sh.pre[0] = 0u; }
     __syncthreads();
   }
-  const uint64_t G = U < gridDim.x ? U : gridDim.x;
+  const uint64_t G = cache_workers(U, sh.items, gridDim.x);
   if (blockIdx.x >= G) return;
-  const uint64_t u0 = deal_first(blockIdx.x, U, G), u1 = deal_first(blockIdx.x + 1u, U, G), here = u1 - u0, W = here < CA_WARPS ? here : CA_WARPS;
-  if (warp < W) {
-    const uint64_t w0 = u0 + deal_first(warp, here, W), w1 = u0 + deal_first(warp + 1u, here, W);
+  // (both ends by one division, in two lanes; eight shares by a shift)
+  const uint64_t end = deal_first(blockIdx.x + (lane & 1u), U, G);
+  const uint64_t u0 = __shfl_sync(0xffffffffu, end, 0), u1 = __shfl_sync(0xffffffffu, end, 1), here = u1 - u0;
+  if (warp < here) {
+    const uint64_t w0 = u0 + (here < CA_WARPS ? warp : warp * here / CA_WARPS), w1 = u0 + (here < CA_WARPS ? warp + 1u : (warp + 1u) * here / CA_WARPS);
     CacheCursor cur;
     cur.seek(geo, sh.pre, sh.seq, w0);
     // pages of a row's blocks of codes, by the lane's page of 32: as the table has them, then checked, as blocks (page * Hkv + kv head)
@@ -113,13 +117,13 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
       return raw * p.c.Hkv + c.hk;
     };
     auto fetch = [&](uint32_t block, uint32_t w) {                         // K (w 0) or V of a block of codes
-      if (lane == 0u) {
+      if (elect_one()) {
         mbar_expect_tx(w ? bar_v : bar_k, CACHE_BLOCK);
         bulk_g2s(ring + w * CACHE_BLOCK, p.c.codes + ((size_t)block * 2u + w) * CACHE_BLOCK, CACHE_BLOCK, w ? bar_v : bar_k);
       }
     };
     auto fetch_tail = [&](const CacheCursor& c, uint32_t w) {              // of a tail, into both buffers
-      if (lane == 0u) {
+      if (elect_one()) {
         mbar_expect_tx(w ? bar_v : bar_k, 2u * CACHE_BLOCK);
         bulk_g2s(ring, p.c.tail + (((size_t)c.b * p.c.Hkv + c.hk) * 2u + w) * CACHE_BLOCK, 2u * CACHE_BLOCK, w ? bar_v : bar_k);
       }
@@ -171,38 +175,45 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
       }
       l[0] = fmaf(zp[0], inv_v, l[0]); l[1] = fmaf(zp[2], inv_v, l[1]);
     };
-    // ---- the first page is on its way before anything else
-    uint32_t blk = block_of(cur, raw_at(cur, cur.t + lane));               // this lane's page of the 32 at hand
-    {
-      const uint32_t first = __shfl_sync(0xffffffffu, blk, 0);
-      if (cur.tail()) fetch_tail(cur, 0u);
-      else { fetch(first, 0u); fetch(first, 1u); }
-    }
-    for (uint64_t u = w0; u < w1;) {
+    // a thread's two query rows (rows past the end repeat the last one; they are not stored)
+    auto queries = [&](const CacheCursor& c) {
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; h++) {
+        const uint32_t r = min(c.rb * 16u + h * 8u + g, c.s.n * p.group - 1u), i = r / p.group;
+        const uint4* q = reinterpret_cast<const uint4*>(p.Q + ((size_t)(c.hk * p.group + (r - i * p.group)) * p.ldq + c.s.r0 + i) * 128u + t4 * 16u);
+#pragma unroll
+        for (uint32_t k = 0; k < 2u; k++) {
+          const uint4 a = ld_now(q + k * 8u), z = ld_now(q + k * 8u + 1u);
+          qa[k * 4u][h] = a.x; qa[k * 4u][2u + h] = a.y; qa[k * 4u + 1u][h] = a.z; qa[k * 4u + 1u][2u + h] = a.w;
+          qa[k * 4u + 2u][h] = z.x; qa[k * 4u + 2u][2u + h] = z.y; qa[k * 4u + 3u][h] = z.z; qa[k * 4u + 3u][2u + h] = z.w;
+        }
+      }
+    };
+    // ---- the first page is on its way before anything else.  (What has to come from memory is asked for before any of it is looked at: one after the
+    // other, an item's loads took 6000 cycles.)
+    const bool any = cur.at != 0u || w1 - w0 > 1u;
+    uint32_t raw = any ? raw_at(cur, cur.t() + lane) : 0u;
+    if (any) queries(cur);
+    uint32_t blk = block_of(cur, raw);                                     // this lane's page of the 32 at hand
+    auto fetch_first = [&](const CacheCursor& c, uint32_t block0) {
+      if (c.tail(c.t())) fetch_tail(c, 0u);
+      else { fetch(block0, 0u); fetch(block0, 1u); }
+    };
+    const uint32_t first = __shfl_sync(0xffffffffu, blk, 0);
+    if (any) fetch_first(cur, first);
+    for (uint64_t u = w0; any;) {
       // ---- an item, or this warp's share of it: pages t .. t + cnt - 1, of which the last may be the tail
-      const uint64_t i0 = u - cur.t;
-      const uint32_t cnt = (uint32_t)min((uint64_t)(cur.v.np - cur.t), w1 - u), rows = cur.s.n * p.group, p0 = cur.s.L - cur.s.n, p1 = cur.s.L - 1u;
-      const bool done = cur.t + cnt == cur.v.np, has_tail = done && (cur.s.L & (CACHE_PAGE - 1u)) != 0u, more = u + cnt < w1;
+      const uint64_t i0 = u - cur.at, end = min(u + (cur.v.np + 1u - cur.at), w1);
+      const uint32_t t = cur.t(), cnt = (uint32_t)(end - u) - (cur.at ? 0u : 1u), rows = cur.s.n * p.group, p0 = cur.s.L - cur.s.n, p1 = cur.s.L - 1u;
+      const bool done = t + cnt == cur.v.np, has_tail = done && (cur.s.L & (CACHE_PAGE - 1u)) != 0u, more = end + 1u < w1;      // (a share may end behind the unit that stands before an item's pages)
       const uint32_t codes = cnt - (has_tail ? 1u : 0u);
-      // (everything that has to come from memory is asked for before any of it is looked at: one after the other these loads took 6000 cycles an item)
       float2 sc = ld_now(p.c.scales + blk), sc2 = sc;
       CacheCursor nxt = cur;
       uint32_t nxt_raw = 0u, nxt_blk = 0u, blk2 = 0u, raw2 = 0u;
-      if (more) { nxt.t = nxt.v.np - 1u; nxt.next(geo, sh.pre, sh.seq); nxt_raw = raw_at(nxt, lane); }
-      const bool nxt_tail = more && nxt.tail();
-      // this thread's two query rows (rows past the end repeat the last one; they are not stored)
+      if (more) { nxt.next_item(geo, sh.pre, sh.seq); nxt_raw = raw_at(nxt, lane); }
+      const bool nxt_tail = more && nxt.tail(0u);
 #pragma unroll
-      for (uint32_t h = 0; h < 2u; h++) {
-        const uint32_t r = min(cur.rb * 16u + h * 8u + g, rows - 1u), i = r / p.group;
-        pos[h] = p0 + i;
-        const uint4* q = reinterpret_cast<const uint4*>(p.Q + ((size_t)(cur.hk * p.group + (r - i * p.group)) * p.ldq + cur.s.r0 + i) * 128u + t4 * 16u);
-#pragma unroll
-        for (uint32_t k = 0; k < 2u; k++) {
-          const uint4 a = ld_now(q + k * 8u), c = ld_now(q + k * 8u + 1u);
-          qa[k * 4u][h] = a.x; qa[k * 4u][2u + h] = a.y; qa[k * 4u + 1u][h] = a.z; qa[k * 4u + 1u][2u + h] = a.w;
-          qa[k * 4u + 2u][h] = c.x; qa[k * 4u + 2u][2u + h] = c.y; qa[k * 4u + 3u][h] = c.z; qa[k * 4u + 3u][2u + h] = c.w;
-        }
-      }
+      for (uint32_t h = 0; h < 2u; h++) pos[h] = p0 + min(cur.rb * 16u + h * 8u + g, rows - 1u) / p.group;
       {
         float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -218,7 +229,7 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
         const uint32_t at = i & 31u;
         if (at == 0u) {                                                    // 32 pages at a time: the next ones' numbers are asked for here, their scales half way
           if (i > 0u) { blk = blk2; sc = sc2; }
-          raw2 = raw_at(cur, cur.t + i + 32u + lane);
+          raw2 = raw_at(cur, t + i + 32u + lane);
         }
         if (at == 16u) { blk2 = block_of(cur, raw2); sc2 = ld_now(p.c.scales + blk2); }
         const float ks = __shfl_sync(0xffffffffu, sc.x, at), vs = __shfl_sync(0xffffffffu, sc.y, at);
@@ -244,7 +255,7 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
         }
         __syncwarp();                                                      // the K buffer is read
         if (follows) fetch(next, 0u);
-        weigh(cache_vis_page(cur.v, cur.t + i), p0, p1, p.scale_log2 * ks * 16777216.0f, ca_lg2(vs), __fdividef(1.0f, vs));
+        weigh(cache_vis_page(cur.v, t + i), p0, p1, p.scale_log2 * ks * 16777216.0f, ca_lg2(vs), __fdividef(1.0f, vs));
         const float c0 = -0x1p-17f * zp[0], c1 = -0x1p-17f * zp[2];        // -128 * 2^-24 each
         if (!wait_v()) break;
 #pragma unroll
@@ -308,7 +319,8 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
         else if (more) { fetch(nxt_block, 0u); fetch(nxt_block, 1u); }
       }
       // ---- the end of the item, or of this warp's share
-      if (done && i0 >= w0) {
+      if (more) queries(nxt);                                              // (on their way while the result leaves)
+      if (done && i0 + 1u >= w0) {
         const float inv[2] = {l[0] > 0.0f ? 1.0f / l[0] : l[0], l[1] > 0.0f ? 1.0f / l[1] : l[1]};
 #pragma unroll
         for (uint32_t h = 0; h < 2u; h++) {
@@ -321,7 +333,7 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
         }
       } else {
         // a share of an item: the warp's first item goes to a place of its own, its last one over its buffers (nothing is in flight then)
-        const uint32_t which = i0 < w0 ? 0u : 1u;
+        const uint32_t which = i0 + 1u < w0 ? 0u : 1u;
         float* dst = which ? tailp : headp;
 #pragma unroll
         for (int d = 0; d < 16; d++) {
@@ -329,32 +341,67 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
           *reinterpret_cast<float2*>(dst + (g + 8u) * CA_LD + d * 8 + 2 * t4) = make_float2(o[d][2], o[d][3]);
         }
         if (t4 == 0u) { sh.ml[warp][which][g] = make_float2(m[0], l[0]); sh.ml[warp][which][g + 8u] = make_float2(m[1], l[1]); }
-        if (lane == 0u) { CaEntry& e = sh.ent[warp * 2u + which]; e.i0 = i0; e.i1 = i0 + cur.v.np; e.b = cur.b; e.hk = cur.hk; e.rb = cur.rb; e.on = 1u; }
+        if (lane == 0u) { CaEntry& e = sh.ent[warp * 2u + which]; e.i0 = i0 + 1u; e.i1 = i0 + 1u + cur.v.np; e.b = cur.b; e.hk = cur.hk; e.rb = cur.rb; e.on = 1u; }
       }
-      u += cnt;
+      if (!more) break;
+      u = end;
       cur = nxt; blk = nxt_blk;
     }
   }
   __syncthreads();
-  // ---- the warps' shares of one item, merged in order; an item that is all here is finished, another one's partial result goes to memory
-  auto store = [&](uint32_t b, uint32_t hk, uint32_t rb, uint32_t r, float4 v) {      // columns 4 lane .. of row r of the row block
-    const CacheSeq q = sh.seq[b];
-    const uint32_t x = rb * 16u + r, i = x / p.group;
-    __half2* d = reinterpret_cast<__half2*>(p.O + (size_t)(q.r0 + i) * p.ldo + (hk * p.group + (x - i * p.group)) * 128u + 4u * lane);
-    d[0] = __floats2half2_rn(v.x, v.y); d[1] = __floats2half2_rn(v.z, v.w);
+  // ---- the warps' shares of one item, merged in order, a row per warp; an item that is all here is finished.  A row of another one goes to memory, and the
+  // warp that brings its last share merges the blocks' shares, in order.  (Row by row, with one release and acquire each, instead of a fence and a
+  // barrier of the block: 6 -> 2 us from the last page to the end.)
+  auto store = [&](const CaEntry& it, uint32_t r, float L, float4 v) {      // columns 4 lane .. of row r of the row block
+    const CacheSeq q = sh.seq[it.b];
+    const uint32_t x = it.rb * 16u + r, i = x / p.group;
+    const float inv = L > 0.0f ? 1.0f / L : L;
+    __half2* d = reinterpret_cast<__half2*>(p.O + (size_t)(q.r0 + i) * p.ldo + (it.hk * p.group + (x - i * p.group)) * 128u + 4u * lane);
+    d[0] = __floats2half2_rn(v.x * inv, v.y * inv); d[1] = __floats2half2_rn(v.z * inv, v.w * inv);
   };
   auto rows_of = [&](const CaEntry& e) { return min(16u, sh.seq[e.b].n * p.group - e.rb * 16u); };
-  CaEntry open[2];                                                         // items that other blocks share: the one that began before, the one that goes on
-  open[0].on = open[1].on = 0u;
+  // one arrival at row r of an item of blocks c0 .. c1; true for the last one
+  auto arrive = [&](uint32_t c0, uint32_t c1, uint32_t r) {
+    uint32_t last = 0u;
+    __syncwarp();
+    if (lane == 0u) {
+      uint32_t* at = p.count + c0 * 16u + r;
+      uint32_t before;
+      asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(at) : "memory");
+      last = before == c1 - c0 ? 1u : 0u;
+      if (last) *at = 0u;
+    }
+    last = __shfl_sync(0xffffffffu, last, 0);
+    __syncwarp();
+    return last != 0u;
+  };
+  if (sh.failed) {                                                         // a wait ran out: the arrivals still have to be told, or the counters would not return to zero
+    if (warp == 0u)
+      for (uint32_t k = 0; k < 2u; k++) {
+        CacheCursor x;
+        x.seek(geo, sh.pre, sh.seq, k ? u1 - 1u : u0);
+        const uint64_t i0 = (k ? u1 - 1u : u0) - x.at + 1u, i1 = i0 + x.v.np;      // the units of the item's pages
+        if (i0 >= u1 || (i0 >= u0 && i1 <= u1) || (k == 1u && i0 < u0)) continue;  // (nothing of it here; all of it; counted already)
+        for (uint32_t r = 0; r < min(16u, x.s.n * p.group - x.rb * 16u); r++) arrive((uint32_t)deal_owner(i0, U, G), (uint32_t)deal_owner(i1 - 1u, U, G), r);
+      }
+    return;
+  }
   const uint64_t my_i0 = lane < CA_WARPS * 2u && sh.ent[lane].on ? sh.ent[lane].i0 : ~0ull;
+  uint32_t before = 0u;                                                    // rows of the items before
   for (uint32_t left = __ballot_sync(0xffffffffu, my_i0 != ~0ull); left;) {
     const uint32_t e0 = __ffs(left) - 1u, run = __ballot_sync(0xffffffffu, my_i0 == __shfl_sync(0xffffffffu, my_i0, e0)) & left;      // (shares of one item stand together, in order)
     left &= ~run;
     const CaEntry it = sh.ent[e0];
     const bool whole = it.i0 >= u0 && it.i1 <= u1;
-    const uint32_t slot = it.i0 < u0 ? 0u : 1u, n = rows_of(it);
-    if (!whole) { if (slot) open[1] = it; else open[0] = it; }
-    for (uint32_t r = warp; r < n; r += CA_WARPS) {
+    const uint32_t n = rows_of(it), r0 = (warp - before) & (CA_WARPS - 1u);
+    before += n;
+    if (r0 >= n) continue;
+    uint32_t c0 = 0u, c1 = 0u;
+    if (!whole) {
+      const uint32_t own = (uint32_t)deal_owner(lane & 1u ? it.i1 - 1u : it.i0, U, G);
+      c0 = __shfl_sync(0xffffffffu, own, 0); c1 = __shfl_sync(0xffffffffu, own, 1);
+    }
+    for (uint32_t r = r0; r < n; r += CA_WARPS) {
       float M = -INFINITY, L = 0.0f;
       for (uint32_t k = run; k; k &= k - 1u) { const uint32_t e = __ffs(k) - 1u; M = fmaxf(M, sh.ml[e >> 1][e & 1u][r].x); }
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -366,69 +413,31 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
         L += f * ml.y;
         acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
       }
-      if (whole) { const float inv = L > 0.0f ? 1.0f / L : L; store(it.b, it.hk, it.rb, r, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv)); }
-      else {
-        const size_t at = ((size_t)blockIdx.x * 2u + slot) * 16u + r;
-        *reinterpret_cast<float4*>(p.part + at * 128u + 4u * lane) = acc;
-        if (lane == 0u) p.part_ml[at] = make_float2(M, L);
-      }
-    }
-  }
-  if (sh.failed) {                                                         // a wait ran out: the arrivals still have to be told, or the counters would not return to zero
-    auto shared = [&](uint64_t u, uint32_t slot) {
-      CacheCursor x;
-      x.seek(geo, sh.pre, sh.seq, u);
-      CaEntry e;
-      e.i0 = u - x.t; e.i1 = e.i0 + x.v.np; e.b = x.b; e.hk = x.hk; e.rb = x.rb;
-      e.on = (e.i0 < u0 || e.i1 > u1) && slot == (e.i0 < u0 ? 0u : 1u) ? 1u : 0u;
-      if (slot) open[1] = e; else open[0] = e;
-    };
-    shared(u0, 0u); shared(u1 - 1u, 1u);
-  }
-  if (!open[0].on && !open[1].on) return;
-  // ---- items that cross blocks: the last of their blocks merges them, in block order
-  uint32_t own0 = 0u, own1 = 0u;                                           // thread k < 2: the first and the last block of open item k
-  if (tid < 2u) {
-    const uint64_t a = tid ? open[1].i0 : open[0].i0, b = tid ? open[1].i1 : open[0].i1;
-    if (tid ? open[1].on : open[0].on) { own0 = (uint32_t)deal_owner(a, U, G); own1 = (uint32_t)deal_owner(b - 1u, U, G); }
-  }
-  __threadfence();
-  __syncthreads();
-  if (tid < 2u) {
-    uint32_t mine = 0u;
-    if (tid ? open[1].on : open[0].on) {
-      mine = atomicAdd(p.count + own0, 1u) == own1 - own0 ? 1u : 0u;
-      if (mine) p.count[own0] = 0u;
-    }
-    sh.last[tid] = mine;
-  }
-  __syncthreads();
-  __threadfence();
-  for (uint32_t k = 0; k < 2u; k++) {
-    if (!sh.last[k]) continue;
-    const CaEntry it = k ? open[1] : open[0];
-    const uint32_t c0 = (uint32_t)deal_owner(it.i0, U, G), c1 = (uint32_t)deal_owner(it.i1 - 1u, U, G), n = rows_of(it);
-    auto at = [&](uint32_t c, uint32_t r) { return ((size_t)c * 2u + (c == c0 ? 1u : 0u)) * 16u + r; };      // (in the item's first block it is the item that goes on)
-    for (uint32_t r = warp; r < n; r += CA_WARPS) {
-      float M = -INFINITY;
-      for (uint32_t c = c0 + lane; c <= c1; c += 32u) M = fmaxf(M, __ldcg(&p.part_ml[at(c, r)]).x);
-#pragma unroll
-      for (uint32_t x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float L = 0.0f;
-      for (uint32_t b = c0; b <= c1; b += 8u) {
+      if (whole) { store(it, r, L, acc); continue; }
+      // (a block has two places: 0 for the item that began before it, 1 for the one that goes on behind it)
+      auto at = [&](uint32_t c) { return ((size_t)c * 2u + (c == c0 ? 1u : 0u)) * 16u + r; };
+      const size_t here_at = ((size_t)blockIdx.x * 2u + (it.i0 < u0 ? 0u : 1u)) * 16u + r;
+      *reinterpret_cast<float4*>(p.part + here_at * 128u + 4u * lane) = acc;
+      if (lane == 0u) p.part_ml[here_at] = make_float2(M, L);
+      if (!arrive(c0, c1, r)) continue;
+      M = -INFINITY; L = 0.0f; acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (uint32_t c = c0; c <= c1; c += 8u) {                            // (eight blocks' shares at a time, the running maximum as elsewhere)
         float4 v[8]; float2 ml[8];
+        float top = M;
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; i++) { const size_t x = at(min(b + i, c1), r); v[i] = __ldcg(reinterpret_cast<const float4*>(p.part + x * 128u) + lane); ml[i] = __ldcg(&p.part_ml[x]); }
+        for (uint32_t i = 0; i < 8u; i++) { const size_t x = at(min(c + i, c1)); v[i] = __ldcg(reinterpret_cast<const float4*>(p.part + x * 128u) + lane); ml[i] = __ldcg(&p.part_ml[x]); }
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) top = fmaxf(top, ml[i].x);
+        const float a = M == -INFINITY ? 0.0f : at_ex2(M - top);
+        M = top; L *= a; acc.x *= a; acc.y *= a; acc.z *= a; acc.w *= a;
 #pragma unroll
         for (uint32_t i = 0; i < 8u; i++) {
-          const float f = b + i <= c1 && ml[i].x != -INFINITY ? at_ex2(ml[i].x - M) : 0.0f;
+          const float f = c + i <= c1 && ml[i].x != -INFINITY ? at_ex2(ml[i].x - M) : 0.0f;
           L += f * ml[i].y;
           acc.x += f * v[i].x; acc.y += f * v[i].y; acc.z += f * v[i].z; acc.w += f * v[i].w;
         }
       }
-      const float inv = L > 0.0f ? 1.0f / L : L;
-      store(it.b, it.hk, it.rb, r, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+      store(it, r, L, acc);
     }
   }
 }

@@ -67,13 +67,13 @@ int main() {
       if (hidden && listed[pg]) CHECK(cache_page_masked(pg, s.L - s.n, s.L - 1, window, sinks));
     }
   }
-  for (int it = 0; it < 600; it++) {   // the units: every worker's walk, and whom a unit belongs to
+  for (int it = 0; it < 600; it++) {   // the units: every worker's items and pages, and whom a unit belongs to
     const uint32_t seqs = 1 + rnd(rnd(2) ? 3 : 40);
     const CacheGeo g{1 + rnd(9), 1 + rnd(20), seqs, rnd(2) ? 1 + rnd(300) : 0, rnd(70)};
     std::vector<CacheSeq> seq(seqs);
     std::vector<uint64_t> pre(seqs + 1, 0);
-    uint64_t U = 0;
-    struct Unit { uint32_t b, hk, rb, t; };
+    uint64_t U = 0, pages = 0;
+    struct Unit { uint32_t b, hk, rb, at; };
     std::vector<Unit> all;
     for (uint32_t b = 0; b < seqs; b++) {
       seq[b] = CacheSeq{0, rnd(3) ? rnd(3) : rnd(40), 0};
@@ -81,11 +81,14 @@ int main() {
       U += cache_units(seq[b], g); pre[b + 1] = U;
       if (!seq[b].n) continue;
       const uint32_t np = cache_visible(seq[b], g.window, g.sinks).np;
-      for (uint32_t h = 0; h < g.Hkv; h++) for (uint32_t rb = 0; rb * 16 < seq[b].n * g.group; rb++) for (uint32_t t = 0; t < np; t++) all.push_back({b, h, rb, t});
+      for (uint32_t h = 0; h < g.Hkv; h++) for (uint32_t rb = 0; rb * 16 < seq[b].n * g.group; rb++) { pages += np; for (uint32_t t = 0; t <= np; t++) all.push_back({b, h, rb, t}); }
     }
     CHECK(U == all.size());
     if (!U) continue;
-    const uint64_t G = U < 148 ? U : 148;
+    uint64_t items = 0, seen = 0;
+    for (const Unit& y : all) items += y.at == 0;
+    const uint64_t G = cache_workers(U, items, 148);
+    CHECK(G >= 1 && G <= U && G <= 148);
     CHECK(deal_first(0, U, G) == 0 && deal_first(G, U, G) == U);
     for (uint64_t c = 0; c < G; c++) {
       const uint64_t u0 = deal_first(c, U, G), u1 = deal_first(c + 1, U, G), n = u1 - u0, W = n < 8 ? n : 8;
@@ -96,13 +99,22 @@ int main() {
         CHECK(w1 > w0);
         CacheCursor x;
         x.seek(g, pre.data(), seq.data(), w0);
-        for (uint64_t u = w0; u < w1; u++) {
-          CHECK(x.b == all[u].b && x.hk == all[u].hk && x.rb == all[u].rb && x.t == all[u].t && x.page() <= (x.s.L - 1) / 64);
-          CHECK(x.tail() == (x.s.L % 64 != 0 && x.page() == x.s.L / 64) && (!x.tail() || x.t + 1 == x.v.np));
-          if (u + 1 < w1) x.next(g, pre.data(), seq.data());
+        for (uint64_t u = w0; u < w1;) {                  // as the kernel walks: item by item
+          const Unit& y = all[u];
+          CHECK(x.b == y.b && x.hk == y.hk && x.rb == y.rb && x.at == y.at);
+          const uint64_t end = u + (x.v.np + 1 - x.at) < w1 ? u + (x.v.np + 1 - x.at) : w1;
+          const uint32_t first = x.t(), cnt = (uint32_t)(end - u) - (x.at ? 0 : 1);
+          for (uint32_t k = first; k < first + cnt; k++, seen++) {
+            const Unit& z = all[u + (x.at ? 0 : 1) + (k - first)];
+            CHECK(z.b == x.b && z.hk == x.hk && z.rb == x.rb && z.at == k + 1 && cache_vis_page(x.v, k) <= (x.s.L - 1) / 64);
+            CHECK(x.tail(k) == (x.s.L % 64 != 0 && k + 1 == x.v.np));
+          }
+          u = end;
+          if (u < w1) x.next_item(g, pre.data(), seq.data());
         }
       }
     }
+    CHECK(seen == pages);
   }
   {   // score columns: every key of a page once, in the order of a lane's V elements
     std::vector<int> seen(64, 0);
