@@ -12,7 +12,7 @@
 // Work: a unit = one visible page of one kv head for up to 16 query rows (the rows of all heads that share the kv head, query-major; more
 // rows are more row blocks).  All units of all sequences in one row are dealt out evenly: to blocks (one per SM), within a block to its 8 warps.  So
 // contexts of any mix of lengths fill the machine, and the numbers on the device decide how: nothing but the launch is fixed on the host.
-// A warp streams its pages through two 8-KB buffers of its own (K, V) by bulk copies, one page ahead.  An item (all pages of a
+// A warp streams its pages through two 8-KB buffers of its own by bulk copies, one page ahead.  An item (all pages of a
 // sequence, kv head and row block) that lies within one warp's share is finished there; otherwise partial results (maximum, sum, O)
 // are merged in the block, and across blocks by the warp that arrives last (a counter per row of an item that crosses blocks; it resets
 // it), in order: deterministic, one launch.
@@ -70,8 +70,8 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
   const CacheGeo geo{p.c.Hkv, p.group, p.c.seqs, p.window, p.sinks};
   float* const headp = reinterpret_cast<float*>(gbase + CA_WARPS * CA_RING + warp * CA_PART);
   float* const tailp = reinterpret_cast<float*>(gbase + warp * CA_RING);
-  const uint32_t bar_k = smem_u32(&sh.bars[warp][0]), bar_v = smem_u32(&sh.bars[warp][1]);
-  if (lane == 0u) { mbar_init(bar_k, 1u); mbar_init(bar_v, 1u); }
+  const uint32_t bars = smem_u32(&sh.bars[warp][0]);
+  if (lane < 2u) mbar_init(bars + 8u * lane, 1u);
   if (tid < CA_WARPS * 2u) sh.ent[tid].on = 0u;
   if (tid == 0u) { sh.failed = 0u; sh.items = 0u; }
   __syncthreads();
@@ -116,22 +116,22 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
       if (raw >= p.c.pages) { cache_tell(p.c.status, CACHE_BAD_PAGE); raw = 0u; }
       return raw * p.c.Hkv + c.hk;
     };
-    auto fetch = [&](uint32_t block, uint32_t w) {                         // K (w 0) or V of a block of codes
+    // Every load is 8 KB, into buffer 0 or 1: a page's K and V, or two quarters of the tail (fp16): its K's lower and upper 32 keys, then its V's lower and
+    // upper 64 of d.  Each buffer is asked for again as soon as it is read.
+    auto load = [&](const void* src, uint32_t buf) {
       if (elect_one()) {
-        mbar_expect_tx(w ? bar_v : bar_k, CACHE_BLOCK);
-        bulk_g2s(ring + w * CACHE_BLOCK, p.c.codes + ((size_t)block * 2u + w) * CACHE_BLOCK, CACHE_BLOCK, w ? bar_v : bar_k);
+        mbar_expect_tx(bars + 8u * buf, CACHE_BLOCK);
+        bulk_g2s(ring + buf * CACHE_BLOCK, src, CACHE_BLOCK, bars + 8u * buf);
       }
     };
-    auto fetch_tail = [&](const CacheCursor& c, uint32_t w) {              // of a tail, into both buffers
-      if (elect_one()) {
-        mbar_expect_tx(w ? bar_v : bar_k, 2u * CACHE_BLOCK);
-        bulk_g2s(ring, p.c.tail + (((size_t)c.b * p.c.Hkv + c.hk) * 2u + w) * CACHE_BLOCK, 2u * CACHE_BLOCK, w ? bar_v : bar_k);
-      }
+    auto code_at = [&](uint32_t block, uint32_t w) -> const void* { return p.c.codes + ((size_t)block * 2u + w) * CACHE_BLOCK; };
+    auto tail_at = [&](const CacheCursor& c, uint32_t quarter) -> const void* {
+      return reinterpret_cast<const uint8_t*>(p.c.tail) + (((size_t)c.b * p.c.Hkv + c.hk) * 4u + quarter) * CACHE_BLOCK;
     };
-    uint32_t ph_k = 0u, ph_v = 0u;
+    auto first_at = [&](const CacheCursor& c, uint32_t block, uint32_t w) { return c.tail(c.t()) ? tail_at(c, w) : code_at(block, w); };
+    uint32_t ph = 0u;                                                      // parities of the two buffers' barriers
     bool ok = true;
-    auto wait_k = [&] { ok = __all_sync(0xffffffffu, mbar_wait(bar_k, ph_k, p.c.status, 611)); ph_k ^= 1u; return ok; };
-    auto wait_v = [&] { ok = __all_sync(0xffffffffu, mbar_wait(bar_v, ph_v, p.c.status, 612)); ph_v ^= 1u; return ok; };
+    auto wait = [&](uint32_t buf) { ok = __all_sync(0xffffffffu, mbar_wait(bars + 8u * buf, (ph >> buf) & 1u, p.c.status, 611 + (int)buf)); ph ^= 1u << buf; return ok; };
     uint32_t qa[8][4], pa[4][4], pos[2];
     float bias[2], o[16][4], m[2], l[2], s[8][4], zp[4];
     // scores (scaled, log2) -> weights pa, their sums zp; the running maximum rises only when it grew by more than 2^8 (weights are at most 256 then)
@@ -195,12 +195,10 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
     uint32_t raw = any ? raw_at(cur, cur.t() + lane) : 0u;
     if (any) queries(cur);
     uint32_t blk = block_of(cur, raw);                                     // this lane's page of the 32 at hand
-    auto fetch_first = [&](const CacheCursor& c, uint32_t block0) {
-      if (c.tail(c.t())) fetch_tail(c, 0u);
-      else { fetch(block0, 0u); fetch(block0, 1u); }
-    };
-    const uint32_t first = __shfl_sync(0xffffffffu, blk, 0);
-    if (any) fetch_first(cur, first);
+    if (any) {
+      const uint32_t first = __shfl_sync(0xffffffffu, blk, 0);
+      load(first_at(cur, first, 0u), 0u); load(first_at(cur, first, 1u), 1u);
+    }
     for (uint64_t u = w0; any;) {
       // ---- an item, or this warp's share of it: pages t .. t + cnt - 1, of which the last may be the tail
       const uint64_t i0 = u - cur.at, end = min(u + (cur.v.np + 1u - cur.at), w1);
@@ -211,7 +209,12 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
       CacheCursor nxt = cur;
       uint32_t nxt_raw = 0u, nxt_blk = 0u, blk2 = 0u, raw2 = 0u;
       if (more) { nxt.next_item(geo, sh.pre, sh.seq); nxt_raw = raw_at(nxt, lane); }
-      const bool nxt_tail = more && nxt.tail(0u);
+      uint32_t nxt_first = 0u;
+      auto next_item = [&](uint32_t w) {                                   // the first loads of what comes after this item
+        if (!more) return;
+        if (w == 0u) { nxt_blk = block_of(nxt, nxt_raw); nxt_first = __shfl_sync(0xffffffffu, nxt_blk, 0); }
+        load(first_at(nxt, nxt_first, w), w);
+      };
 #pragma unroll
       for (uint32_t h = 0; h < 2u; h++) pos[h] = p0 + min(cur.rb * 16u + h * 8u + g, rows - 1u) / p.group;
       {
@@ -223,8 +226,6 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
 #pragma unroll
       for (int d = 0; d < 16; d++) { o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f; }
       m[0] = m[1] = -INFINITY; l[0] = l[1] = 0.0f;
-      if (more) nxt_blk = block_of(nxt, nxt_raw);
-      const uint32_t nxt_block = __shfl_sync(0xffffffffu, nxt_blk, 0);
       for (uint32_t i = 0; i < codes && ok; i++) {
         const uint32_t at = i & 31u;
         if (at == 0u) {                                                    // 32 pages at a time: the next ones' numbers are asked for here, their scales half way
@@ -233,11 +234,13 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
         }
         if (at == 16u) { blk2 = block_of(cur, raw2); sc2 = ld_now(p.c.scales + blk2); }
         const float ks = __shfl_sync(0xffffffffu, sc.x, at), vs = __shfl_sync(0xffffffffu, sc.y, at);
-        const bool last = i + 1u == codes;
-        const uint32_t next = last ? nxt_block : __shfl_sync(0xffffffffu, at == 31u ? blk2 : blk, (at + 1u) & 31u);
-        // what follows: a page of codes (of this item or the next) can be asked for buffer by buffer, a tail needs both
-        const bool follows = !last || (!has_tail && more && !nxt_tail), tail_follows = last && (has_tail || nxt_tail);
-        if (!wait_k()) break;
+        const uint32_t next = __shfl_sync(0xffffffffu, at == 31u ? blk2 : blk, (at + 1u) & 31u);
+        auto follow = [&](uint32_t w) {
+          if (i + 1u < codes) load(code_at(next, w), w);
+          else if (has_tail) load(tail_at(cur, w), w);
+          else next_item(w);
+        };
+        if (!wait(0u)) break;
 #pragma unroll
         for (uint32_t n = 0; n < 8u; n += 4u) {                            // (four sums at a time: a product waits for the one before it on the same sum)
 #pragma unroll
@@ -254,10 +257,10 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
           }
         }
         __syncwarp();                                                      // the K buffer is read
-        if (follows) fetch(next, 0u);
+        follow(0u);
         weigh(cache_vis_page(cur.v, t + i), p0, p1, p.scale_log2 * ks * 16777216.0f, ca_lg2(vs), __fdividef(1.0f, vs));
         const float c0 = -0x1p-17f * zp[0], c1 = -0x1p-17f * zp[2];        // -128 * 2^-24 each
-        if (!wait_v()) break;
+        if (!wait(1u)) break;
 #pragma unroll
         for (uint32_t d = 0; d < 16u; d += 4u) {
           uint32_t w[4][4];
@@ -274,29 +277,36 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
             for (uint32_t h = 0; h < 4u; h++) at_mma(o[d + h], pa[j], __byte_perm(w[h][j], 0u, 0x4140), __byte_perm(w[h][j], 0u, 0x4342));
         }
         __syncwarp();                                                      // the V buffer is read
-        if (follows) fetch(next, 1u);
-        if (tail_follows) fetch_tail(has_tail ? cur : nxt, 0u);
+        follow(1u);
       }
       if (!ok) { sh.failed = 1u; break; }
       // from here on O is in real units
 #pragma unroll
       for (int d = 0; d < 16; d++) { o[d][0] *= 16777216.0f; o[d][1] *= 16777216.0f; o[d][2] *= 16777216.0f; o[d][3] *= 16777216.0f; }
       if (has_tail) {
-        if (!wait_k()) { sh.failed = 1u; break; }
+        auto scores = [&](uint32_t from, uint32_t n0) {                    // of 32 keys
 #pragma unroll
-        for (uint32_t n = 0; n < 8u; n++) {
-          s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+          for (uint32_t n = 0; n < 4u; n++) {
+            float (&y)[4] = s[n0 + n];
+            y[0] = y[1] = y[2] = y[3] = 0.0f;
 #pragma unroll
-          for (uint32_t k = 0; k < 2u; k++) {
-            const uint4 w = ca_lds(ring + n * 2048u + k * 1024u + lane * 32u), x = ca_lds(ring + n * 2048u + k * 1024u + lane * 32u + 16u);
-            at_mma(s[n], qa[k * 4u], w.x, w.y);
-            at_mma(s[n], qa[k * 4u + 1u], w.z, w.w);
-            at_mma(s[n], qa[k * 4u + 2u], x.x, x.y);
-            at_mma(s[n], qa[k * 4u + 3u], x.z, x.w);
+            for (uint32_t k = 0; k < 2u; k++) {
+              const uint4 w = ca_lds(from + n * 2048u + k * 1024u + lane * 32u), x = ca_lds(from + n * 2048u + k * 1024u + lane * 32u + 16u);
+              at_mma(y, qa[k * 4u], w.x, w.y);
+              at_mma(y, qa[k * 4u + 1u], w.z, w.w);
+              at_mma(y, qa[k * 4u + 2u], x.x, x.y);
+              at_mma(y, qa[k * 4u + 3u], x.z, x.w);
+            }
           }
-        }
+        };
+        if (!wait(0u)) { sh.failed = 1u; break; }
+        scores(ring, 0u);
         __syncwarp();
-        fetch_tail(cur, 1u);
+        load(tail_at(cur, 2u), 0u);
+        if (!wait(1u)) { sh.failed = 1u; break; }
+        scores(ring + CACHE_BLOCK, 4u);
+        __syncwarp();
+        load(tail_at(cur, 3u), 1u);
         weigh(cur.s.L / CACHE_PAGE, p0, p1, p.scale_log2, 0.0f, 1.0f);
         // (behind the sequence's end the tail may hold anything: those values weigh nothing, but 0 * NaN would count)
         const int have = (int)(cur.s.L & (CACHE_PAGE - 1u)) - (int)(4u * t4);
@@ -305,18 +315,24 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
         for (int j = 0; j < 4; j++)
 #pragma unroll
           for (int h = 0; h < 2; h++) { const int r = have - 16 * j - 2 * h; keep[j][h] = r >= 2 ? 0xffffffffu : r == 1 ? 0xffffu : 0u; }
-        if (!wait_v()) { sh.failed = 1u; break; }
+        auto values = [&](uint32_t from, uint32_t d0) {                    // of 64 d
 #pragma unroll
-        for (uint32_t d = 0; d < 16u; d++) {
-          const uint4 w = ca_lds(ring + d * 1024u + lane * 32u), x = ca_lds(ring + d * 1024u + lane * 32u + 16u);
-          at_mma(o[d], pa[0], w.x & keep[0][0], w.y & keep[0][1]);
-          at_mma(o[d], pa[1], w.z & keep[1][0], w.w & keep[1][1]);
-          at_mma(o[d], pa[2], x.x & keep[2][0], x.y & keep[2][1]);
-          at_mma(o[d], pa[3], x.z & keep[3][0], x.w & keep[3][1]);
-        }
+          for (uint32_t d = 0; d < 8u; d++) {
+            const uint4 w = ca_lds(from + d * 1024u + lane * 32u), x = ca_lds(from + d * 1024u + lane * 32u + 16u);
+            at_mma(o[d0 + d], pa[0], w.x & keep[0][0], w.y & keep[0][1]);
+            at_mma(o[d0 + d], pa[1], w.z & keep[1][0], w.w & keep[1][1]);
+            at_mma(o[d0 + d], pa[2], x.x & keep[2][0], x.y & keep[2][1]);
+            at_mma(o[d0 + d], pa[3], x.z & keep[3][0], x.w & keep[3][1]);
+          }
+        };
+        if (!wait(0u)) { sh.failed = 1u; break; }
+        values(ring, 0u);
         __syncwarp();
-        if (nxt_tail) fetch_tail(nxt, 0u);
-        else if (more) { fetch(nxt_block, 0u); fetch(nxt_block, 1u); }
+        next_item(0u);
+        if (!wait(1u)) { sh.failed = 1u; break; }
+        values(ring + CACHE_BLOCK, 8u);
+        __syncwarp();
+        next_item(1u);
       }
       // ---- the end of the item, or of this warp's share
       if (more) queries(nxt);                                              // (on their way while the result leaves)
@@ -402,16 +418,31 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
       c0 = __shfl_sync(0xffffffffu, own, 0); c1 = __shfl_sync(0xffffffffu, own, 1);
     }
     for (uint32_t r = r0; r < n; r += CA_WARPS) {
-      float M = -INFINITY, L = 0.0f;
-      for (uint32_t k = run; k; k &= k - 1u) { const uint32_t e = __ffs(k) - 1u; M = fmaxf(M, sh.ml[e >> 1][e & 1u][r].x); }
+      // lane e has share e's maximum and sum, and its weight
+      const bool mine = (run >> lane) & 1u;
+      const float2 ml = mine ? sh.ml[lane >> 1][lane & 1u][r] : make_float2(-INFINITY, 0.0f);
+      float M = ml.x;
+#pragma unroll
+      for (uint32_t x = 8; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+      M = __shfl_sync(0xffffffffu, M, 0);                                  // (16 shares: the lower lanes)
+      const float f = ml.x == -INFINITY ? 0.0f : at_ex2(ml.x - M);
+      float L = mine ? f * ml.y : 0.0f;
+#pragma unroll
+      for (uint32_t x = 8; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+      L = __shfl_sync(0xffffffffu, L, 0);
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (uint32_t k = run; k; k &= k - 1u) {
-        const uint32_t e = __ffs(k) - 1u;
-        const float2 ml = sh.ml[e >> 1][e & 1u][r];
-        const float f = ml.x == -INFINITY ? 0.0f : at_ex2(ml.x - M);
-        const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(gbase + ((e & 1u) ? (e >> 1) * CA_RING : CA_WARPS * CA_RING + (e >> 1) * CA_PART)) + r * CA_LD + 4u * lane);
-        L += f * ml.y;
-        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+      for (uint32_t k = run; k;) {                                         // four at a time
+        float4 v[4]; float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const uint32_t e = k ? __ffs(k) - 1u : e0;
+          w[i] = __shfl_sync(0xffffffffu, f, e) * (k ? 1.0f : 0.0f);
+          v[i] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(gbase + ((e & 1u) ? (e >> 1) * CA_RING : CA_WARPS * CA_RING + (e >> 1) * CA_PART)) + r * CA_LD + 4u * lane);
+          if (k) k &= k - 1u;
+          else v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) { acc.x = fmaf(w[i], v[i].x, acc.x); acc.y = fmaf(w[i], v[i].y, acc.y); acc.z = fmaf(w[i], v[i].z, acc.z); acc.w = fmaf(w[i], v[i].w, acc.w); }
       }
       if (whole) { store(it, r, L, acc); continue; }
       // (a block has two places: 0 for the item that began before it, 1 for the one that goes on behind it)
@@ -422,19 +453,19 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
       if (!arrive(c0, c1, r)) continue;
       M = -INFINITY; L = 0.0f; acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (uint32_t c = c0; c <= c1; c += 8u) {                            // (eight blocks' shares at a time, the running maximum as elsewhere)
-        float4 v[8]; float2 ml[8];
+        float4 v[8]; float2 z[8];
         float top = M;
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; i++) { const size_t x = at(min(c + i, c1)); v[i] = __ldcg(reinterpret_cast<const float4*>(p.part + x * 128u) + lane); ml[i] = __ldcg(&p.part_ml[x]); }
+        for (uint32_t i = 0; i < 8u; i++) { const size_t x = at(min(c + i, c1)); v[i] = __ldcg(reinterpret_cast<const float4*>(p.part + x * 128u) + lane); z[i] = __ldcg(&p.part_ml[x]); }
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; i++) top = fmaxf(top, ml[i].x);
+        for (uint32_t i = 0; i < 8u; i++) top = fmaxf(top, z[i].x);
         const float a = M == -INFINITY ? 0.0f : at_ex2(M - top);
         M = top; L *= a; acc.x *= a; acc.y *= a; acc.z *= a; acc.w *= a;
 #pragma unroll
         for (uint32_t i = 0; i < 8u; i++) {
-          const float f = c + i <= c1 && ml[i].x != -INFINITY ? at_ex2(ml[i].x - M) : 0.0f;
-          L += f * ml[i].y;
-          acc.x += f * v[i].x; acc.y += f * v[i].y; acc.z += f * v[i].z; acc.w += f * v[i].w;
+          const float w = c + i <= c1 && z[i].x != -INFINITY ? at_ex2(z[i].x - M) : 0.0f;
+          L += w * z[i].y;
+          acc.x += w * v[i].x; acc.y += w * v[i].y; acc.z += w * v[i].z; acc.w += w * v[i].w;
         }
       }
       store(it, r, L, acc);
