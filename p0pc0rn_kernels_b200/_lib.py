@@ -51,26 +51,6 @@ class AttnArgs(C.Structure):
                 + [(n, C.c_void_p) for n in ("q", "k", "v", "o")] + [(n, C.c_uint64) for n in ("q_off", "k_off", "v_off", "o_off")] + [("kernel", C.c_uint32)])
 
 
-class Cache(C.Structure):
-    _fields_ = ([(n, C.c_uint32) for n in ("Hkv", "pages", "seqs", "max_pages")] + [(n, C.c_void_p) for n in ("codes", "scales", "tail", "table", "lens")]
-                + [(n, C.c_uint64) for n in ("codes_off", "scales_off", "tail_off", "table_off", "lens_off")])
-
-
-class CacheArgs(C.Structure):
-    _fields_ = ([(n, C.c_uint32) for n in ("struct_size", "M", "ldk", "ldv")] + [("cache", Cache)] + [(n, C.c_void_p) for n in ("k", "v", "rows")]
-                + [(n, C.c_uint64) for n in ("k_off", "v_off", "rows_off")])
-
-
-class CacheAttnArgs(C.Structure):
-    _fields_ = ([(n, C.c_uint32) for n in ("struct_size", "Hq", "M", "ldq", "ldo", "max_new", "window", "sinks")] + [("scale", C.c_float), ("kernel", C.c_uint32), ("cache", Cache)]
-                + [(n, C.c_void_p) for n in ("q", "o", "rows")] + [(n, C.c_uint64) for n in ("q_off", "o_off", "rows_off")])
-
-
-class RopeArgs(C.Structure):
-    _fields_ = ([(n, C.c_uint32) for n in ("struct_size", "H", "M", "ldx", "ldy", "seqs", "mode", "rot")] + [(n, C.c_double) for n in ("theta", "factor", "original", "fast", "slow", "mscale")]
-                + [(n, C.c_void_p) for n in ("x", "y", "lens", "rows")] + [(n, C.c_uint64) for n in ("x_off", "y_off", "lens_off", "rows_off")])
-
-
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is missing: build it with `python p0pc0rn_kernels_b200/build.py` (needs nvcc); there is no CPU fallback")
@@ -93,8 +73,7 @@ def _load():
         "p0p_gn_finalize": (i, [vp, vp, u32, u32, C.c_float, vp, u32, u32, vp, u32]),
         "p0p_alloc_shareable": (i, [vp, u64, C.POINTER(vp)]), "p0p_ipc_export": (i, [vp, vp, vp]), "p0p_ipc_open": (i, [vp, vp, u64, C.POINTER(vp)]),
         "p0p_gemm": (i, [vp, C.POINTER(GemmArgs), C.POINTER(C.c_double)]), "p0p_attention": (i, [vp, C.POINTER(AttnArgs), C.POINTER(C.c_double)]), "p0p_last_kernel": (i, [vp]), "p0p_launch_count": (u64, [vp]), "p0p_last_plan": (i, [vp, C.POINTER(C.c_uint32)]),
-        "p0p_cache_write": (i, [vp, C.POINTER(CacheArgs)]), "p0p_cache_read": (i, [vp, C.POINTER(CacheArgs)]),
-        "p0p_cache_attention": (i, [vp, C.POINTER(CacheAttnArgs)]), "p0p_rope": (i, [vp, C.POINTER(RopeArgs)]),
+        "p0p_cache_write": (i, [vp, C.c_char_p]), "p0p_cache_read": (i, [vp, C.c_char_p]), "p0p_cache_attention": (i, [vp, C.c_char_p]), "p0p_rope": (i, [vp, C.c_char_p]),
         "p0p_dequant": (i, [vp, u32, vp, u64, u32, u32, u32, u32, u32, vp, u64]),
         "p0p_rowstats": (i, [vp, vp, u64, u32, u32, u32, u32, u32, C.c_float, vp, u32]),
         "p0p_f2h": (C.c_uint16, [C.c_float]), "p0p_h2f": (C.c_float, [C.c_uint16]),

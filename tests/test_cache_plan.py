@@ -232,15 +232,47 @@ int main() {
 
 
 def test_argument_blocks_match_the_header(tmp_path):
-    """the ctypes transcriptions have the header's sizes and field offsets"""
-    import ctypes as C
+    """the packed argument blocks have the header's sizes, and every field the header's place"""
+    import struct
 
-    from p0pc0rn_kernels_b200._lib import Cache, CacheArgs, CacheAttnArgs, RopeArgs
-    blocks = {"p0p_cache": Cache, "p0p_cache_args": CacheArgs, "p0p_cache_attn_args": CacheAttnArgs, "p0p_rope_args": RopeArgs}
+    from p0pc0rn_kernels_b200 import cache
+    in_cache = ["cache." + f for f in "Hkv pages seqs max_pages codes scales tail table lens codes_off scales_off tail_off table_off lens_off".split()]
+    blocks = {"p0p_cache_args": (cache._MOVE, ["struct_size", "M", "ldk", "ldv", *in_cache, "k", "v", "rows", "k_off", "v_off", "rows_off"]),
+              "p0p_cache_attn_args": (cache._ATTN, ["struct_size", "Hq", "M", "ldq", "ldo", "max_new", "window", "sinks", "scale", "kernel", *in_cache, "q", "o", "rows", "q_off", "o_off", "rows_off"]),
+              "p0p_rope_args": (cache._ROPE, "struct_size H M ldx ldy seqs mode rot theta factor original fast slow mscale x y lens rows x_off y_off lens_off rows_off".split())}
     src, exe = tmp_path / "layout.c", tmp_path / "layout"
-    lines = "".join(f'printf("%zu\\n", sizeof({n}));' + "".join(f'printf("%zu\\n", offsetof({n}, {f[0]}));' for f in t._fields_) for n, t in blocks.items())
+    lines = "".join(f'printf("%zu\\n", sizeof({n}));' + "".join(f'printf("%zu\\n", offsetof({n}, {f}));' for f in fields) for n, (_, fields) in blocks.items())
     src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "p0p.h"\nint main(void){' + lines + "return 0;}\n")
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
     got = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
-    want = [v for t in blocks.values() for v in [C.sizeof(t)] + [getattr(t, f[0]).offset for f in t._fields_]]
+    want = []
+    for layout, fields in blocks.values():
+        want.append(layout.size)
+        zero = [0.0 if c in "fd" else 0 for c in _codes(layout.format)]
+        for i, c in enumerate(_codes(layout.format)):                      # where a value put into field i shows up first
+            raw = layout.pack(*zero[:i], -1.0 if c in "fd" else 255, *zero[i + 1:])
+            at = next(k for k, b in enumerate(raw) if b)
+            want.append(at - at % struct.calcsize(c))
+        assert len(fields) == len(zero)
     assert got == want
+
+
+def _codes(fmt):
+    """a struct format as one letter per value"""
+    import re
+    return "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([IQfd])", fmt))
+
+
+def test_bad_numbers_are_refused_before_the_call():
+    import p0pc0rn_kernels_b200 as P
+    import pytest
+
+    class Gpu:
+        _h = _check = None
+    for bad in (-1, 1 << 32, 1.5):
+        with pytest.raises(ValueError, match="rope: bad argument"):
+            P.rope(Gpu(), {"x": {"buf": type("B", (), {"handle": None})()}, "H": 1, "M": bad, "seqs": 1, "lens": None})
+    with pytest.raises(ValueError, match="unknown mode"):
+        P.rope(Gpu(), {"x": {}, "H": 1, "M": 1, "seqs": 1, "lens": None, "mode": "both"})
+    with pytest.raises(ValueError, match="unknown kernel"):
+        P.cacheAttention(Gpu(), {"q": {}, "o": {}, "kernel": "warp"})
