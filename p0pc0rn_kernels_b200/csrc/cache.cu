@@ -23,7 +23,7 @@ int cache_move(p0p_ctx* c, const char* op, const p0p_cache_args* a, Kern kern, T
   const uint64_t per = p.rows ? 0u : cache_touched_bound(p.each, 1u), blocks = p.rows ? cache_touched_bound(M, p.seqs) : per * p.seqs;
   if (blocks > 0x7fffffffu) return fail(c, -5, "%s: too many rows for one call", op);
   DeviceGuard g(c->device);
-  const cudaError_t e = launch_chained(kern, dim3((uint32_t)blocks, p.Hkv), dim3(256), CW_SMEM, c->stream, p, (T*)k, (T*)v, ldk, ldv, (uint32_t)per);
+  const cudaError_t e = launch_chained(kern, dim3((uint32_t)blocks, p.Hkv), dim3(256), 0, c->stream, p, (T*)k, (T*)v, ldk, ldv, (uint32_t)per);
   if (e != cudaSuccess) return cuda_fail(c, e, op);
   c->launches += 1;
   return 0;

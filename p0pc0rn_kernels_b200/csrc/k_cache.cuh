@@ -8,33 +8,48 @@
 
 namespace p0p {
 
-// Block x of a call's touched pages: the sequence and which of its touched pages it is.  False: there are fewer.  All 256 threads.
-__device__ __forceinline__ bool cache_find_page(const CacheP& p, uint32_t x, uint32_t per_seq, uint32_t& b, uint32_t& local) {
+// Block x of a call's touched pages: the sequence, and which of its touched pages it is.  False: there are fewer.  All 256 threads.
+__device__ __forceinline__ bool cache_find_page(const CacheP& p, uint32_t x, uint32_t per_seq, uint32_t& b, uint32_t& local, CacheSeq& s) {
   if (!p.rows) {                                                         // equal counts: as many blocks for every sequence
     b = x / per_seq; local = x - b * per_seq;
+    s = cache_seq(p, b);
+    return local < cache_touched(s);
+  }
+  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  auto scan = [&](uint32_t inc) {
+#pragma unroll
+    for (uint32_t o = 1; o < 32u; o <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += v; }
+    return inc;
+  };
+  if (p.seqs <= 32u) {                                                   // every warp by itself: one look at the sequences, no barrier
+    CacheSeq mine{0u, 0u, 0u};
+    if (lane < p.seqs) mine = cache_seq(p, lane);
+    const uint32_t c = cache_touched(mine), inc = scan(c), hit = __ballot_sync(0xffffffffu, x < inc && x >= inc - c);
+    if (!hit) return false;
+    b = __ffs(hit) - 1u;
+    local = x - __shfl_sync(0xffffffffu, inc - c, b);
+    s.r0 = __shfl_sync(0xffffffffu, mine.r0, b); s.n = __shfl_sync(0xffffffffu, mine.n, b); s.L = __shfl_sync(0xffffffffu, mine.L, b);
     return true;
   }
-  __shared__ uint32_t warp_sum[8], found[2];
-  const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+  __shared__ uint32_t warp_sum[8], found[5];
   if (tid == 0u) found[0] = 0xffffffffu;
   uint64_t base = 0u;
   for (uint32_t b0 = 0; b0 < p.seqs; b0 += 256u) {
-    const uint32_t c = b0 + tid < p.seqs ? cache_touched(cache_seq(p, b0 + tid)) : 0u;
-    uint32_t inc = c;
-#pragma unroll
-    for (uint32_t o = 1; o < 32u; o <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += v; }
+    CacheSeq mine{0u, 0u, 0u};
+    if (b0 + tid < p.seqs) mine = cache_seq(p, b0 + tid);
+    const uint32_t c = cache_touched(mine), inc = scan(c);
     if (lane == 31u) warp_sum[warp] = inc;
     __syncthreads();
     uint32_t before = 0u, all = 0u;
 #pragma unroll
     for (uint32_t w = 0; w < 8u; w++) { if (w < warp) before += warp_sum[w]; all += warp_sum[w]; }
     const uint64_t first = base + before + inc - c;
-    if (c && x >= first && x < first + c) { found[0] = b0 + tid; found[1] = (uint32_t)(x - first); }
+    if (c && x >= first && x < first + c) { found[0] = b0 + tid; found[1] = (uint32_t)(x - first); found[2] = mine.r0; found[3] = mine.n; found[4] = mine.L; }
     base += all;
     __syncthreads();
     if (found[0] != 0xffffffffu || x < base) break;
   }
-  b = found[0]; local = found[1];
+  b = found[0]; local = found[1]; s.r0 = found[2]; s.n = found[3]; s.L = found[4];
   return b != 0xffffffffu;
 }
 
@@ -47,8 +62,20 @@ __device__ __forceinline__ uint32_t cache_clean(uint32_t v) {
   return *reinterpret_cast<const uint32_t*>(&c);
 }
 
-constexpr uint32_t CW_LD = 132u;        // halves per row of the staging tile: 16 rows apart is another bank
-constexpr uint32_t CW_SMEM = 2u * CACHE_PAGE * CW_LD * 2u;
+constexpr uint32_t CW_LD = 136u;        // halves per row of the tile that V is turned in: 16-byte rows, and 4 keys further another half of the banks
+
+// A lane's 16 values of one d (keys 16 j + 4 t + i, t = lane % 4; word w: j = w / 2, i = 2 (w % 2) and the next) into the tile [key][d], together with
+// the lane of the other d of the pair (lane ^ 4): the even one's lane takes the even keys, so that a store has two d
+__device__ __forceinline__ void cache_turn(__half* tile, uint32_t d, uint32_t lane, const uint32_t (&h)[8]) {
+  const bool odd = (lane & 4u) != 0u;
+#pragma unroll
+  for (uint32_t w = 0; w < 8u; w++) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, h[w], 4);
+    const uint32_t both = odd ? __byte_perm(other, h[w], 0x7632) : __byte_perm(h[w], other, 0x5410);
+    *reinterpret_cast<uint32_t*>(tile + ((w >> 1) * 16u + 4u * (lane & 3u) + 2u * (w & 1u) + (odd ? 1u : 0u)) * CW_LD + (d & ~1u)) = both;
+  }
+}
+__device__ __forceinline__ void cache_bar(uint32_t id) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(id) : "memory"); }      // of the 128 threads of K or V
 
 // New tokens t0 .. t1 - 1 of the unfinished page `pg` (positions) into the tail.  All 256 threads.
 __device__ __forceinline__ void cache_append(__half* tk, __half* tv, const __half* K, const __half* V, uint32_t row_of_pos0, uint32_t pg, uint32_t t0, uint32_t t1) {
@@ -75,21 +102,20 @@ __device__ __forceinline__ float cache_scale(float amax) {
   return amax > 0.0f ? __uint_as_float((__float_as_uint(__fdiv_rn(amax, 127.0f)) + 4095u) & ~4095u) : 1.0f;
 }
 
-// One block = one touched page of one kv head; 128 threads for K, 128 for V.  A page that the call finishes is gathered (old tokens
-// from the tail, new ones from the rows) in shared memory with its largest magnitude found on the way, then leaves as codes in the cache's
-// order: 16 codes per thread and store.  The unfinished last page only takes its new tokens into the tail; where the call also
-// finishes a page that began in the tail, that page's block does it, after it has read the tail.
+// One block = one touched page of one kv head; 128 threads for K, 128 for V, each half by itself.  A page that the call finishes: its tokens (old ones from
+// the tail, new ones from the rows) are read with their largest magnitude found on the way; K's codes leave from the registers, 8 per thread and store, V's
+// through a tile in shared memory that turns them.  The unfinished last page only takes its new tokens into the tail; where the call
+// also finishes a page that began in the tail, that page's block does it, after it has read the tail.
 // Bound: HBM for prompts (256 bytes read and 128 written per token, head and K or V), launch latency for steps.
-__global__ void __launch_bounds__(256) k_cache_write(const CacheP p, const __half* K, const __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
-  extern __shared__ __align__(16) unsigned char cw_smem[];
+__global__ void __launch_bounds__(256, 4) k_cache_write(const CacheP p, const __half* K, const __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
+  __shared__ __align__(16) __half tile[CACHE_PAGE * CW_LD];
   __shared__ float sm_max[8];
   const uint32_t tid = threadIdx.x, hk = blockIdx.y;
   grid_dependency_wait();
   grid_launch_dependents();
   uint32_t b, local;
-  if (!cache_find_page(p, blockIdx.x, per_seq, b, local)) return;
-  const CacheSeq s = cache_seq(p, b);
-  if (local >= cache_touched(s)) return;
+  CacheSeq s;
+  if (!cache_find_page(p, blockIdx.x, per_seq, b, local, s)) return;
   const uint32_t first = cache_first_page(s), old = s.L - s.n, pg = first + local, last = s.L / CACHE_PAGE;
   const uint32_t row0 = s.r0 - old;                                       // (wraps: only sums with positions >= old are rows)
   __half* tk = p.tail + ((size_t)b * p.Hkv + hk) * 2u * CACHE_BLOCK; __half* tv = tk + CACHE_BLOCK;
@@ -99,61 +125,67 @@ __global__ void __launch_bounds__(256) k_cache_write(const CacheP p, const __hal
     if (pg == first || !began) cache_append(tk, tv, Kh, Vh, row0, pg, max(old, pg * CACHE_PAGE), s.L);
     return;
   }
-  const uint32_t w = tid >> 7, i = tid & 127u;
-  __half* tile = reinterpret_cast<__half*>(cw_smem) + w * CACHE_PAGE * CW_LD;
+  const uint32_t page = ld_now(p.table + (size_t)b * p.max_pages + pg);
+  const uint32_t w = tid >> 7, i = tid & 127u, lane = tid & 31u;
+  const uint32_t have = pg == first ? old & (CACHE_PAGE - 1u) : 0u;       // keys that are in the tail
   const __half* src = w ? Vh : Kh; const __half* tl = w ? tv : tk;
   uint4 x[8];
 #pragma unroll
   for (uint32_t it = 0; it < 8u; it++) {
-    const uint32_t key = it * 8u + (i >> 4), d = (i & 15u) * 8u, pos = pg * CACHE_PAGE + key;
-    if (pos >= old) {
-      x[it] = ld_now(reinterpret_cast<const uint4*>(src + (size_t)(row0 + pos) * 128u + d));
-      x[it].x = cache_clean(x[it].x); x[it].y = cache_clean(x[it].y); x[it].z = cache_clean(x[it].z); x[it].w = cache_clean(x[it].w);
-    } else if (w == 0u) x[it] = ld_now(reinterpret_cast<const uint4*>(tl + cache_k_off(key, d)));
-    else {
-      uint32_t v[8];
-#pragma unroll
-      for (uint32_t j = 0; j < 8u; j++) v[j] = __half_as_ushort(ld_now(tl + cache_v_off(key, d + j)));
-      x[it] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
-    }
+    const uint32_t key = it * 8u + (i >> 4), d = (i & 15u) * 8u;
+    x[it] = make_uint4(0u, 0u, 0u, 0u);
+    if (key >= have) x[it] = ld_now(reinterpret_cast<const uint4*>(src + (size_t)(row0 + pg * CACHE_PAGE + key) * 128u + d));
+    else if (w == 0u) x[it] = ld_now(reinterpret_cast<const uint4*>(tl + cache_k_off(key, d)));
   }
   __half2 mx = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+  auto largest = [&](uint32_t v) { mx = __hmax2(mx, __habs2(*reinterpret_cast<const __half2*>(&v))); };
+  if (w && have) {                                                        // V's old tokens: pieces of 16 keys of one d
+#pragma unroll 1
+    for (uint32_t it = 0; it < 4u; it++) {
+      const uint32_t u = it * 128u + i;
+      const uint4 a = ld_now(reinterpret_cast<const uint4*>(tl) + 2u * u), z = ld_now(reinterpret_cast<const uint4*>(tl) + 2u * u + 1u);
+      uint32_t h[8] = {a.x, a.y, a.z, a.w, z.x, z.y, z.z, z.w};
+#pragma unroll
+      for (int k = 0; k < 8; k++) {                                       // (what lies behind them is of another page or of none: new tokens take its place below)
+        const int r = (int)have - (int)(4u * (u & 3u)) - 16 * (k >> 1) - 2 * (k & 1);
+        h[k] = r >= 2 ? h[k] : r == 1 ? h[k] & 0xffffu : 0u;
+        largest(h[k]);
+      }
+      cache_turn(tile, u >> 2, lane, h);
+    }
+    cache_bar(2u);
+  }
 #pragma unroll
   for (uint32_t it = 0; it < 8u; it++) {
-    const uint32_t key = it * 8u + (i >> 4), d = (i & 15u) * 8u;
-    const __half2* h = reinterpret_cast<const __half2*>(&x[it]);
-#pragma unroll
-    for (int j = 0; j < 4; j++) mx = __hmax2(mx, __habs2(h[j]));
-    uint2* dst = reinterpret_cast<uint2*>(tile + key * CW_LD + d);
-    dst[0] = make_uint2(x[it].x, x[it].y); dst[1] = make_uint2(x[it].z, x[it].w);
+    const uint32_t key = it * 8u + (i >> 4);
+    x[it].x = cache_clean(x[it].x); x[it].y = cache_clean(x[it].y); x[it].z = cache_clean(x[it].z); x[it].w = cache_clean(x[it].w);
+    largest(x[it].x); largest(x[it].y); largest(x[it].z); largest(x[it].w);
+    if (w && key >= have) *reinterpret_cast<uint4*>(tile + key * CW_LD + (i & 15u) * 8u) = x[it];
   }
   float m = fmaxf(__low2float(mx), __high2float(mx));
 #pragma unroll
   for (uint32_t o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((tid & 31u) == 0u) sm_max[tid >> 5] = m;
-  __syncthreads();                                                        // (every read of the tail has ended, too)
+  if (lane == 0u) sm_max[tid >> 5] = m;
+  cache_bar(1u + w);
   const float sc = cache_scale(fmaxf(fmaxf(sm_max[w * 4u], sm_max[w * 4u + 1u]), fmaxf(sm_max[w * 4u + 2u], sm_max[w * 4u + 3u]))), inv = __fdiv_rn(1.0f, sc);
-  const uint32_t page = ld_now(p.table + (size_t)b * p.max_pages + pg);
   if (page >= p.pages) { if (tid == 0u) cache_tell(p.status, CACHE_BAD_PAGE); }
   else {
-    uint4* out = reinterpret_cast<uint4*>(p.codes + (((size_t)page * p.Hkv + hk) * 2u + w) * CACHE_BLOCK);
+    uint8_t* out = p.codes + (((size_t)page * p.Hkv + hk) * 2u + w) * CACHE_BLOCK;
     if (w == 0u) {
 #pragma unroll
-      for (uint32_t it = 0; it < 4u; it++) {                              // unit u = 16 consecutive d of one key
-        const uint32_t u = it * 128u + i, key = (u >> 7) * 16u + ((u >> 3) & 3u) * 4u + ((u >> 6) & 1u) * 2u + ((u >> 2) & 1u), d = ((u >> 5) & 1u) * 64u + (u & 3u) * 16u;
-        const uint2* r = reinterpret_cast<const uint2*>(tile + key * CW_LD + d);
-        uint32_t q[4];
+      for (uint32_t it = 0; it < 8u; it++) {
+        uint32_t q[2];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const uint2 v = r[j];
-          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
-          q[j] = cache_pack4(cache_code(f0.x, inv), cache_code(f0.y, inv), cache_code(f1.x, inv), cache_code(f1.y, inv));
+        for (int k = 0; k < 2; k++) {
+          const uint32_t v0 = k ? x[it].z : x[it].x, v1 = k ? x[it].w : x[it].y;
+          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&v0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&v1));
+          q[k] = cache_pack4(cache_code(f0.x, inv), cache_code(f0.y, inv), cache_code(f1.x, inv), cache_code(f1.y, inv));
         }
-        out[u] = make_uint4(q[0], q[1], q[2], q[3]);
+        *reinterpret_cast<uint2*>(out + cache_k_off(it * 8u + (i >> 4), (i & 15u) * 8u)) = make_uint2(q[0], q[1]);
       }
     } else {
 #pragma unroll
-      for (uint32_t it = 0; it < 2u; it++) {                              // two units: keys 16 j + 4 t + e of d and of d + 1
+      for (uint32_t it = 0; it < 2u; it++) {                              // two pieces: keys 16 j + 4 t + e of d and of d + 1
         const uint32_t u = it * 128u + i, d = (u >> 2) * 2u, t = u & 3u;
         uint32_t q0[4], q1[4];
 #pragma unroll
@@ -166,47 +198,46 @@ __global__ void __launch_bounds__(256) k_cache_write(const CacheP p, const __hal
           }
           q0[j] = cache_pack4(c0[0], c0[1], c0[2], c0[3]); q1[j] = cache_pack4(c1[0], c1[1], c1[2], c1[3]);
         }
-        out[d * 4u + t] = make_uint4(q0[0], q0[1], q0[2], q0[3]); out[(d + 1u) * 4u + t] = make_uint4(q1[0], q1[1], q1[2], q1[3]);
+        reinterpret_cast<uint4*>(out)[d * 4u + t] = make_uint4(q0[0], q0[1], q0[2], q0[3]);
+        reinterpret_cast<uint4*>(out)[(d + 1u) * 4u + t] = make_uint4(q1[0], q1[1], q1[2], q1[3]);
       }
     }
     if (i == 0u) reinterpret_cast<float*>(p.scales + (size_t)page * p.Hkv + hk)[w] = sc;
   }
   // (new tokens behind the last finished page: positions last * 64 >= old, since page `first` is finished)
-  if (pg == first && began) cache_append(tk, tv, Kh, Vh, row0, last, last * CACHE_PAGE, s.L);
+  if (have) {
+    __syncthreads();                                                      // (every read of the tail has ended)
+    cache_append(tk, tv, Kh, Vh, row0, last, last * CACHE_PAGE, s.L);
+  }
 }
 
-// ---- read back: one block = one touched page of one kv head, as in k_cache_write; values go through shared memory to whole rows
-__global__ void __launch_bounds__(256) k_cache_read(const CacheP p, __half* K, __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
-  extern __shared__ __align__(16) unsigned char cw_smem[];
-  const uint32_t tid = threadIdx.x, hk = blockIdx.y;
+// ---- read back: one block = one touched page of one kv head, as in k_cache_write.  K's values go straight to their rows (two lanes swap halves, so
+// that a store fills whole 32-byte pieces), V's through the tile that turns them.
+__global__ void __launch_bounds__(256, 4) k_cache_read(const CacheP p, __half* K, __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
+  __shared__ __align__(16) __half tile[CACHE_PAGE * CW_LD];
+  const uint32_t tid = threadIdx.x, hk = blockIdx.y, lane = tid & 31u;
   grid_dependency_wait();
   grid_launch_dependents();
   uint32_t b, local;
-  if (!cache_find_page(p, blockIdx.x, per_seq, b, local)) return;
-  const CacheSeq s = cache_seq(p, b);
-  if (local >= cache_touched(s)) return;
+  CacheSeq s;
+  if (!cache_find_page(p, blockIdx.x, per_seq, b, local, s)) return;
   const uint32_t old = s.L - s.n, pg = cache_first_page(s) + local, row0 = s.r0 - old;
   const uint32_t w = tid >> 7, i = tid & 127u;
-  __half* tile = reinterpret_cast<__half*>(cw_smem) + w * CACHE_PAGE * CW_LD;
   const bool whole = pg < s.L / CACHE_PAGE;
   uint32_t page = 0u;
   if (whole) {
     page = ld_now(p.table + (size_t)b * p.max_pages + pg);
     if (page >= p.pages) { if (tid == 0u) cache_tell(p.status, CACHE_BAD_PAGE); return; }
   }
-  const uint4* in = reinterpret_cast<const uint4*>(p.codes + (((size_t)page * p.Hkv + hk) * 2u + w) * CACHE_BLOCK);
-  const __half* tl = p.tail + (((size_t)b * p.Hkv + hk) * 2u + w) * CACHE_BLOCK;
-  const float sc = whole ? ld_now(reinterpret_cast<const float*>(p.scales + (size_t)page * p.Hkv + hk) + w) : 0.0f;
-  uint4 c[4];
+  uint32_t h[4][8];                                                       // four pieces of 16 values: of one key (K) or of one d (V)
   if (whole) {
+    const uint4* in = reinterpret_cast<const uint4*>(p.codes + (((size_t)page * p.Hkv + hk) * 2u + w) * CACHE_BLOCK);
+    const float sc = ld_now(reinterpret_cast<const float*>(p.scales + (size_t)page * p.Hkv + hk) + w);
+    uint4 c[4];
 #pragma unroll
     for (uint32_t it = 0; it < 4u; it++) c[it] = ld_now(in + it * 128u + i);
-  }
 #pragma unroll
-  for (uint32_t it = 0; it < 4u; it++) {
-    const uint32_t u = it * 128u + i;
-    uint32_t h[8];                                                        // 16 values: of one key (K) or of one d (V)
-    if (whole) {
+    for (uint32_t it = 0; it < 4u; it++) {
       const uint32_t q[4] = {c[it].x, c[it].y, c[it].z, c[it].w};
 #pragma unroll
       for (int j = 0; j < 8; j++) {
@@ -214,32 +245,43 @@ __global__ void __launch_bounds__(256) k_cache_read(const CacheP p, __half* K, _
         // (a code of 127 times a scale that was rounded up may pass the largest fp16: it stays finite)
         const float lo = fmaxf(fminf((float)((int)(v & 255u) - 128) * sc, 65504.0f), -65504.0f), hi = fmaxf(fminf((float)((int)((v >> 8) & 255u) - 128) * sc, 65504.0f), -65504.0f);
         const __half2 r = __floats2half2_rn(lo, hi);
-        h[j] = *reinterpret_cast<const uint32_t*>(&r);
+        h[it][j] = *reinterpret_cast<const uint32_t*>(&r);
       }
-    } else {
-      const uint4 a = ld_now(reinterpret_cast<const uint4*>(tl) + 2u * u), z = ld_now(reinterpret_cast<const uint4*>(tl) + 2u * u + 1u);
-      h[0] = a.x; h[1] = a.y; h[2] = a.z; h[3] = a.w; h[4] = z.x; h[5] = z.y; h[6] = z.z; h[7] = z.w;
     }
-    if (w == 0u) {
-      const uint32_t key = (u >> 7) * 16u + ((u >> 3) & 3u) * 4u + ((u >> 6) & 1u) * 2u + ((u >> 2) & 1u), d = ((u >> 5) & 1u) * 64u + (u & 3u) * 16u;
-      uint2* r = reinterpret_cast<uint2*>(tile + key * CW_LD + d);
+  } else {
+    const uint4* tl = reinterpret_cast<const uint4*>(p.tail + (((size_t)b * p.Hkv + hk) * 2u + w) * CACHE_BLOCK);
 #pragma unroll
-      for (int j = 0; j < 4; j++) r[j] = make_uint2(h[2 * j], h[2 * j + 1]);
-    } else {
-      const uint32_t d = u >> 2, t = u & 3u;
-#pragma unroll
-      for (uint32_t j = 0; j < 16u; j++) tile[((j >> 2) * 16u + 4u * t + (j & 3u)) * CW_LD + d] = __ushort_as_half((unsigned short)(h[j >> 1] >> (16u * (j & 1u))));
+    for (uint32_t it = 0; it < 4u; it++) {
+      const uint4 a = ld_now(tl + 2u * (it * 128u + i)), z = ld_now(tl + 2u * (it * 128u + i) + 1u);
+      h[it][0] = a.x; h[it][1] = a.y; h[it][2] = a.z; h[it][3] = a.w; h[it][4] = z.x; h[it][5] = z.y; h[it][6] = z.z; h[it][7] = z.w;
     }
   }
-  __syncthreads();
-  __half* dst = w ? V + (size_t)hk * ldv * 128u : K + (size_t)hk * ldk * 128u;
+  if (w == 0u) {
+    __half* dst = K + (size_t)hk * ldk * 128u;
+#pragma unroll
+    for (uint32_t it = 0; it < 4u; it++) {
+      const uint32_t u = it * 128u + i, key = (u >> 7) * 16u + ((u >> 3) & 3u) * 4u + ((u >> 6) & 1u) * 2u + ((u >> 2) & 1u), d = ((u >> 5) & 1u) * 64u + (u & 3u) * 16u, pos = pg * CACHE_PAGE + key;
+      const bool odd = (lane & 1u) != 0u;
+      uint32_t got[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) got[k] = __shfl_xor_sync(0xffffffffu, odd ? h[it][k] : h[it][4 + k], 1);      // (the even lane gives its upper half for the odd one's lower)
+      const uint4 a = odd ? make_uint4(got[0], got[1], got[2], got[3]) : make_uint4(h[it][0], h[it][1], h[it][2], h[it][3]);
+      const uint4 z = odd ? make_uint4(h[it][4], h[it][5], h[it][6], h[it][7]) : make_uint4(got[0], got[1], got[2], got[3]);
+      if (pos >= old && pos < s.L) {                                      // (both lanes have the same key)
+        __half* r = dst + (size_t)(row0 + pos) * 128u + (d & ~16u) + (odd ? 8u : 0u);
+        *reinterpret_cast<uint4*>(r) = a; *reinterpret_cast<uint4*>(r + 16u) = z;
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (uint32_t it = 0; it < 4u; it++) cache_turn(tile, (it * 128u + i) >> 2, lane, h[it]);
+  cache_bar(2u);
+  __half* dst = V + (size_t)hk * ldv * 128u;
 #pragma unroll
   for (uint32_t it = 0; it < 8u; it++) {
     const uint32_t key = it * 8u + (i >> 4), d = (i & 15u) * 8u, pos = pg * CACHE_PAGE + key;
-    if (pos < old || pos >= s.L) continue;
-    const uint2* r = reinterpret_cast<const uint2*>(tile + key * CW_LD + d);
-    const uint2 a = r[0], z = r[1];
-    *reinterpret_cast<uint4*>(dst + (size_t)(row0 + pos) * 128u + d) = make_uint4(a.x, a.y, z.x, z.y);
+    if (pos >= old && pos < s.L) *reinterpret_cast<uint4*>(dst + (size_t)(row0 + pos) * 128u + d) = *reinterpret_cast<const uint4*>(tile + key * CW_LD + d);
   }
 }
 
@@ -302,10 +344,7 @@ __global__ void __launch_bounds__(128) k_rope(const RopeP p) {
   float2 cs[8];
 #pragma unroll
   for (uint32_t i = 0; i < 8u; i++) cs[i] = rope_cs(p, i0 + i, pos);
-  for (uint32_t h = h0; h < h1; h++) {
-    const uint4* x = reinterpret_cast<const uint4*>(p.X + ((size_t)h * p.ldx + r) * 128u);
-    uint4* y = reinterpret_cast<uint4*>(p.Y + ((size_t)h * p.ldy + r) * 128u);
-    uint4 v[2] = {ld_now(x + c0), ld_now(x + c1)};
+  auto turned = [&](uint4 (&v)[2]) {
     __half2* e = reinterpret_cast<__half2*>(v);
     if (HALF) {
       if (i0 < 64u) {
@@ -323,7 +362,21 @@ __global__ void __launch_bounds__(128) k_rope(const RopeP p) {
         if (2u * (i0 + i) < p.rot) { rope_turn(cs[i], a.x, a.y); e[i] = __floats2half2_rn(a.x, a.y); }
       }
     }
-    y[c0] = v[0]; y[c1] = v[1];
+  };
+  auto x_at = [&](uint32_t h) { return reinterpret_cast<const uint4*>(p.X + ((size_t)h * p.ldx + r) * 128u); };
+  auto y_at = [&](uint32_t h) { return reinterpret_cast<uint4*>(p.Y + ((size_t)h * p.ldy + r) * 128u); };
+  uint32_t h = h0;
+  for (; h + 4u <= h1; h += 4u) {                      // four heads' loads in flight
+    uint4 v[4][2];
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++) { v[k][0] = ld_now(x_at(h + k) + c0); v[k][1] = ld_now(x_at(h + k) + c1); }
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++) { turned(v[k]); y_at(h + k)[c0] = v[k][0]; y_at(h + k)[c1] = v[k][1]; }
+  }
+  for (; h < h1; h++) {
+    uint4 v[2] = {ld_now(x_at(h) + c0), ld_now(x_at(h) + c1)};
+    turned(v);
+    y_at(h)[c0] = v[0]; y_at(h)[c1] = v[1];
   }
 }
 // the half layout with a part that is no multiple of 16: a warp per row, one pair (or two elements that are copied) per lane and pass
