@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(256, 4) k_cache_write(const CacheP p, const __
 
 // ---- read back: one block = one touched page of one kv head, as in k_cache_write.  K's values go straight to their rows (two lanes swap halves, so
 // that a store fills whole 32-byte pieces), V's through the tile that turns them.
-__global__ void __launch_bounds__(256, 4) k_cache_read(const CacheP p, __half* K, __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
+__global__ void __launch_bounds__(256, 5) k_cache_read(const CacheP p, __half* K, __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
   __shared__ __align__(16) __half tile[CACHE_PAGE * CW_LD];
   const uint32_t tid = threadIdx.x, hk = blockIdx.y, lane = tid & 31u;
   grid_dependency_wait();
@@ -229,15 +229,16 @@ __global__ void __launch_bounds__(256, 4) k_cache_read(const CacheP p, __half* K
     page = ld_now(p.table + (size_t)b * p.max_pages + pg);
     if (page >= p.pages) { if (tid == 0u) cache_tell(p.status, CACHE_BAD_PAGE); return; }
   }
-  uint32_t h[4][8];                                                       // four pieces of 16 values: of one key (K) or of one d (V)
+  uint4 c[4];                                                             // four pieces of 16 codes: of one key (K) or of one d (V)
+  float sc = 0.0f;
   if (whole) {
     const uint4* in = reinterpret_cast<const uint4*>(p.codes + (((size_t)page * p.Hkv + hk) * 2u + w) * CACHE_BLOCK);
-    const float sc = ld_now(reinterpret_cast<const float*>(p.scales + (size_t)page * p.Hkv + hk) + w);
-    uint4 c[4];
+    sc = ld_now(reinterpret_cast<const float*>(p.scales + (size_t)page * p.Hkv + hk) + w);
 #pragma unroll
     for (uint32_t it = 0; it < 4u; it++) c[it] = ld_now(in + it * 128u + i);
-#pragma unroll
-    for (uint32_t it = 0; it < 4u; it++) {
+  }
+  auto values = [&](uint32_t it, uint32_t (&h)[8]) {
+    if (whole) {
       const uint32_t q[4] = {c[it].x, c[it].y, c[it].z, c[it].w};
 #pragma unroll
       for (int j = 0; j < 8; j++) {
@@ -245,28 +246,27 @@ __global__ void __launch_bounds__(256, 4) k_cache_read(const CacheP p, __half* K
         // (a code of 127 times a scale that was rounded up may pass the largest fp16: it stays finite)
         const float lo = fmaxf(fminf((float)((int)(v & 255u) - 128) * sc, 65504.0f), -65504.0f), hi = fmaxf(fminf((float)((int)((v >> 8) & 255u) - 128) * sc, 65504.0f), -65504.0f);
         const __half2 r = __floats2half2_rn(lo, hi);
-        h[it][j] = *reinterpret_cast<const uint32_t*>(&r);
+        h[j] = *reinterpret_cast<const uint32_t*>(&r);
       }
+    } else {
+      const uint4* tl = reinterpret_cast<const uint4*>(p.tail + (((size_t)b * p.Hkv + hk) * 2u + w) * CACHE_BLOCK) + 2u * (it * 128u + i);
+      const uint4 a = ld_now(tl), z = ld_now(tl + 1u);
+      h[0] = a.x; h[1] = a.y; h[2] = a.z; h[3] = a.w; h[4] = z.x; h[5] = z.y; h[6] = z.z; h[7] = z.w;
     }
-  } else {
-    const uint4* tl = reinterpret_cast<const uint4*>(p.tail + (((size_t)b * p.Hkv + hk) * 2u + w) * CACHE_BLOCK);
-#pragma unroll
-    for (uint32_t it = 0; it < 4u; it++) {
-      const uint4 a = ld_now(tl + 2u * (it * 128u + i)), z = ld_now(tl + 2u * (it * 128u + i) + 1u);
-      h[it][0] = a.x; h[it][1] = a.y; h[it][2] = a.z; h[it][3] = a.w; h[it][4] = z.x; h[it][5] = z.y; h[it][6] = z.z; h[it][7] = z.w;
-    }
-  }
+  };
   if (w == 0u) {
     __half* dst = K + (size_t)hk * ldk * 128u;
 #pragma unroll
     for (uint32_t it = 0; it < 4u; it++) {
+      uint32_t h[8];
+      values(it, h);
       const uint32_t u = it * 128u + i, key = (u >> 7) * 16u + ((u >> 3) & 3u) * 4u + ((u >> 6) & 1u) * 2u + ((u >> 2) & 1u), d = ((u >> 5) & 1u) * 64u + (u & 3u) * 16u, pos = pg * CACHE_PAGE + key;
       const bool odd = (lane & 1u) != 0u;
       uint32_t got[4];
 #pragma unroll
-      for (int k = 0; k < 4; k++) got[k] = __shfl_xor_sync(0xffffffffu, odd ? h[it][k] : h[it][4 + k], 1);      // (the even lane gives its upper half for the odd one's lower)
-      const uint4 a = odd ? make_uint4(got[0], got[1], got[2], got[3]) : make_uint4(h[it][0], h[it][1], h[it][2], h[it][3]);
-      const uint4 z = odd ? make_uint4(h[it][4], h[it][5], h[it][6], h[it][7]) : make_uint4(got[0], got[1], got[2], got[3]);
+      for (int k = 0; k < 4; k++) got[k] = __shfl_xor_sync(0xffffffffu, odd ? h[k] : h[4 + k], 1);      // (the even lane gives its upper half for the odd one's lower)
+      const uint4 a = odd ? make_uint4(got[0], got[1], got[2], got[3]) : make_uint4(h[0], h[1], h[2], h[3]);
+      const uint4 z = odd ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(got[0], got[1], got[2], got[3]);
       if (pos >= old && pos < s.L) {                                      // (both lanes have the same key)
         __half* r = dst + (size_t)(row0 + pos) * 128u + (d & ~16u) + (odd ? 8u : 0u);
         *reinterpret_cast<uint4*>(r) = a; *reinterpret_cast<uint4*>(r + 16u) = z;
@@ -275,7 +275,11 @@ __global__ void __launch_bounds__(256, 4) k_cache_read(const CacheP p, __half* K
     return;
   }
 #pragma unroll
-  for (uint32_t it = 0; it < 4u; it++) cache_turn(tile, (it * 128u + i) >> 2, lane, h[it]);
+  for (uint32_t it = 0; it < 4u; it++) {
+    uint32_t h[8];
+    values(it, h);
+    cache_turn(tile, (it * 128u + i) >> 2, lane, h);
+  }
   cache_bar(2u);
   __half* dst = V + (size_t)hk * ldv * 128u;
 #pragma unroll
@@ -304,11 +308,29 @@ __device__ __forceinline__ float2 rope_cs(const RopeP& p, uint32_t i, double pos
   sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
   return make_float2(cs * p.mscale, sn * p.mscale);
 }
-// the position of row r; false for a row of no sequence
+// the position of row r; false for a row of no sequence.  WHOLE: every lane of the warp asks, for one of four rows (lane / 8) from r & ~3 on
+template <bool WHOLE>
 __device__ __forceinline__ bool rope_pos(const RopeP& p, uint32_t r, double& pos) {
   uint32_t b, r0, r1;
-  if (!p.rows) { b = r / p.each; r0 = b * p.each; r1 = r0 + p.each; }
-  else {
+  if (!p.rows) {
+    if (r >= p.M) return false;
+    b = r / p.each; r0 = b * p.each; r1 = r0 + p.each;
+  } else if (WHOLE && p.seqs <= 32u) {                  // one look at the sequences instead of a search
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t from = 0u, to = 0xffffffffu, len = 0u;
+    if (lane < p.seqs) { from = ld_now(p.rows + lane); to = ld_now(p.rows + lane + 1u); len = ld_now(p.lens + lane); }
+    b = 0u;
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++) { const uint32_t n = __popc(__ballot_sync(0xffffffffu, to <= (r & ~3u) + k)); if ((r & 3u) == k) b = n; }
+    r0 = __shfl_sync(0xffffffffu, from, b & 31u); r1 = __shfl_sync(0xffffffffu, to, b & 31u); len = __shfl_sync(0xffffffffu, len, b & 31u);
+    if (b >= p.seqs) return false;
+    if (r < r0 || r >= r1) { if (b > 0u) cache_tell(p.status, CACHE_BAD_ROWS); return false; }
+    CacheSeq s;
+    cache_tell(p.status, cache_seq_check(r0, r1, len, p.M, 0xffffffffu, s));
+    if (s.n == 0u) return false;
+    pos = (double)(s.L - s.n + (r - r0));
+    return true;
+  } else {
     uint32_t lo = 0u, hi = p.seqs;                    // the first sequence whose end is behind r
     while (lo < hi) { const uint32_t mid = (lo + hi) >> 1; if (ld_now(p.rows + mid + 1u) > r) hi = mid; else lo = mid + 1u; }
     if (lo == p.seqs) return false;
@@ -333,9 +355,8 @@ __global__ void __launch_bounds__(128) k_rope(const RopeP p) {
   const uint32_t l = threadIdx.x & 7u, r = blockIdx.x * 16u + (threadIdx.x >> 3), h0 = blockIdx.y * p.hpt, h1 = min(h0 + p.hpt, p.H);
   grid_dependency_wait();
   grid_launch_dependents();
-  if (r >= p.M) return;
-  double pos;
-  if (!rope_pos(p, r, pos)) return;
+  double pos = 0.0;
+  if (!rope_pos<true>(p, r, pos) || r >= p.M) return;
   const uint32_t q = p.rot >> 4;                       // HALF: pieces per half of the turned part
   uint32_t c0, c1, i0;                                 // the thread's two pieces, its first pair
   if (HALF) {
@@ -386,7 +407,7 @@ __global__ void __launch_bounds__(128) k_rope_odd(const RopeP p) {
   grid_launch_dependents();
   if (r >= p.M) return;
   double pos;
-  if (!rope_pos(p, r, pos)) return;
+  if (!rope_pos<false>(p, r, pos)) return;
   const uint32_t half = p.rot >> 1;
   float2 cs[2]; uint32_t a[2], b[2];
 #pragma unroll

@@ -153,6 +153,8 @@ STEPS = [
     dict(label="chunks that begin and end inside pages", Hkv=3, maxp=8, steps=[[37], [64], [27], [130], [1], [63], [65]], rows=False),
     dict(label="several sequences, some without new tokens", Hkv=1, maxp=6, steps=[[5, 0, 70, 1], [60, 1, 0, 63], [1, 0, 64, 0], [130, 200, 3, 1]], rows=True),
     dict(label="equal counts", Hkv=2, maxp=4, steps=[[40] * 5, [1] * 5, [23] * 5, [1] * 5, [100] * 5], rows=False),
+    dict(label="33 sequences", Hkv=2, maxp=4, steps=[[(b * 7) % 66 for b in range(33)], [b % 3 for b in range(33)], [64 + b for b in range(33)]], rows=True),
+    dict(label="128 sequences", Hkv=1, maxp=3, steps=[[(b * 11) % 66 for b in range(128)], [b % 2 for b in range(128)], [70] * 128], rows=True),
     dict(label="more sequences than a block has threads", Hkv=1, maxp=2, steps=[[(b * 7) % 66 for b in range(300)], [1 + b % 3 for b in range(300)]], rows=True),
 ]
 
