@@ -13,8 +13,12 @@ using namespace p0p;
 namespace {
 
 constexpr char OP[] = "cacheAttention";
-// Query rows per kv head up to which a sequence is the split-key kernel's.
-constexpr uint32_t CACHE_SPLIT_ROWS = 64u;
+// Query rows per kv head up to which a sequence is the split-key kernel's.  Its time grows with every 16 rows, the tensor-memory kernel's hardly up to
+// 256, but that one starts later (two launches, a longer pipeline).  Measured, split keys / tensor memory, 8 kv heads:
+//   8 sequences of 16000:  32 rows 78 / 118 us, 48 rows 126 / 119, 64 rows 164 / 121      64 of 4000: 32 rows 175 / 234, 48 rows 253 / 255, 64 rows 332 / 263
+//   1 sequence of 500:     96 rows 13 / 24, 128 rows 13 / 24      of 4000: 96 rows 18 / 29, 128 rows 20 / 28      of 32000: 64 rows 47 / 49, 96 rows 58 / 50, 128 rows 81 / 51
+// so with few sequences and heads, whose contexts hardly fill the machine, the border lies higher.
+inline uint32_t split_rows(uint32_t seqs, uint32_t Hkv) { return (uint64_t)seqs * Hkv <= 16u ? 96u : 48u; }
 
 int run_split(p0p_ctx* c, CacheAttnP& p, uint32_t G) {
   static DeviceOnce once;
@@ -74,7 +78,7 @@ extern "C" int p0p_cache_attention(p0p_ctx* c, const p0p_cache_attn_args* a) {
   const uint32_t M = a->M, Hq = a->Hq, ldq = a->ldq ? a->ldq : M, ldo = a->ldo ? a->ldo : Hq * 128u;
   if (!Hq || Hq > 65535u || Hq % p.c.Hkv) return fail(c, -3, "cacheAttention: Hq must be a multiple of Hkv, at most 65535");
   if (a->kernel != 0u && a->kernel != P0P_K_CACHE_SPLIT && a->kernel != P0P_K_CACHE_TMEM) return fail(c, -2, "cacheAttention: unknown kernel selector %u", a->kernel);
-  if (std::isnan(a->scale) || std::isinf(a->scale)) return fail(c, -2, "cacheAttention: the scale must be finite");
+  if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return fail(c, -2, "cacheAttention: the scale must be finite and not negative");
   if (!M) return 0;
   __half* q;
   if (int rc = cache_heads(c, op, "q", a->q, a->q_off, Hq, M, ldq, q)) return rc;
@@ -92,16 +96,17 @@ extern "C" int p0p_cache_attention(p0p_ctx* c, const p0p_cache_attn_args* a) {
   // Which kernel a sequence is for depends on its number of new tokens.  Without row offsets the host knows it; with them it knows the most any
   // sequence has, if the caller says so, and where that is many, both kernels run, each for its sequences.
   const uint64_t most = (uint64_t)p.group * (p.c.rows ? (a->max_new ? std::min(a->max_new, M) : M) : p.c.each);
+  const uint32_t border = split_rows(p.c.seqs, p.c.Hkv);
   const bool fits = p.group <= 128u, forced = a->kernel != 0u;
   if (a->kernel == P0P_K_CACHE_TMEM && !fits) return fail(c, -2, "cacheAttention: more than 128 heads per kv head are not for the tensor-memory kernel");
-  const bool tc = forced ? a->kernel == P0P_K_CACHE_TMEM : fits && most > CACHE_SPLIT_ROWS, split = forced ? !tc : !tc || p.c.rows;
+  const bool tc = forced ? a->kernel == P0P_K_CACHE_TMEM : fits && most > border, split = forced ? !tc : !tc || p.c.rows;
   if (int rc = ensure_scratch(c, std::max(split ? split_scratch(G) : 0u, tc ? tc_scratch(G) : 0u))) return rc;
   if (split) {
-    p.max_rows = tc ? CACHE_SPLIT_ROWS : 0xffffffffu;
+    p.max_rows = tc ? border : 0xffffffffu;
     if (int rc = run_split(c, p, G)) return rc;
   }
   if (tc) {
-    if (int rc = run_tc(c, p, G, split ? CACHE_SPLIT_ROWS : 0u)) return rc;
+    if (int rc = run_tc(c, p, G, split ? border : 0u)) return rc;
   }
   c->last_kernel = tc ? (split ? P0P_K_CACHE_BOTH : P0P_K_CACHE_TMEM) : P0P_K_CACHE_SPLIT;
   const uint32_t plan[8] = {G};

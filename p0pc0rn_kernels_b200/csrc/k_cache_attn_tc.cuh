@@ -81,7 +81,11 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
   extern __shared__ __align__(1024) unsigned char ctc_raw[];             // (the swizzled tiles; there is no room to align them by hand, and no static shared memory before them)
   const uint32_t base = smem_u32(ctc_raw);
   unsigned char* gbase = ctc_raw;
-  if (base & 1023u) { cache_tell(p.c.status, 633); return; }
+  if (base & 1023u) {
+    grid_dependency_wait();
+    if (threadIdx.x == 0u) { p.desc[blockIdx.x].on = 0u; cache_tell(p.c.status, 633); }
+    return;
+  }
   const uint32_t q_sm = base, kv_sm = base + 2u * ATC_TILE, st_sm = kv_sm + CTC_SLOTS * ATC_TILE, bars = st_sm + 8u * CTC_STAGE;
   const uint32_t q_full = bars, q_empty = bars + 8u, st_full = bars + 16u, kv_full = st_full + 64u, kv_empty = kv_full + 8u * CTC_SLOTS, s_full = kv_empty + 8u * CTC_SLOTS, p_full = s_full + 16u;
   const uint32_t o_full = p_full + 16u, seg_full = o_full + 16u, seg_empty = seg_full + 8u * CTC_SEGS, pair_full = seg_empty + 8u * CTC_SEGS, pair_empty = pair_full + 8u * CTC_PAIRS;

@@ -116,16 +116,17 @@ def _attn_want(q, K, V, window, sinks, scale=None):
     return o.permute(2, 0, 1, 3).reshape(n, Hq, 128).cpu().numpy()
 
 
-def _attend(cache, news, group, window=0, sinks=0, scale=None, rows=True, new=None, kernel=None, seed=5, qstd=1.0, extra=0, ldo=None, nan_row=None):
+def _attend(cache, news, group, window=0, sinks=0, scale=None, rows=True, new=None, kernel=None, seed=5, qstd=1.0, extra=0, ldo=None, nan_row=None, ldq=0):
     """runs cacheAttention for the last `news` tokens of each sequence; returns (out [M][Hq][128], wanted list, q list)"""
     P, gpu, Hq = cache.P, cache.gpu, cache.Hkv * group
     rng = np.random.default_rng(seed)
     offs = np.concatenate([[0], np.cumsum(news)]).astype(np.uint32); M = int(offs[-1]) + extra
-    q = rng.normal(0, qstd, (Hq, M, 128)).astype(np.float16)
+    q = rng.normal(0, qstd, (Hq, M + ldq, 128)).astype(np.float16)
+    if ldq: q[:, M:] = np.nan                                                                  # rows of another call between the heads
     if nan_row is not None: q[nan_row[0], nan_row[1], 3] = np.nan
     ldo = ldo or Hq * 128
     qb, ob, rb = gpu.upload(q), gpu.upload(np.full((M, ldo), 0x7E01, np.uint16)), gpu.upload(offs)
-    P.cacheAttention(gpu, {"cache": cache.d, "q": {"buf": qb}, "o": {"buf": ob, "ld": ldo}, "Hq": Hq, "M": M, "rows": {"buf": rb} if rows else None, "new": new, "window": window,
+    P.cacheAttention(gpu, {"cache": cache.d, "q": {"buf": qb, "ld": M + ldq}, "o": {"buf": ob, "ld": ldo}, "Hq": Hq, "M": M, "rows": {"buf": rb} if rows else None, "new": new, "window": window,
                            "sinks": sinks, "scale": scale, "kernel": kernel})
     raw = gpu.read(ob).view(np.uint16)[:M * ldo].reshape(M, ldo)
     for b in (qb, ob, rb): gpu.free(b)
@@ -169,7 +170,7 @@ def test_write_and_read(gpu, c):
     try:
         for news in c["steps"]:
             k, v = ([(rng.normal(0, 1, (Hkv, n, 128)) * np.exp(rng.normal(0, 1, (Hkv, 1, 1)))).astype(np.float16) for n in news] for _ in range(2))
-            cache.write(news, k, v, rows=c["rows"], extra=2 if c["rows"] else 0)
+            cache.write(news, k, v, rows=c["rows"], extra=2 if c["rows"] else 0, ld=sum(news) + 5)
             got, offs = cache.read(news, rows=c["rows"], extra=1 if c["rows"] else 0)
             for b in range(0, seqs, max(1, seqs // 20)):
                 for g, w in zip(got, cache.held(b)):
@@ -247,6 +248,7 @@ ATT = [
     dict(label="own scale", Hkv=2, group=2, lens=[200], news=[3], scale=0.02),
     dict(label="peaked scores", Hkv=2, group=2, lens=[700], news=[2], qstd=12.0),
     dict(label="output rows with a stride, 4-byte aligned", Hkv=2, group=2, lens=[200], news=[3], ldo=4 * 128 + 6),
+    dict(label="heads with a stride", Hkv=2, group=2, lens=[200, 70], news=[3, 40], ldq=7),
 ]
 
 
@@ -278,12 +280,34 @@ def test_attention(gpu, c, kernel):
     import p0pc0rn_kernels_b200 as P
     cache = _att_cache(P, gpu, c)
     try:
-        kw = {k: c[k] for k in ("window", "sinks", "scale", "qstd", "extra", "ldo") if k in c}
+        kw = {k: c[k] for k in ("window", "sinks", "scale", "qstd", "extra", "ldo", "ldq") if k in c}
         kw["kernel"] = kernel
         for _ in range(2): _check(cache, c["news"], c["group"], **kw)                          # (twice: a counter left over would show)
         if len(set(c["news"])) == 1: _check(cache, c["news"], c["group"], rows=False, new=c["news"][0], **{k: v for k, v in kw.items() if k != "extra"})
     finally:
         cache.free()
+
+
+def test_attention_chooses_by_rows(gpu):
+    """few query rows per kv head go to the split-key kernel, many to the tensor-memory kernel; a batch of both kinds, or one the host cannot know, to both"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 8, 3, 5)
+    cache.fill([300, 200, 250])
+    try:
+        for news, group, rows, new, want in (([1, 1, 1], 4, False, None, 24), ([48, 48, 48], 1, False, None, 24), ([13, 13, 13], 4, False, None, 25), ([1, 0, 2], 4, True, 2, 24),
+                                             ([1, 100, 2], 4, True, 100, 26), ([1, 100, 2], 4, True, None, 26), ([1, 1, 1], 200, False, None, 24)):
+            _check(cache, news, group, rows=rows, new=new)
+            assert gpu.lastKernel == want, (news, group, gpu.lastKernel)
+    finally:
+        cache.free()
+    one = Cache(P, gpu, 8, 1, 5)
+    one.fill([300])
+    try:
+        for n, want in ((24, 24), (25, 25)):
+            _check(one, [n], 4, rows=False)
+            assert gpu.lastKernel == want
+    finally:
+        one.free()
 
 
 def test_attention_scales_far_apart(gpu):
@@ -461,6 +485,44 @@ def _step_check(s, x, turn, own, Hq, Hkv):
         assert np.abs(out[b] - w).max() <= np.abs(V).max() * (2 * (2.0 ** -11 + 1e-4) + 2.0 ** -11 + K.shape[1] * 2.0 ** -25)
 
 
+def test_attention_recorded_before_its_scratch_memory_exists(gpu):
+    import p0pc0rn_kernels_b200 as P
+    own = P.createGpu({"device": 0})
+    cache = Cache(P, own, 2, 1, 3)
+    cache.fill([130])
+    q, o = own.buffer(4 * 256), own.buffer(4 * 256)
+    call = lambda: P.cacheAttention(own, {"cache": cache.d, "q": {"buf": q}, "o": {"buf": o}, "Hq": 4, "M": 1})  # noqa: E731
+    try:
+        with pytest.raises(ValueError, match="run it once before"): own.record(call)
+        assert not own.lost
+        call()
+        g = own.record(call)
+        g.launch(); own.done(); g.free()
+    finally:
+        cache.free(); own.close()
+
+
+def test_same_result_twice_and_in_one_call_of_many(gpu):
+    """bit for bit the same from run to run; a prefix shared by two sequences (one page in two tables) is read by both"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 2, 2, 8)
+    cache.fill([400, 0])
+    try:
+        for kernel in ("split", "tmem"):
+            outs = [_attend(cache, [5, 0], 4, kernel=kernel)[0].tobytes() for _ in range(3)]
+            assert outs[0] == outs[1] == outs[2]
+        t = cache.table.copy(); t[1, :6] = t[0, :6]
+        gpu.upload(t, dst=cache.d["table"]["buf"])
+        rng = np.random.default_rng(3)
+        k, v = (rng.normal(0, 1, (2, 3, 128)).astype(np.float16) for _ in range(2))
+        cache.tok[1] = tuple(x[:, :384] for x in cache.tok[0]); cache.lens[1] = 384
+        empty = np.zeros((2, 0, 128), np.float16)
+        cache.write([0, 3], [empty, k], [empty, v])                        # its own tail behind the shared pages
+        for kernel in ("split", "tmem"): _check(cache, [5, 3], 4, kernel=kernel)
+    finally:
+        cache.free()
+
+
 def test_another_stream(gpu):
     """a context on the host framework's stream: tensors made there, no waiting in between"""
     import torch
@@ -504,7 +566,7 @@ def test_refusals(gpu):
         no(P.cacheWrite, kv, "k needs", M=3000); no(P.cacheWrite, kv, "v.ld", v={"buf": b, "ld": 5}); no(P.cacheWrite, kv, "multiple of 16", k={"buf": b, "off": 4})
         no(P.cacheAttention, at, "multiple of Hkv", Hq=3); no(P.cacheAttention, at, "o needs", o={"buf": b, "ld": 1 << 18}); no(P.cacheAttention, at, "o.ld", o={"buf": b, "ld": 511})
         no(P.cacheAttention, dict(at, Hq=2 * 130), "128 heads", kernel="tmem", q={"buf": b}, o={"buf": b})
-        no(P.cacheAttention, at, "finite", scale=float("nan")); no(P.cacheAttention, at, "q needs", M=3000)
+        no(P.cacheAttention, at, "finite", scale=float("nan")); no(P.cacheAttention, at, "not negative", scale=-0.1); no(P.cacheAttention, at, "q needs", M=3000)
         no(P.rope, ro, "even", rot=7); no(P.rope, ro, "even", rot=130); no(P.rope, ro, "unknown mode", mode="x"); no(P.rope, ro, "positive", theta=-1.0); no(P.rope, ro, "fast above slow", fast=1.0, slow=2.0)
         no(P.rope, ro, "multiple of seqs", M=7); no(P.rope, ro, "x needs", M=3000); no(P.rope, ro, "sequences", seqs=0); no(P.rope, ro, "multiple of 16", x={"buf": b, "off": 2})
         assert not gpu.lost
