@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(256, 4) k_cache_write(const CacheP p, const __
     else if (w == 0u) x[it] = ld_now(reinterpret_cast<const uint4*>(tl + cache_k_off(key, d)));
   }
   __half2 mx = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-  auto largest = [&](uint32_t v) { mx = __hmax2(mx, __habs2(*reinterpret_cast<const __half2*>(&v))); };
+  auto largest = [&](uint32_t v) { mx = __hmax2_nan(mx, __habs2(*reinterpret_cast<const __half2*>(&v))); };
   if (w && have) {                                                        // V's old tokens: pieces of 16 keys of one d
 #pragma unroll 1
     for (uint32_t it = 0; it < 4u; it++) {
@@ -155,12 +155,24 @@ __global__ void __launch_bounds__(256, 4) k_cache_write(const CacheP p, const __
     }
     cache_bar(2u);
   }
+  // (new tokens are cleaned where something is to clean: the largest magnitude says so, a NaN in it stays one)
+  const __half2 old_mx = mx;
 #pragma unroll
-  for (uint32_t it = 0; it < 8u; it++) {
-    const uint32_t key = it * 8u + (i >> 4);
-    x[it].x = cache_clean(x[it].x); x[it].y = cache_clean(x[it].y); x[it].z = cache_clean(x[it].z); x[it].w = cache_clean(x[it].w);
-    largest(x[it].x); largest(x[it].y); largest(x[it].z); largest(x[it].w);
-    if (w && key >= have) *reinterpret_cast<uint4*>(tile + key * CW_LD + (i & 15u) * 8u) = x[it];
+  for (uint32_t it = 0; it < 8u; it++) { largest(x[it].x); largest(x[it].y); largest(x[it].z); largest(x[it].w); }
+  if (!(__low2float(mx) + __high2float(mx) <= 131008.0f)) {
+    mx = old_mx;
+#pragma unroll
+    for (uint32_t it = 0; it < 8u; it++) {
+      x[it].x = cache_clean(x[it].x); x[it].y = cache_clean(x[it].y); x[it].z = cache_clean(x[it].z); x[it].w = cache_clean(x[it].w);
+      largest(x[it].x); largest(x[it].y); largest(x[it].z); largest(x[it].w);
+    }
+  }
+  if (w) {
+#pragma unroll
+    for (uint32_t it = 0; it < 8u; it++) {
+      const uint32_t key = it * 8u + (i >> 4);
+      if (key >= have) *reinterpret_cast<uint4*>(tile + key * CW_LD + (i & 15u) * 8u) = x[it];
+    }
   }
   float m = fmaxf(__low2float(mx), __high2float(mx));
 #pragma unroll
@@ -237,15 +249,18 @@ __global__ void __launch_bounds__(256, 5) k_cache_read(const CacheP p, __half* K
 #pragma unroll
     for (uint32_t it = 0; it < 4u; it++) c[it] = ld_now(in + it * 128u + i);
   }
+  const bool big = sc > 515.0f;                                           // a code of 127 times a scale that was rounded up may pass the largest fp16: it stays finite
   auto values = [&](uint32_t it, uint32_t (&h)[8]) {
     if (whole) {
+      // a byte under 0x4b0000 is 2^23 + code + 128 (the conversion instruction has a sixteenth of the lanes)
       const uint32_t q[4] = {c[it].x, c[it].y, c[it].z, c[it].w};
+      auto value = [&](int k) {
+        const float f = (__uint_as_float(__byte_perm(q[k >> 2], 0x4b000000u, 0x7440 + (k & 3))) - 8388736.0f) * sc;
+        return big ? fmaxf(fminf(f, 65504.0f), -65504.0f) : f;
+      };
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const uint32_t v = q[j >> 1] >> (16 * (j & 1));
-        // (a code of 127 times a scale that was rounded up may pass the largest fp16: it stays finite)
-        const float lo = fmaxf(fminf((float)((int)(v & 255u) - 128) * sc, 65504.0f), -65504.0f), hi = fmaxf(fminf((float)((int)((v >> 8) & 255u) - 128) * sc, 65504.0f), -65504.0f);
-        const __half2 r = __floats2half2_rn(lo, hi);
+        const __half2 r = __floats2half2_rn(value(2 * j), value(2 * j + 1));
         h[j] = *reinterpret_cast<const uint32_t*>(&r);
       }
     } else {
@@ -355,13 +370,23 @@ __global__ void __launch_bounds__(128) k_rope(const RopeP p) {
   const uint32_t l = threadIdx.x & 7u, r = blockIdx.x * 16u + (threadIdx.x >> 3), h0 = blockIdx.y * p.hpt, h1 = min(h0 + p.hpt, p.H);
   grid_dependency_wait();
   grid_launch_dependents();
-  double pos = 0.0;
-  if (!rope_pos<true>(p, r, pos) || r >= p.M) return;
   const uint32_t q = p.rot >> 4;                       // HALF: pieces per half of the turned part
   uint32_t c0, c1, i0;                                 // the thread's two pieces, its first pair
   if (HALF) {
     if (l < q) { c0 = l; c1 = l + q; i0 = 8u * l; } else { c0 = 2u * q + 2u * (l - q); c1 = c0 + 1u; i0 = 64u; }
   } else { c0 = 2u * l; c1 = c0 + 1u; i0 = 8u * l; }
+  auto x_at = [&](uint32_t h) { return reinterpret_cast<const uint4*>(p.X + ((size_t)h * p.ldx + r) * 128u); };
+  auto y_at = [&](uint32_t h) { return reinterpret_cast<uint4*>(p.Y + ((size_t)h * p.ldy + r) * 128u); };
+  // the first four heads are asked for before the position is known (a row of the call can be read whether or not it is a sequence's)
+  uint4 v[4][2];
+  auto four = [&](uint32_t h) {
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++)
+      if (r < p.M && h + k < h1) { v[k][0] = ld_now(x_at(h + k) + c0); v[k][1] = ld_now(x_at(h + k) + c1); }
+  };
+  four(h0);
+  double pos = 0.0;
+  if (!rope_pos<true>(p, r, pos) || r >= p.M) return;
   float2 cs[8];
 #pragma unroll
   for (uint32_t i = 0; i < 8u; i++) cs[i] = rope_cs(p, i0 + i, pos);
@@ -384,20 +409,11 @@ __global__ void __launch_bounds__(128) k_rope(const RopeP p) {
       }
     }
   };
-  auto x_at = [&](uint32_t h) { return reinterpret_cast<const uint4*>(p.X + ((size_t)h * p.ldx + r) * 128u); };
-  auto y_at = [&](uint32_t h) { return reinterpret_cast<uint4*>(p.Y + ((size_t)h * p.ldy + r) * 128u); };
-  uint32_t h = h0;
-  for (; h + 4u <= h1; h += 4u) {                      // four heads' loads in flight
-    uint4 v[4][2];
+  for (uint32_t h = h0; h < h1; h += 4u) {
+    if (h > h0) four(h);
 #pragma unroll
-    for (uint32_t k = 0; k < 4u; k++) { v[k][0] = ld_now(x_at(h + k) + c0); v[k][1] = ld_now(x_at(h + k) + c1); }
-#pragma unroll
-    for (uint32_t k = 0; k < 4u; k++) { turned(v[k]); y_at(h + k)[c0] = v[k][0]; y_at(h + k)[c1] = v[k][1]; }
-  }
-  for (; h < h1; h++) {
-    uint4 v[2] = {ld_now(x_at(h) + c0), ld_now(x_at(h) + c1)};
-    turned(v);
-    y_at(h)[c0] = v[0]; y_at(h)[c1] = v[1];
+    for (uint32_t k = 0; k < 4u; k++)
+      if (h + k < h1) { turned(v[k]); y_at(h + k)[c0] = v[k][0]; y_at(h + k)[c1] = v[k][1]; }
   }
 }
 // the half layout with a part that is no multiple of 16: a warp per row, one pair (or two elements that are copied) per lane and pass
