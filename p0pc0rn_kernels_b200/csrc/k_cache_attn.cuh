@@ -6,17 +6,20 @@
 //   sum of the weights as rounded to fp16 comes from a product with ones: it serves the second term and, times 1 / vs, the softmax's sum.
 //   The second term is taken off page by page: left to the end, the sums of u grow 128 times the number of keys and their rounding with
 //   them (8000 keys in one accumulator: 2e-3 of the result; page by page 2.3e-4, of which 2.1e-4 is the result's own rounding).
-// The running maximum m is that of score + log2 vs: weights are at most 1.  Statistics and sums are fp32; the weights' rounding to fp16 (2^-11 each,
+// The running maximum m is that of score + log2 vs, raised when it grew by more than 2^8: weights are at most 256.  Statistics and sums are fp32; the weights' rounding to fp16 (2^-11 each,
 // independent from key to key) is what tensor-core products of fp32 sums cost, as in k_attn.cuh.
 //
 // Work: a unit = one visible page of one kv head for up to 16 query rows (the rows of all heads that share the kv head, query-major; more
-// rows are more row blocks).  All units of all sequences in one row are dealt out evenly: to blocks (one per SM), within a block to its 8 warps.  So
-// contexts of any mix of lengths fill the machine, and the numbers on the device decide how: nothing but the launch is fixed on the host.
+// rows are more row blocks), and one unit before an item's pages for its fixed cost.  All units of all sequences in one row are dealt out evenly: to
+// blocks (one per SM), within a block to its 8 warps.  So contexts of any mix of lengths fill the machine, and the numbers on the device decide how: nothing but the launch is fixed on the host.
 // A warp streams its pages through two 8-KB buffers of its own by bulk copies, one page ahead.  An item (all pages of a
 // sequence, kv head and row block) that lies within one warp's share is finished there; otherwise partial results (maximum, sum, O)
 // are merged in the block, and across blocks by the warp that arrives last (a counter per row of an item that crosses blocks; it resets
 // it), in order: deterministic, one launch.
-// Bound: one pass over the visible codes (HBM).
+// Bound: one pass over the visible codes (HBM).  32:8 heads, 64 sequences of up to 4096 tokens, 328 MB: 61 to 63 us = 5.3 TB/s, 0.80 of the measured copy (while
+// all warps stream, at its rate; the rest is the launch, the first pages' latency and the end: shares of whole pages of 2.3 us, 3 us to
+// merge).  One sequence of 32000, 66 MB: 19.9 us = 0.50 (three or four pages per warp).  One of 300: 7.1 us, all latency.  Tried and slower: K one more page
+// ahead in a third buffer (66 -> 70 us: V then comes late), asking the L2 for pages 1, 2 or 4 ahead (63 -> 70, 80, 92).
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>

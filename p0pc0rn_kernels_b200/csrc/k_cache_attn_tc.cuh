@@ -2,16 +2,21 @@
 // and tensor memory are those of k_attn_tc.cuh (S = Q K^T, O += P V, two tiles of 128 rows that share every K / V tile, lane = row); what differs:
 //   rows    a tile's rows are the queries of ALL heads that share a kv head, query by query (row = query * group + head), so a page is read
 //           and converted once for them
-//   K, V    arrive as codes (bulk copies) and are turned into fp16 whole numbers - exact - by two
-//           warps for K and two for V, into the swizzled tiles that the multiplies read.  The cache's order makes a lane's 16 codes 32 consecutive bytes of a tile: for K 16 d of
-//           one key, for V 16 keys of one d (so V's tile is K-major).  The keys stand in the order of V's elements in both (cache_col_key).
+//   K, V    arrive as codes (bulk copies) and are turned into fp16 whole numbers - exact - by two warps for K and two for V, into the swizzled
+//           tiles that the multiplies read.  The cache's order makes a lane's 16 codes 32 consecutive bytes of a tile: for K 16 d of one key, for V
+//           16 keys of one d (so V's tile is K-major).  The keys stand in the order of V's elements in both (cache_col_key).
 //   scales  a thread's 64 scores belong to one page: its K scale joins the softmax scale, its V scale the exponent (w = 2^(score + log2 vs - m),
 //           and the sum of the weights is weighted with 1 / vs), as in k_cache_attn.cuh
 //   work    the pairs of visible pages of all items (block of queries, kv head) in one row are dealt out evenly to one block per SM, from the
 //           numbers on the device; an item that crosses blocks leaves partial results that k_cache_merge adds up, in order
-// Roles: warp 0 loads, warp 1 multiplies, warps 4-7 convert, warps 8-15 and 16-23 are the softmax of the two tiles, two threads per row.  The softmax
-// threads take the registers that the others leave (setmaxnreg; per scheduler 4 x 104 + 2 x 32 = the 6 x 80 of the launch).
-// Bound: instruction issue (softmax and conversion) and the tensor cores, in that order.
+// Roles: warp 0 keeps the list of work (items, and page by page what the others need to know), warp 1 multiplies, warp 2 loads queries, warps 4-7 convert,
+// warps 8-15 and 16-23 are the softmax of the two tiles, two threads per row.  The softmax threads take the registers that the others leave
+// (setmaxnreg; per scheduler 4 x 104 + 2 x 32 = the 6 x 80 of the launch).
+// Bound: 2000 tokens over 6100 of 32:8 heads, 233 GFLOP: 247 us = 940 TFLOP/s, 0.57 of the measured burst, under the power limit (1.6 to 1.7 GHz).  A pair of
+// pages takes about 4200 cycles of a block: its multiplies alone 1900 (tensor pipe active 52 %), its traffic through shared memory 2500 (operands, codes
+// in, tiles out), the converting warps about 3500 (latency: a warp's 16 units of 32 bytes, waits and fences in a row), a softmax warp 1700.  Tried and slower: conversion
+// by the softmax warps between two tiles (308 us), K as fp16 subnormals with a row sum of q (255 against 260 then, but 147 against 141 for short
+// items), 96 registers for the softmax and 48 for the others (390), three slots of tiles and more codes (256).
 #pragma once
 #include <cuda.h>
 
@@ -38,9 +43,6 @@ struct CacheTcP {
 // shared memory holds one pair's codes: 4 KB of each page for each converting warp, which asks for the next ones itself as soon as it has read them (one
 // warp loading for all four, or a lane for each of the eight, came late: 4000 cycles from the last read to the next codes).
 constexpr uint32_t CTC_THREADS = 768u, CTC_SLOTS = 4u, CTC_STAGE = CACHE_BLOCK / 2u;
-// of every 16 pairs of scores, how many take their exponential on the FMA pipe: with the conversion in the same issue slots fewer than in k_attn_tc
-// (2000 tokens over 6100, four prompts under a window: 6 260, 148 us; 5 258, 146.8; 4 256, 146.2)
-constexpr int CTC_EMU = 2;
 constexpr int CTC_REGS = 16 * 104 + 8 * 32;      // registers per lane of all warps, after setmaxnreg
 constexpr uint32_t CTC_PAIRS = 4u;     // pairs of pages that are described ahead
 constexpr uint32_t CTC_SEGS = 4u;      // items that are announced ahead
@@ -465,9 +467,9 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
 #pragma unroll
           for (int e = 0; e < 16; e++) {
             const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[32 * c + 2 * e]), __uint_as_float(s[32 * c + 2 * e + 1])), sc2, nm2);
-            float2 pr;
-            if ((e * CTC_EMU) % 16 < CTC_EMU) pr = atc_ex2_poly2(x);
-            else pr = make_float2(atc_ex2(x.x), atc_ex2(x.y));
+            // (all on the special-function unit: here, where the conversion shares the issue slots, a part of them as polynomials on the FMA pipe, which
+            // k_attn_tc.cuh gains from, costs: of 16 pairs 6 260, 148 us; 4 256, 146; 2 254, 140; none 247, 139.6, 2000 tokens over 6100 and four prompts under a window)
+            const float2 pr = make_float2(atc_ex2(x.x), atc_ex2(x.y));
             ls[e & 1] = __fadd2_rn(ls[e & 1], pr);
             const __half2 hp = __floats2half2_rn(pr.x, pr.y);
             pk[e] = *reinterpret_cast<const uint32_t*>(&hp);
