@@ -260,21 +260,22 @@ typedef struct p0p_cache_attn_args {
   uint32_t Hq, M, ldq, ldo;              /* q [Hq][ldq][128] f16 (0 = M); o [M][ldo] f16 token-major at column h * 128 (0 = Hq * 128) */
   uint32_t max_new;                      /* no sequence has more new tokens than this (0 = M; M / seqs without row offsets) */
   uint32_t window, sinks;                /* a query sees the last `window` keys, itself included, and the first `sinks` (window 0: all) */
-  float scale;                           /* 0 = 1 / sqrt(128) */
+  float scale;                           /* 0 = 1 / sqrt(128); at most 2^64 */
   uint32_t kernel;                       /* 0 = the library chooses; P0P_K_CACHE_SPLIT / P0P_K_CACHE_TMEM force one (tests) */
   p0p_cache cache;
   p0p_buf *q, *o, *rows;
   uint64_t q_off, o_off, rows_off;
 } p0p_cache_attn_args;
 /* causal attention of the call's queries over the cache, which holds their own keys and values already (p0p_cache_write comes first).
- * Query head h reads kv head h / (Hq / Hkv).  Partial results are kept in the context's scratch memory. */
+ * Query head h reads kv head h / (Hq / Hkv).  Partial results are kept in the context's scratch memory.  o may overlap neither q nor the cache.
+ * Arithmetic: scores and sums in fp32; a weight of the softmax, times its block's V scale, is rounded to fp16 relative to the largest such product of its row. */
 int p0p_cache_attention(p0p_ctx* ctx, const p0p_cache_attn_args* args);
 
-/* rotary positions: y = x with the first `rot` elements of every head turned by its token's position (y may be x).  x, y [H][ld][128] f16; positions
- * and rows as for a cache.  mode 0 interleaved: pairs (2i, 2i + 1); 1 half: pairs (i, i + rot / 2).  Pair i turns by position * f_i,
- * f_i = theta^(-2i / rot); with factor != 1: f_i / factor where original == 0, else f_i (g + (1 - g) / factor) with
- * g = clamp((original f_i / 2 pi - slow) / (fast - slow), 0, 1): frequencies that turn at least `fast` times within the original context stay,
- * those below `slow` times are divided.  The turned elements are multiplied by mscale.  Angles are reduced in 64 bits. */
+/* rotary positions: y = x with the first `rot` elements of every head turned by its token's position (y may be x, but not overlap it
+ * otherwise). x, y [H][ld][128] f16; positions and rows as for a cache. mode 0 interleaved: pairs (2i, 2i + 1); 1 half: pairs (i, i + rot /
+ * 2). Pair i turns by position * f_i, f_i = theta^(-2i / rot); with factor != 1: f_i / factor where original == 0, else f_i (g + (1 - g) /
+ * factor) with g = clamp((original f_i / 2 pi - slow) / (fast - slow), 0, 1): frequencies that turn at least `fast` times within the
+ * original context stay, those below `slow` times are divided. The turned elements are multiplied by mscale. Angles are reduced in 64 bits. */
 typedef struct p0p_rope_args {
   uint32_t struct_size;
   uint32_t H, M, ldx, ldy, seqs, mode, rot;                              /* ld 0 = M; rot even, at most 128 */

@@ -78,7 +78,7 @@ extern "C" int p0p_cache_attention(p0p_ctx* c, const p0p_cache_attn_args* a) {
   const uint32_t M = a->M, Hq = a->Hq, ldq = a->ldq ? a->ldq : M, ldo = a->ldo ? a->ldo : Hq * 128u;
   if (!Hq || Hq > 65535u || Hq % p.c.Hkv) return fail(c, -3, "cacheAttention: Hq must be a multiple of Hkv, at most 65535");
   if (a->kernel != 0u && a->kernel != P0P_K_CACHE_SPLIT && a->kernel != P0P_K_CACHE_TMEM) return fail(c, -2, "cacheAttention: unknown kernel selector %u", a->kernel);
-  if (!(a->scale >= 0.0f) || std::isinf(a->scale)) return fail(c, -2, "cacheAttention: the scale must be finite and not negative");
+  if (!(a->scale >= 0.0f) || a->scale > 0x1p64f) return fail(c, -2, "cacheAttention: the scale must be finite and not negative, at most 2^64");
   if (!M) return 0;
   __half* q;
   if (int rc = cache_heads(c, op, "q", a->q, a->q_off, Hq, M, ldq, q)) return rc;
@@ -90,7 +90,8 @@ extern "C" int p0p_cache_attention(p0p_ctx* c, const p0p_cache_attn_args* a) {
   if (reinterpret_cast<uintptr_t>(p.O) & 3u) return fail(c, -5, "cacheAttention: o must lie at a multiple of 4 bytes");
   p.Hq = Hq; p.group = Hq / p.c.Hkv; p.ldq = ldq; p.ldo = ldo; p.window = a->window; p.sinks = a->window ? a->sinks : 0u;
   if ((uint64_t)M * p.group > 0x7fffffffu) return fail(c, -5, "cacheAttention: too many rows for one call");
-  p.scale_log2 = (a->scale > 0.0f ? a->scale : 1.0f / std::sqrt(128.0f)) * 1.4426950408889634f;
+  // (a product of 128 pairs is below 2^39: scores stay finite, and a scale below 2^-80 leaves nothing of them.  It is kept above 0: a hidden key's -infinity times it)
+  p.scale_log2 = std::max(a->scale > 0.0f ? a->scale : 1.0f / std::sqrt(128.0f), 0x1p-80f) * 1.4426950408889634f;
   DeviceGuard g(c->device);
   const uint32_t G = std::min<uint32_t>((uint32_t)c->prop.multiProcessorCount, c->n_counters / 16u);
   // Which kernel a sequence is for depends on its number of new tokens.  Without row offsets the host knows it; with them it knows the most any

@@ -2,8 +2,9 @@
 // with a sliding window and first tokens that stay visible.  K and V go from the cache's codes straight to the tensor cores:
 //   a code byte u = code + 128 put into an fp16's low bits IS the subnormal u * 2^-24, one byte permute per pair, so
 //   q . k = ks (2^24 (q . u 2^-24) - 128 sum q): the second term is the accumulator's starting value (a product with a constant operand)
-//   sum p v = vs (2^24 (sum p u 2^-24) - 128 sum p): the page's scale joins the probability's exponent, w = 2^(score + log2 vs - m), and the
-//   sum of the weights as rounded to fp16 comes from a product with ones: it serves the second term and, times 1 / vs, the softmax's sum.
+//   sum p v = vs (2^24 (sum p u 2^-24) - 128 sum p): the page's scale joins the probability's exponent, w = 2^(score + log2 vs - m).  The second
+//   term takes the weights as rounded to fp16, summed by a product with ones.  The softmax's sum adds up w / vs from the weights before their
+//   rounding: where a page's scale is 2^20 times another's, the other's weights are subnormals or 0, which its own small values bear but the sum would not.
 //   The second term is taken off page by page: left to the end, the sums of u grow 128 times the number of keys and their rounding with
 //   them (8000 keys in one accumulator: 2e-3 of the result; page by page 2.3e-4, of which 2.1e-4 is the result's own rounding).
 // The running maximum m is that of score + log2 vs, raised when it grew by more than 2^8: weights are at most 256.  Statistics and sums are fp32; the weights' rounding to fp16 (2^-11 each,
@@ -16,7 +17,7 @@
 // sequence, kv head and row block) that lies within one warp's share is finished there; otherwise partial results (maximum, sum, O)
 // are merged in the block, and across blocks by the warp that arrives last (a counter per row of an item that crosses blocks; it resets
 // it), in order: deterministic, one launch.
-// Bound: one pass over the visible codes (HBM).  32:8 heads, 64 sequences of up to 4096 tokens, 328 MB: 61 to 63 us = 5.3 TB/s, 0.80 of the measured copy (while
+// Bound: one pass over the visible codes (HBM).  32:8 heads, 64 sequences of up to 4096 tokens, 328 MB: 62 to 64 us = 5.2 TB/s, 0.79 of the measured copy (while
 // all warps stream, at its rate; the rest is the launch, the first pages' latency and the end: shares of whole pages of 2.3 us, 3 us to
 // merge).  One sequence of 32000, 66 MB: 19.9 us = 0.50 (three or four pages per warp).  One of 300: 7.1 us, all latency.  Tried and slower: K one more page
 // ahead in a third buffer (66 -> 70 us: V then comes late), asking the L2 for pages 1, 2 or 4 ahead (63 -> 70, 80, 92).
@@ -165,18 +166,21 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
       }
       const float e0 = m[0] == -INFINITY ? 0.0f : lv - m[0], e1 = m[1] == -INFINITY ? 0.0f : lv - m[1];      // (a row that has seen no key yet: all its weights are 0)
       zp[0] = zp[1] = zp[2] = zp[3] = 0.0f;
+      float2 z0 = make_float2(0.0f, 0.0f), z1 = z0;
 #pragma unroll
       for (uint32_t j = 0; j < 4u; j++) {
 #pragma unroll
         for (uint32_t h = 0; h < 2u; h++) {
           const float* x = s[2u * j + h];
           const float2 u0 = __ffma2_rn(make_float2(x[0], x[1]), make_float2(f, f), make_float2(e0, e0)), u1 = __ffma2_rn(make_float2(x[2], x[3]), make_float2(f, f), make_float2(e1, e1));
-          pa[j][2u * h] = at_pack(at_ex2(u0.x), at_ex2(u0.y));
-          pa[j][2u * h + 1u] = at_pack(at_ex2(u1.x), at_ex2(u1.y));
+          const float2 w0 = make_float2(at_ex2(u0.x), at_ex2(u0.y)), w1 = make_float2(at_ex2(u1.x), at_ex2(u1.y));
+          z0 = __fadd2_rn(z0, w0); z1 = __fadd2_rn(z1, w1);
+          pa[j][2u * h] = at_pack(w0.x, w0.y);
+          pa[j][2u * h + 1u] = at_pack(w1.x, w1.y);
         }
         at_mma(zp, pa[j], 0x3c003c00u, 0x3c003c00u);
       }
-      l[0] = fmaf(zp[0], inv_v, l[0]); l[1] = fmaf(zp[2], inv_v, l[1]);
+      l[0] = fmaf(z0.x + z0.y, inv_v, l[0]); l[1] = fmaf(z1.x + z1.y, inv_v, l[1]);
     };
     // a thread's two query rows (rows past the end repeat the last one; they are not stored)
     auto queries = [&](const CacheCursor& c) {
@@ -338,6 +342,8 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
         next_item(1u);
       }
       // ---- the end of the item, or of this warp's share
+#pragma unroll
+      for (int h = 0; h < 2; h++) { l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1); l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2); }
       if (more) queries(nxt);                                              // (on their way while the result leaves)
       if (done && i0 + 1u >= w0) {
         const float inv[2] = {l[0] > 0.0f ? 1.0f / l[0] : l[0], l[1] > 0.0f ? 1.0f / l[1] : l[1]};

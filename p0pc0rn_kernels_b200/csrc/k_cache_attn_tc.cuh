@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
           if (!__all_sync(0xffffffffu, rdy)) { ok = false; break; }
           const uint64_t vd = umma_desc_sw128(kv_sm + sv * ATC_TILE), kd = umma_desc_sw128(kv_sm + sk * ATC_TILE);
           for (uint32_t t = 0; t < nt; t++) {
-                        if (!__all_sync(0xffffffffu, mbar_wait(p_full + 8u * t, np[t] & 1u, p.c.status, 627))) { ok = false; break; }
+            if (!__all_sync(0xffffffffu, mbar_wait(p_full + 8u * t, np[t] & 1u, p.c.status, 627))) { ok = false; break; }
             np[t]++;
             tc_fence_after();
             const uint32_t s_col = tmem_base + t * 128u, o_col = tmem_base + 256u + t * 128u;
@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
       float m_used = -INFINITY, l = 0.0f;
       for (uint32_t j = 0; j < cnt; j++, n++, pair++) {
         // (a wait that ran out: the thread goes on without it, so that its partner is not left at the barrier; the status word is set)
-                if (ok && !mbar_wait(s_full + 8u * t, n & 1u, p.c.status, 630)) ok = false;
+        if (ok && !mbar_wait(s_full + 8u * t, n & 1u, p.c.status, 630)) ok = false;
         tc_fence_after();
         uint32_t s[64];
 #pragma unroll

@@ -327,6 +327,41 @@ def test_attention_scales_far_apart(gpu):
         cache.free()
 
 
+@pytest.mark.parametrize("kernel", ["split", "tmem"])
+@pytest.mark.parametrize("shift", [14, 20, 26])
+def test_attention_sum_where_a_small_page_weighs_most(gpu, shift, kernel):
+    """half of the weight, or nearly all of it, lies on pages whose values are 2^-shift of the others': it counts in full"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 2, 1, 6)
+    rng = np.random.default_rng(6)
+    k = rng.normal(0, 0.02, (2, 300, 128)); v = rng.normal(0, 1, (2, 300, 128))
+    k[1, :128] *= 30.0                                                                         # (the second head: weights that vary)
+    v[:, :128] *= 2.0 ** (9 - shift); v[:, 128:] *= 2.0 ** 9
+    try:
+        cache.write([300], [k.astype(np.float16)], [v.astype(np.float16)], rows=False)
+        _check(cache, [2], 4, kernel=kernel)
+        _check(cache, [170], 4, kernel=kernel)
+    finally:
+        cache.free()
+
+
+@pytest.mark.parametrize("kernel", ["split", "tmem"])
+@pytest.mark.parametrize("scale", [1e-45, 1e-30, 1e-6, 300.0])
+def test_attention_scales_of_any_size(gpu, scale, kernel):
+    """a scale that leaves nothing of the scores is an average; a large one is the largest score's value, kept apart here by their distance"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 1, 1, 4)
+    rng = np.random.default_rng(7)
+    k = np.zeros((1, 200, 128)); k[0, :, 0] = rng.permutation(200) - 100.0                     # (scores apart by |q0|: nothing is rounded, a second key has no weight)
+    v = rng.normal(0, 1, (1, 200, 128))
+    try:
+        cache.write([200], [k.astype(np.float16)], [v.astype(np.float16)], rows=False)
+        _check(cache, [3], 2, scale=scale, kernel=kernel)
+        _check(cache, [3], 2, window=90, sinks=3, scale=scale, kernel=kernel)
+    finally:
+        cache.free()
+
+
 def test_attention_nan_query_stays_in_its_row(gpu):
     import p0pc0rn_kernels_b200 as P
     cache = Cache(P, gpu, 2, 2, 10)
