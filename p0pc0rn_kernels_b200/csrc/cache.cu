@@ -74,7 +74,7 @@ extern "C" int p0p_rope(p0p_ctx* c, const p0p_rope_args* a) {
   const bool odd = a->mode == 1u && (a->rot & 15u);
   const uint32_t rows_per_block = odd ? 4u : 16u, gx = (M + rows_per_block - 1u) / rows_per_block;
   // heads per thread: the angles are worked out once per thread, so as many as leave one round of blocks (7 of 128 threads fit an SM).  (5 sequences, 4145
-  // tokens, 40 heads: eight heads each, a round and a quarter, 21.5 us)
+  // tokens, 40 heads: eight heads each, a round and a quarter, 21.5 us; so 19.6)
   const uint32_t gy = (uint32_t)std::min<uint64_t>(p.H, std::max<uint64_t>(1u, 7ull * (uint32_t)c->prop.multiProcessorCount / gx));
   p.hpt = (p.H + gy - 1u) / gy;
   DeviceGuard g(c->device);

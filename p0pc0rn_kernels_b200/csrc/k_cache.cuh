@@ -106,7 +106,9 @@ __device__ __forceinline__ float cache_scale(float amax) {
 // the tail, new ones from the rows) are read with their largest magnitude found on the way; K's codes leave from the registers, 8 per thread and store, V's
 // through a tile in shared memory that turns them.  The unfinished last page only takes its new tokens into the tail; where the call
 // also finishes a page that began in the tail, that page's block does it, after it has read the tail.
-// Bound: HBM for prompts (256 bytes read and 128 written per token, head and K or V), launch latency for steps.
+// Bound: HBM for prompts (256 bytes read and 128 written per token, head and K or V), launch latency for steps.  8000 tokens of 8 heads, 49 MB: 17.3 us =
+// 2.8 TB/s, 0.43 of the measured copy (126 pages x 8 heads are 1008 blocks, 1.7 rounds of four per SM; five per SM, at 48 registers, are slower by
+// 0.3 us).  One token for each of 64 sequences: 4.9 us.
 __global__ void __launch_bounds__(256, 4) k_cache_write(const CacheP p, const __half* K, const __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
   __shared__ __align__(16) __half tile[CACHE_PAGE * CW_LD];
   __shared__ float sm_max[8];
@@ -225,6 +227,8 @@ __global__ void __launch_bounds__(256, 4) k_cache_write(const CacheP p, const __
 
 // ---- read back: one block = one touched page of one kv head, as in k_cache_write.  K's values go straight to their rows (two lanes swap halves, so
 // that a store fills whole 32-byte pieces), V's through the tile that turns them.
+// Bound: HBM.  Four sequences of up to 20000 tokens, 8 heads, 352 MB: 65 us = 5.4 TB/s, 0.83 of the measured copy; 8000 tokens, 49 MB: 12.5 us, 0.60 (the
+// launch and one round of blocks); 300 tokens: 4.8 us.
 __global__ void __launch_bounds__(256, 5) k_cache_read(const CacheP p, __half* K, __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
   __shared__ __align__(16) __half tile[CACHE_PAGE * CW_LD];
   const uint32_t tid = threadIdx.x, hk = blockIdx.y, lane = tid & 31u;
@@ -364,7 +368,8 @@ __device__ __forceinline__ void rope_turn(float2 cs, float& a, float& b) { const
 // 8 threads per row, 16 elements each as two 16-byte pieces; a thread works out its 8 angles once and turns hpt heads with them.
 // HALF: pieces l and l + rot / 16 of the row's first part pair up (rot a multiple of 16: a pair of pieces holds pairs of one
 // index each); threads whose pieces lie behind the turned part copy.  Otherwise: pieces 2 l and 2 l + 1, pairs within a piece.
-// Bound: HBM for prompts (512 bytes per row and head), launch latency for a step.
+// Bound: HBM for prompts (512 bytes per row and head), launch latency for a step.  4145 rows of 40 heads, 85 MB: 19.6 us = 4.3 TB/s, 0.66 of the measured
+// copy (the positions, eight sines each reduced in 64 bits, stand before the first store).  One row: 5.2 us.
 template <bool HALF>
 __global__ void __launch_bounds__(128) k_rope(const RopeP p) {
   const uint32_t l = threadIdx.x & 7u, r = blockIdx.x * 16u + (threadIdx.x >> 3), h0 = blockIdx.y * p.hpt, h1 = min(h0 + p.hpt, p.H);

@@ -13,7 +13,7 @@
 // warps 8-15 and 16-23 are the softmax of the two tiles, two threads per row.  The softmax threads take the registers that the others leave
 // (setmaxnreg; per scheduler 4 x 104 + 2 x 32 = the 6 x 80 of the launch).
 // Bound: 2000 tokens over 6100 of 32:8 heads, 233 GFLOP: 247 us = 940 TFLOP/s, 0.57 of the measured burst, under the power limit (1.6 to 1.7 GHz).  A pair of
-// pages takes about 4200 cycles of a block: its multiplies alone 1900 (tensor pipe active 52 %), its traffic through shared memory 2500 (operands, codes
+// pages takes about 4200 cycles of a block: its multiplies alone 1900 (tensor pipe active 54 %), its traffic through shared memory 2500 (operands, codes
 // in, tiles out), the converting warps about 3500 (latency: a warp's 16 units of 32 bytes, waits and fences in a row), a softmax warp 1700.  Tried and slower: conversion
 // by the softmax warps between two tiles (308 us), K as fp16 subnormals with a row sum of q (255 against 260 then, but 147 against 141 for short
 // items), 96 registers for the softmax and 48 for the others (390), three slots of tiles and more codes (256).

@@ -362,6 +362,44 @@ def test_attention_scales_of_any_size(gpu, scale, kernel):
         cache.free()
 
 
+@pytest.mark.parametrize("kernel", ["split", "tmem"])
+def test_pages_behind_the_window_can_be_given_away(gpu, kernel):
+    """the table's entries of pages that no query sees, and that hold no sink, are not followed: they name no page here"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 2, 2, 20)
+    cache.fill([1000, 520])
+    try:
+        table = cache.table.copy()
+        for b, (L, n) in enumerate(((1000, 70), (520, 3))):                                    # window 200: the oldest query, L - n, sees L - n - 199 and later ones; sinks: 130 tokens
+            table[b, 3:(L - n - 199) // 64] = 0xFFFFFFFF
+            table[b, L // 64:] = 0xFFFFFFFF
+        assert (table[0, 3:11] == 0xFFFFFFFF).all() and table[1, 3] == 0xFFFFFFFF and table[1, 4] != 0xFFFFFFFF
+        gpu.upload(table, dst=cache.d["table"]["buf"])
+        _check(cache, [70, 3], 4, window=200, sinks=130, kernel=kernel)
+        gpu.done()
+    finally:
+        cache.free()
+
+
+def test_layers_that_share_table_and_lengths(gpu):
+    """two layers' caches with one table and one set of lengths, which a program uploads once a step"""
+    import p0pc0rn_kernels_b200 as P
+    one = Cache(P, gpu, 2, 2, 4)
+    two = Cache(P, gpu, 1, 2, 4, seed=0)
+    for k in ("table", "lens"): gpu.free(two.d[k]["buf"])
+    two.d = {**two.d, **{k: P.kvCache(gpu, {"Hkv": 1, "pages": two.pages, "seqs": 2, "maxPages": 4, "table": one.d["table"], "lens": one.d["lens"]})[k] for k in ("table", "lens")}}
+    try:
+        assert two.d["table"]["buf"] is one.d["table"]["buf"] and two.d["lens"]["buf"] is one.d["lens"]["buf"]
+        rng = np.random.default_rng(3)
+        for news in ([100, 7], [1, 1], [30, 60]):
+            for c in (one, two):
+                c.write(news, *([rng.normal(0, 1, (c.Hkv, n, 128)).astype(np.float16) for n in news] for _ in range(2)))
+        for c in (one, two): _check(c, [30, 60], 2)
+    finally:
+        for k in ("codes", "scales", "tail"): gpu.free(two.d[k]["buf"])
+        one.free()
+
+
 def test_attention_nan_query_stays_in_its_row(gpu):
     import p0pc0rn_kernels_b200 as P
     cache = Cache(P, gpu, 2, 2, 10)
