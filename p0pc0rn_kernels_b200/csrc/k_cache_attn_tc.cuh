@@ -11,7 +11,7 @@
 //           numbers on the device; an item that crosses blocks leaves partial results that k_cache_merge adds up, in order
 // Roles: warp 0 keeps the list of work (items, and page by page what the others need to know), warp 1 multiplies, warp 2 loads queries, warps 4-7 convert,
 // warps 8-15 and 16-23 are the softmax of the two tiles, two threads per row.  The softmax threads take the registers that the others leave
-// (setmaxnreg; per scheduler 4 x 104 + 2 x 32 = the 6 x 80 of the launch).
+// (setmaxnreg; per scheduler 4 x 104 + 24 + 40 = the 6 x 80 of the launch; with 32 for each of the others the converting warps spilled: 249 against 246.5 us).
 // Bound: 2000 tokens over 6100 of 32:8 heads, 233 GFLOP: 247 us = 940 TFLOP/s, 0.57 of the measured burst, under the power limit (1.6 to 1.7 GHz).  A pair of
 // pages takes about 4200 cycles of a block: its multiplies alone 1900 (tensor pipe active 54 %), its traffic through shared memory 2500 (operands, codes
 // in, tiles out), the converting warps about 3500 (latency: a warp's 16 units of 32 bytes, waits and fences in a row), a softmax warp 1700.  Tried and slower: conversion
@@ -43,7 +43,7 @@ struct CacheTcP {
 // shared memory holds one pair's codes: 4 KB of each page for each converting warp, which asks for the next ones itself as soon as it has read them (one
 // warp loading for all four, or a lane for each of the eight, came late: 4000 cycles from the last read to the next codes).
 constexpr uint32_t CTC_THREADS = 768u, CTC_SLOTS = 4u, CTC_STAGE = CACHE_BLOCK / 2u;
-constexpr int CTC_REGS = 16 * 104 + 8 * 32;      // registers per lane of all warps, after setmaxnreg
+constexpr int CTC_REGS = 16 * 104 + 4 * 24 + 4 * 40;      // registers per lane of all warps, after setmaxnreg
 constexpr uint32_t CTC_PAIRS = 4u;     // pairs of pages that are described ahead
 constexpr uint32_t CTC_SEGS = 4u;      // items that are announced ahead
 // an item's share
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
   auto seg_done = [&](uint32_t seg) { __syncwarp(); if (lane == 0u) mbar_arrive(seg_empty + 8u * (seg % CTC_SEGS)); };
 
   if (warp < 4u) {
-    regs_down<32>();
+    regs_down<24>();
     if (warp == 0u) {
       // ================================================================= the list of work: items, and page by page what the others need to know.  Lane l looks
       // after the l-th of 32 visible pages
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
     }
   } else if (warp < 8u) {
     // ================================================================= codes (or the tail's fp16) -> fp16 tiles
-    regs_down<32>();
+    regs_down<40>();
     // Two warps for K, two for V; a warp has half of each page: units 256 part + 32 e + lane of its 512 (16 elements each).  A unit's 32 bytes go to row r of the
     // tile's half h, pieces 2 (u % 4) and the next, swizzled
     //   K: r = 64 page + 16 (u / 8 % 4) + 4 (u / 128) + 2 (u / 64 % 2) + u / 4 % 2 (the key's column), h = u / 32 % 2 (which 64 of d);   V: r = u / 4 (d), h = page
