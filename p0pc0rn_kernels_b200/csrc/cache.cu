@@ -10,7 +10,7 @@ using namespace p0p;
 namespace {
 
 template <class Kern, class T>
-int cache_move(p0p_ctx* c, const char* op, const p0p_cache_args* a, Kern kern, T*) {
+int cache_move(p0p_ctx* c, const char* op, const p0p_cache_args* a, Kern kern, bool heads_first, T*) {
   P0P_ALIVE(c);
   if (!a || a->struct_size < sizeof(p0p_cache_args)) return fail(c, -1, "%s: bad argument block", op);
   CacheP p{};
@@ -21,9 +21,9 @@ int cache_move(p0p_ctx* c, const char* op, const p0p_cache_args* a, Kern kern, T
   if (int rc = cache_heads(c, op, "k", a->k, a->k_off, p.Hkv, M, ldk, k)) return rc;
   if (int rc = cache_heads(c, op, "v", a->v, a->v_off, p.Hkv, M, ldv, v)) return rc;
   const uint64_t per = p.rows ? 0u : cache_touched_bound(p.each, 1u), blocks = p.rows ? cache_touched_bound(M, p.seqs) : per * p.seqs;
-  if (blocks > 0x7fffffffu) return fail(c, -5, "%s: too many rows for one call", op);
+  if (blocks * p.Hkv > 0x7fffffffu) return fail(c, -5, "%s: too many rows for one call", op);
   DeviceGuard g(c->device);
-  const cudaError_t e = launch_chained(kern, dim3((uint32_t)blocks, p.Hkv), dim3(256), 0, c->stream, p, (T*)k, (T*)v, ldk, ldv, (uint32_t)per);
+  const cudaError_t e = launch_chained(kern, heads_first ? dim3((uint32_t)blocks * p.Hkv) : dim3((uint32_t)blocks, p.Hkv), dim3(256), 0, c->stream, p, (T*)k, (T*)v, ldk, ldv, (uint32_t)per);
   if (e != cudaSuccess) return cuda_fail(c, e, op);
   c->launches += 1;
   return 0;
@@ -31,8 +31,8 @@ int cache_move(p0p_ctx* c, const char* op, const p0p_cache_args* a, Kern kern, T
 
 }  // namespace
 
-extern "C" int p0p_cache_write(p0p_ctx* c, const p0p_cache_args* a) { return cache_move(c, "cacheWrite", a, k_cache_write, (const __half*)nullptr); }
-extern "C" int p0p_cache_read(p0p_ctx* c, const p0p_cache_args* a) { return cache_move(c, "cacheRead", a, k_cache_read, (__half*)nullptr); }
+extern "C" int p0p_cache_write(p0p_ctx* c, const p0p_cache_args* a) { return cache_move(c, "cacheWrite", a, k_cache_write, true, (const __half*)nullptr); }
+extern "C" int p0p_cache_read(p0p_ctx* c, const p0p_cache_args* a) { return cache_move(c, "cacheRead", a, k_cache_read, false, (__half*)nullptr); }
 
 extern "C" int p0p_rope(p0p_ctx* c, const p0p_rope_args* a) {
   P0P_ALIVE(c);

@@ -106,18 +106,19 @@ __device__ __forceinline__ float cache_scale(float amax) {
 // the tail, new ones from the rows) are read with their largest magnitude found on the way; K's codes leave from the registers, 8 per thread and store, V's
 // through a tile in shared memory that turns them.  The unfinished last page only takes its new tokens into the tail; where the call
 // also finishes a page that began in the tail, that page's block does it, after it has read the tail.
-// Bound: HBM for prompts (256 bytes read and 128 written per token, head and K or V), launch latency for steps.  8000 tokens of 8 heads, 49 MB: 17.3 us =
-// 2.8 TB/s, 0.43 of the measured copy (126 pages x 8 heads are 1008 blocks, 1.7 rounds of four per SM; five per SM, at 48 registers, are slower by
-// 0.3 us).  One token for each of 64 sequences: 4.9 us.
+// Bound: HBM for prompts (256 bytes read and 128 written per token, head and K or V), launch latency for steps.  8000 tokens of 8 heads, 49 MB: 15.3 us =
+// 3.2 TB/s, 0.49 of the measured copy (126 pages x 8 heads are 1008 blocks, 1.7 rounds of four per SM; five per SM, at 48 registers, are slower by
+// 0.3 us).  One token for each of 64 sequences: 4.9 us.  The heads of a page are neighbours in the grid: the pages that began in the tail take longest and
+// stand first (with pages as neighbours the last heads' came in the last round, 17.3 us).
 __global__ void __launch_bounds__(256, 4) k_cache_write(const CacheP p, const __half* K, const __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
   __shared__ __align__(16) __half tile[CACHE_PAGE * CW_LD];
   __shared__ float sm_max[8];
-  const uint32_t tid = threadIdx.x, hk = blockIdx.y;
+  const uint32_t tid = threadIdx.x, hk = blockIdx.x % p.Hkv;
   grid_dependency_wait();
   grid_launch_dependents();
   uint32_t b, local;
   CacheSeq s;
-  if (!cache_find_page(p, blockIdx.x, per_seq, b, local, s)) return;
+  if (!cache_find_page(p, blockIdx.x / p.Hkv, per_seq, b, local, s)) return;
   const uint32_t first = cache_first_page(s), old = s.L - s.n, pg = first + local, last = s.L / CACHE_PAGE;
   const uint32_t row0 = s.r0 - old;                                       // (wraps: only sums with positions >= old are rows)
   __half* tk = p.tail + ((size_t)b * p.Hkv + hk) * 2u * CACHE_BLOCK; __half* tv = tk + CACHE_BLOCK;
@@ -227,6 +228,7 @@ __global__ void __launch_bounds__(256, 4) k_cache_write(const CacheP p, const __
 
 // ---- read back: one block = one touched page of one kv head, as in k_cache_write.  K's values go straight to their rows (two lanes swap halves, so
 // that a store fills whole 32-byte pieces), V's through the tile that turns them.
+// (Here pages are neighbours in the grid: no page takes longer, and 352 MB are read in 66.3 us against 67.3 with heads as neighbours.)
 // Bound: HBM.  Four sequences of up to 20000 tokens, 8 heads, 352 MB: 65 us = 5.4 TB/s, 0.83 of the measured copy; 8000 tokens, 49 MB: 12.5 us, 0.60 (the
 // launch and one round of blocks); 300 tokens: 4.8 us.
 __global__ void __launch_bounds__(256, 5) k_cache_read(const CacheP p, __half* K, __half* V, uint32_t ldk, uint32_t ldv, uint32_t per_seq) {
