@@ -15,8 +15,8 @@ namespace {
 constexpr char OP[] = "cacheAttention";
 // Query rows per kv head up to which a sequence is the split-key kernel's.  Its time grows with every 16 rows, the tensor-memory kernel's hardly up to
 // 256, but that one starts later (two launches, a longer pipeline).  Measured, split keys / tensor memory, 8 kv heads:
-//   8 sequences of 16000:  32 rows 78 / 118 us, 48 rows 126 / 119, 64 rows 164 / 121      64 of 4000: 32 rows 175 / 234, 48 rows 253 / 255, 64 rows 332 / 263
-//   1 sequence of 500:     96 rows 13 / 24, 128 rows 13 / 24      of 4000: 96 rows 18 / 29, 128 rows 20 / 28      of 32000: 64 rows 47 / 49, 96 rows 58 / 50, 128 rows 81 / 51
+//   8 sequences of 16000:  32 rows 84 / 113 us, 48 rows 126 / 114, 64 rows 163 / 116      64 of 4000: 32 rows 177 / 225, 48 rows 254 / 247, 64 rows 330 / 250
+//   1 sequence of 500:     96 rows 13 / 21, 128 rows 14 / 22      of 4000: 96 rows 18 / 25, 128 rows 20 / 24      of 32000: 64 rows 49 / 48, 96 rows 61 / 49, 128 rows 86 / 49
 // so with few sequences and heads, whose contexts hardly fill the machine, the border lies higher.
 inline uint32_t split_rows(uint32_t seqs, uint32_t Hkv) { return (uint64_t)seqs * Hkv <= 16u ? 96u : 48u; }
 
@@ -32,7 +32,7 @@ int run_split(p0p_ctx* c, CacheAttnP& p, uint32_t G) {
   return 0;
 }
 constexpr uint64_t split_scratch(uint64_t G) { return G * 2u * 16u * (512u + 8u); }
-constexpr uint64_t tc_scratch(uint64_t G) { return G * 2u * 256u * (512u + 8u) + G * sizeof(CacheTcDesc); }
+constexpr uint64_t tc_scratch(uint64_t G) { return G * 2u * 256u * (512u + 2u * 8u) + G * sizeof(CacheTcDesc); }
 
 int run_tc(p0p_ctx* c, const CacheAttnP& a, uint32_t G, uint32_t min_rows) {
   static DeviceOnce once;
@@ -52,7 +52,12 @@ int run_tc(p0p_ctx* c, const CacheAttnP& a, uint32_t G, uint32_t min_rows) {
   p.geo = CacheTcGeo{a.c.Hkv, a.group, a.c.seqs, a.window, a.sinks, 128u / a.group, min_rows};
   p.part = reinterpret_cast<float4*>(c->scratch.ptr);
   p.part_ml = reinterpret_cast<float2*>((char*)c->scratch.ptr + (uint64_t)G * 2u * 256u * 512u);
-  p.desc = reinterpret_cast<CacheTcDesc*>((char*)c->scratch.ptr + (uint64_t)G * 2u * 256u * 520u);
+  p.count = c->counters;
+  // Few items are cut into many shares each, which a kernel of its own adds up faster than the block that arrives last with one; where there are none, that launch costs
+  // 2 us.  Measured, within / by a second kernel, 8 kv heads: 1 sequence of 32000 (18 shares an item) 63 / 48 us, of 4000 29 / 24, of 500 (two shares)
+  // 16 / 18; 8 sequences (two or three) of 16000 115 / 113, of 4000 42.5 / 41, of 500 16.7 / 18.8.  With row offsets this counts all sequences and all rows.
+  const bool merge = (uint64_t)a.c.Hkv * std::max<uint64_t>(a.c.seqs, (a.c.M - 1u) / (2u * p.geo.qpt) + 1u) * 4u < G;
+  p.desc = merge ? reinterpret_cast<CacheTcDesc*>((char*)c->scratch.ptr + (uint64_t)G * 2u * 256u * (512u + 2u * 8u)) : nullptr;
   // Q [Hq][ldq][128] as {64 of d, the heads of a group, qpt queries, a kv head}: a tile's rows query by query
   CUtensorMap mq;
   const cuuint64_t dims[4] = {128u, a.group, a.c.M, a.c.Hkv}, strides[3] = {(cuuint64_t)a.ldq * 256u, 256u, (cuuint64_t)a.ldq * a.group * 256u};
@@ -61,9 +66,9 @@ int run_tc(p0p_ctx* c, const CacheAttnP& a, uint32_t G, uint32_t min_rows) {
         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return fail(c, -12, "cacheAttention: a tensor map could not be encoded");
   cudaError_t e = launch_chained(k_cache_attn_tc, dim3(G), dim3(CTC_THREADS), CTC_SMEM, c->stream, p, mq);
-  if (e == cudaSuccess) e = launch_chained(k_cache_merge, dim3(G, 8u), dim3(256), 0, c->stream, CacheMergeP{p.part, p.part_ml, p.desc, p.O, p.ldo, a.group, p.geo.qpt});
+  if (e == cudaSuccess && merge) e = launch_chained(k_cache_merge, dim3(G, 8u), dim3(256), 0, c->stream, CacheMergeP{p.part, p.part_ml, p.desc, p.O, p.ldo, a.group, p.geo.qpt});
   if (e != cudaSuccess) return cuda_fail(c, e, "cacheAttention launch");
-  c->launches += 2;
+  c->launches += merge ? 2 : 1;
   return 0;
 }
 

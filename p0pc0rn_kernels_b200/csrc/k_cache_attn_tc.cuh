@@ -8,11 +8,11 @@
 //   scales  a thread's 64 scores belong to one page: its K scale joins the softmax scale, its V scale the exponent (w = 2^(score + log2 vs - m),
 //           and the sum of the weights is weighted with 1 / vs), as in k_cache_attn.cuh
 //   work    the pairs of visible pages of all items (block of queries, kv head) in one row are dealt out evenly to one block per SM, from the
-//           numbers on the device; an item that crosses blocks leaves partial results that k_cache_merge adds up, in order
+//           numbers on the device; the shares of an item that crosses blocks are added up by the warp that arrives last with one
 // Roles: warp 0 keeps the list of work (items, and page by page what the others need to know), warp 1 multiplies, warp 2 loads queries, warps 4-7 convert,
 // warps 8-15 and 16-23 are the softmax of the two tiles, two threads per row.  The softmax threads take the registers that the others leave
 // (setmaxnreg; per scheduler 4 x 104 + 24 + 40 = the 6 x 80 of the launch; with 32 for each of the others the converting warps spilled: 249 against 246.5 us).
-// Bound: 2000 tokens over 6100 of 32:8 heads, 233 GFLOP: 247 us = 940 TFLOP/s, 0.57 of the measured burst, under the power limit (1.6 to 1.7 GHz).  A pair of
+// Bound: 2000 tokens over 6100 of 32:8 heads, 233 GFLOP: 232 us = 1000 TFLOP/s, 0.61 of the measured burst, under the power limit (1.6 to 1.7 GHz).  A pair of
 // pages takes about 4200 cycles of a block: its multiplies alone 1900 (tensor pipe active 54 %), its traffic through shared memory 2500 (operands, codes
 // in, tiles out), the converting warps about 3500 (latency: a warp's 16 units of 32 bytes, waits and fences in a row), a softmax warp 1700.  Tried and slower: conversion
 // by the softmax warps between two tiles (308 us), K as fp16 subnormals with a row sum of q (255 against 260 then, but 147 against 141 for short
@@ -27,7 +27,7 @@
 
 namespace p0p {
 
-struct CacheTcDesc { uint32_t on, row0, q, hk, c1; };      // an item that begins in this block and goes on: its first row, its queries, its last block
+struct CacheTcDesc { uint32_t on, row0, q, hk, c1; };      // an item of more than two shares that begins in this block: its first row, its queries, its last block
 struct CacheTcP {
   CacheP c;
   __half* O;
@@ -35,8 +35,9 @@ struct CacheTcP {
   CacheTcGeo geo;
   float scale_log2;
   float4* part;          // [block][2][32 groups of 4 columns][256 rows] unnormalised O
-  float2* part_ml;       // [block][2][256 rows] (maximum, sum)
-  CacheTcDesc* desc;     // [block]
+  float2* part_ml;       // [block][2][2 halves][256 rows] (maximum, sum)
+  uint32_t* count;       // [block][16 warps] arrivals, zero between calls
+  CacheTcDesc* desc;     // [block]; NULL: items of more than two shares are added up here as well
 };
 
 // Four slots of tiles: with three the K tile two pairs ahead takes the V tile's place, and its conversion waits for that product.  What is left of
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
   unsigned char* gbase = ctc_raw;
   if (base & 1023u) {
     grid_dependency_wait();
-    if (threadIdx.x == 0u) { p.desc[blockIdx.x].on = 0u; cache_tell(p.c.status, 633); }
+    if (threadIdx.x == 0u) { if (p.desc) p.desc[blockIdx.x].on = 0u; cache_tell(p.c.status, 633); }
     return;
   }
   const uint32_t q_sm = base, kv_sm = base + 2u * ATC_TILE, st_sm = kv_sm + CTC_SLOTS * ATC_TILE, bars = st_sm + 8u * CTC_STAGE;
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
       if (lane == 0u) {
         at[4] = (uint32_t)(u1 - u0);
         at[6] = (uint32_t)U; at[7] = (uint32_t)(U >> 32); at[8] = (uint32_t)G; at[9] = (uint32_t)u0; at[10] = (uint32_t)(u0 >> 32);
-        p.desc[blockIdx.x].on = 0u;
+        if (p.desc) p.desc[blockIdx.x].on = 0u;
       }
       if (u1 > u0) {
         uint64_t r = u0;                                                  // cost before ours, from here on within a sequence, then a block of queries
@@ -491,24 +492,91 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
       items++;
       tc_fence_after();
       const uint32_t q = t * p.geo.qpt + qi, gt = g.t;                    // the row's query within the block
-      const bool live = qi < p.geo.qpt && q < g.n, whole = gt == 0u && cnt == g.units;
-      const uint32_t slot = gt > 0u ? 0u : 1u;
-      const float inv = l > 0.0f ? 1.0f / l : l;
-      const int64_t at_o = live && ok ? (int64_t)(g.r0 + q) * p.ldo + (g.hk * p.geo.group + hh) * 128u + half * 64u : -1;      // the row's half columns in O; -1: not stored
-      const bool vec = ((reinterpret_cast<uintptr_t>(p.O) | ((uintptr_t)p.ldo * 2u)) & 15u) == 0u;
-#pragma unroll 1
-      for (uint32_t c = 0; c < 2u; c++) {                                 // 32 columns at a time
-        uint32_t o[32];
+      const bool live = qi < p.geo.qpt && q < g.n, whole = gt == 0u && cnt == g.units, fine = __all_sync(0xffffffffu, ok);
+      const int64_t at_o = live && fine ? (int64_t)(g.r0 + q) * p.ldo + (g.hk * p.geo.group + hh) * 128u + half * 64u : -1;      // the row's half columns in O; -1: not stored
+      auto tmem_o = [&](uint32_t c, uint32_t (&o)[32]) {                  // 32 columns
         tmem_ld16(o_addr + 32u * c, *reinterpret_cast<uint32_t(*)[16]>(&o[0]));
         tmem_ld16(o_addr + 32u * c + 16u, *reinterpret_cast<uint32_t(*)[16]>(&o[16]));
         tmem_ld_wait();
-        if (!whole) {
-          float4* pt = p.part + ((size_t)(blockIdx.x * 2u + slot) * 32u + half * 16u + 8u * c) * 256u + t * 128u + row;
-          if (at_o >= 0) {
+      };
+      // An item that crosses blocks: each of them leaves (maximum, sum, O) in memory, and the warp that arrives last (of those that have these rows and columns, one in
+      // each block) adds them up.  A block has two places: 0 for the item that began before it, 1 for the one that goes on behind it.  Mostly there are two shares, and the
+      // first block's, at its end, finds the second's, which that block began with: its own then stays in tensor memory.  Sums of two do not depend on
+      // which is whose (both products are rounded); more are all read back and added in block order, or left to k_cache_merge (p.desc).
+      bool last = false, two = false;
+      uint32_t c0 = blockIdx.x, c1 = c0;
+      float m_all = m_used, f = 1.0f, f_other = 0.0f;
+      auto part_at = [&](uint32_t b, uint32_t c) { return p.part + ((size_t)(b * 2u + (b == c0 ? 1u : 0u)) * 32u + half * 16u + 8u * c) * 256u + t * 128u + row; };
+      auto ml_at = [&](uint32_t b) { return p.part_ml + ((size_t)(b * 2u + (b == c0 ? 1u : 0u)) * 2u + half) * 256u + t * 128u + row; };
+      if (!whole && fine) {
+        const uint64_t U = (uint64_t)at[6] | (uint64_t)at[7] << 32, u0 = (uint64_t)at[9] | (uint64_t)at[10] << 32, first = u0 + g.spent - gt;      // (the item's unit 0)
+        const uint32_t owner = (uint32_t)deal_owner(lane & 1u ? first + g.units - 1u : first, U, at[8]);
+        c0 = __shfl_sync(0xffffffffu, owner, 0); c1 = __shfl_sync(0xffffffffu, owner, 1);
+        two = c1 == c0 + 1u;
+        uint32_t* const arrivals = p.count + c0 * 16u + (warp - 8u);
+        uint32_t before = 0u;
+        if (two && lane == 0u) asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(before) : "l"(arrivals) : "memory");
+        last = __shfl_sync(0xffffffffu, before, 0) == 1u;
+        const bool later = !two && p.desc;
+        if (!last) {
+          *ml_at(blockIdx.x) = make_float2(m_used, l);
+#pragma unroll 1
+          for (uint32_t c = 0; c < 2u; c++) {
+            uint32_t o[32];
+            tmem_o(c, o);
+            float4* pt = part_at(blockIdx.x, c);
+            if (at_o >= 0) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) pt[e * 256] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+              for (int e = 0; e < 8; e++) pt[e * 256] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+            }
           }
-          continue;
+          __syncwarp();
+          if (later) {
+            if (blockIdx.x == c0 && t == 0u && half == 0u && row == 0u) p.desc[c0] = CacheTcDesc{1u, g.r0, g.n, g.hk, c1};
+          } else {
+            if (lane == 0u) asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(arrivals) : "memory");
+            last = __shfl_sync(0xffffffffu, before, 0) == c1 - c0;
+          }
+        }
+        __syncwarp();
+        if (last) {
+          if (lane == 0u) *arrivals = 0u;
+          if (two) {
+            const float2 z = __ldcg(ml_at(blockIdx.x == c0 ? c1 : c0));
+            m_all = fmaxf(m_used, z.x);
+            f = m_used == -INFINITY ? 0.0f : atc_ex2(m_used - m_all);
+            f_other = z.x == -INFINITY ? 0.0f : atc_ex2(z.x - m_all);
+            l = __fadd_rn(__fmul_rn(f, l), __fmul_rn(f_other, z.y));
+          } else {
+            for (uint32_t b = c0; b <= c1; b++) m_all = fmaxf(m_all, __ldcg(ml_at(b)).x);
+            l = 0.0f; f = 0.0f;
+            for (uint32_t b = c0; b <= c1; b++) { const float2 z = __ldcg(ml_at(b)); l = fmaf(z.x == -INFINITY ? 0.0f : atc_ex2(z.x - m_all), z.y, l); }
+          }
+        }
+      }
+      const float inv = l > 0.0f ? 1.0f / l : l;
+      const bool vec = ((reinterpret_cast<uintptr_t>(p.O) | ((uintptr_t)p.ldo * 2u)) & 15u) == 0u;
+#pragma unroll 1
+      for (uint32_t c = 0; c < 2u && (whole || last); c++) {              // 32 columns at a time
+        uint32_t o[32];
+        tmem_o(c, o);
+        if (last) {
+#pragma unroll
+          for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__fmul_rn(f, __uint_as_float(o[e])));
+          for (uint32_t b = c0; b <= c1; b++) {
+            if (two && b == blockIdx.x) continue;
+            float w = f_other;
+            if (!two) { const float zx = __ldcg(ml_at(b)).x; w = zx == -INFINITY ? 0.0f : atc_ex2(zx - m_all); }
+            const float4* pt = part_at(b, c);
+            if (at_o >= 0) {
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const float4 x = __ldcg(pt + e * 256);
+                o[4 * e] = __float_as_uint(__fadd_rn(__uint_as_float(o[4 * e]), __fmul_rn(w, x.x))); o[4 * e + 1] = __float_as_uint(__fadd_rn(__uint_as_float(o[4 * e + 1]), __fmul_rn(w, x.y)));
+                o[4 * e + 2] = __float_as_uint(__fadd_rn(__uint_as_float(o[4 * e + 2]), __fmul_rn(w, x.z))); o[4 * e + 3] = __float_as_uint(__fadd_rn(__uint_as_float(o[4 * e + 3]), __fmul_rn(w, x.w)));
+              }
+            }
+          }
         }
         uint32_t v[4][4];                                                 // four pieces of 8 columns
 #pragma unroll
@@ -545,14 +613,6 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
         }
       }
       tc_fence_before();                     // (the reads of O end before the next item's weights are handed over)
-      if (!whole) {
-        if (half == 0u) p.part_ml[(size_t)(blockIdx.x * 2u + slot) * 256u + t * 128u + row] = make_float2(m_used, l);
-        if (slot == 1u && t == 0u && half == 0u && row == 0u) {
-          const uint64_t U = (uint64_t)at[6] | (uint64_t)at[7] << 32;
-          const uint64_t u0 = (uint64_t)at[9] | (uint64_t)at[10] << 32;
-          p.desc[blockIdx.x] = CacheTcDesc{1u, g.r0, g.n, g.hk, (uint32_t)deal_owner(u0 + g.spent + g.units - 1u, U, at[8])};
-        }
-      }
       seg_done(seg);
     }
   }
@@ -561,7 +621,8 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
   if (warp == 1u) { tc_fence_after(); tmem_dealloc(tmem_base, 512u); }
 }
 
-// ---- items that cross blocks: (maximum, sum, O) of their blocks added up in block order.  A block takes 32 rows of one item's 256.
+// ---- items of more than two shares: (maximum, sum, O) of their blocks added up in block order.  A block takes 32 rows of one item's 256.  (8 kv heads, 64 rows over
+// 32000 tokens, 18 shares an item: the whole call 49 us; 63 where the block that arrives last reads them all by itself.)
 struct CacheMergeP {
   const float4* part; const float2* part_ml; const CacheTcDesc* desc;
   __half* O;
@@ -578,7 +639,7 @@ __global__ void __launch_bounds__(256) k_cache_merge(const CacheMergeP p) {
   if (__syncthreads_or(live(row)) == 0) return;
   auto slab = [&](uint32_t c) { return (size_t)c * 2u + (c == c0 ? 1u : 0u); };
   float M = -INFINITY;
-  if (live(row)) for (uint32_t c = c0; c <= d.c1; c++) M = fmaxf(M, p.part_ml[slab(c) * 256u + row].x);
+  if (live(row)) for (uint32_t c = c0; c <= d.c1; c++) M = fmaxf(M, p.part_ml[slab(c) * 512u + row].x);
   float L = 0.0f;
   float4 acc[4];
 #pragma unroll
@@ -586,7 +647,7 @@ __global__ void __launch_bounds__(256) k_cache_merge(const CacheMergeP p) {
   if (live(row)) {
 #pragma unroll 2
     for (uint32_t c = c0; c <= d.c1; c++) {
-      const float2 ml = p.part_ml[slab(c) * 256u + row];
+      const float2 ml = p.part_ml[slab(c) * 512u + row];
       const float f = ml.x == -INFINITY ? 0.0f : atc_ex2(ml.x - M);
       L = fmaf(f, ml.y, L);
 #pragma unroll

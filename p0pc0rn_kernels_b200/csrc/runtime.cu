@@ -46,6 +46,9 @@ int p0p_open(int device, const p0p_opts* opts, p0p_ctx** out) {
 static int check_kernel_status(p0p_ctx* c) {
   if (c->host_status && *c->host_status) {
     int code = *c->host_status; *c->host_status = 0;
+    // blocks that gave up may not have arrived where the last arrival resets a counter (the first code stands: another one may hide that)
+    const cudaError_t e = cudaMemsetAsync(c->counters, 0, c->n_counters * sizeof(uint32_t), c->stream);
+    if (e != cudaSuccess) return cuda_fail(c, e, "arrival counters");
     if (code == CACHE_BAD_ROWS) return fail(c, -10, "cache: row offsets that fall, or exceed M; the sequence was left out");
     if (code == CACHE_BAD_LENS) return fail(c, -10, "cache: a sequence has fewer tokens than rows, or more than its table holds; it was left out");
     if (code == CACHE_BAD_PAGE) return fail(c, -10, "cache: a page number of the table is outside the cache; results of the queued work are invalid");

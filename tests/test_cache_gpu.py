@@ -362,6 +362,20 @@ def test_attention_scales_of_any_size(gpu, scale, kernel):
         cache.free()
 
 
+@pytest.mark.parametrize("window", [0, 9000])
+def test_attention_long_items_among_many(gpu, window):
+    """a long context among many short items: its items lie over many blocks, which add them up without another kernel; the same again, bit for bit"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 8, 3, 320)
+    cache.fill([400, 20000, 37])
+    try:
+        for _ in range(2): _check(cache, [310, 12, 20], 16, window=window, kernel="tmem")
+        got = [_attend(cache, [310, 12, 20], 16, window=window, kernel="tmem")[0].view(np.uint16) for _ in range(3)]
+        assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+    finally:
+        cache.free()
+
+
 @pytest.mark.parametrize("kernel", ["split", "tmem"])
 def test_pages_behind_the_window_can_be_given_away(gpu, kernel):
     """the table's entries of pages that no query sees, and that hold no sink, are not followed: they name no page here"""
