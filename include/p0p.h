@@ -268,7 +268,8 @@ typedef struct p0p_cache_attn_args {
 } p0p_cache_attn_args;
 /* causal attention of the call's queries over the cache, which holds their own keys and values already (p0p_cache_write comes first).
  * Query head h reads kv head h / (Hq / Hkv).  Partial results are kept in the context's scratch memory.  o may overlap neither q nor the cache.
- * Arithmetic: scores and sums in fp32; a weight of the softmax, times its block's V scale, is rounded to fp16 relative to the largest such product of its row. */
+ * Arithmetic: scores and sums in fp32 (a score's error is 2^-22 or so of the largest product that it sums: scores beyond 2^20 are told apart only so far);
+ * a weight of the softmax, times its block's V scale, is rounded to fp16 relative to the largest such product of its row. */
 int p0p_cache_attention(p0p_ctx* ctx, const p0p_cache_attn_args* args);
 
 /* rotary positions: y = x with the first `rot` elements of every head turned by its token's position (y may be x, but not overlap it

@@ -69,6 +69,9 @@ P0P_HD uint32_t cache_vis_page(const CacheVis& v, uint32_t t) { return t < v.sp 
 P0P_HD bool cache_key_visible(uint32_t key, uint32_t p, uint32_t window, uint32_t sinks) {
   return key <= p && (window == 0u || p - key < window || key < sinks);
 }
+// Scores are fp32, and a weight's exponent is score * factor - maximum in one multiply-add.  Where the maximum (in powers of two) is larger than this, the
+// rounding of that reference would show in the weights (2^-15 here; at 2^28 it is 16, and weights overflow): the page's largest score is taken off first.
+P0P_HD bool cache_far(float m) { return m > 1024.0f || (m < -1024.0f && m > -3.0e38f); }      // (-infinity: no key yet)
 // may a page's key be hidden from a query at positions p0 .. p1?
 P0P_HD bool cache_page_masked(uint32_t page, uint32_t p0, uint32_t p1, uint32_t window, uint32_t sinks) {
   const uint32_t k0 = page * CACHE_PAGE, k1 = k0 + (CACHE_PAGE - 1u);

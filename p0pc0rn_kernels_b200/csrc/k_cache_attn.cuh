@@ -138,6 +138,7 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
     auto wait = [&](uint32_t buf) { ok = __all_sync(0xffffffffu, mbar_wait(bars + 8u * buf, (ph >> buf) & 1u, p.c.status, 611 + (int)buf)); ph ^= 1u << buf; return ok; };
     uint32_t qa[8][4], pa[4][4], pos[2];
     float bias[2], o[16][4], m[2], l[2], s[8][4], zp[4];
+    bool far = false;                                                      // the item's maximum is large
     // scores (scaled, log2) -> weights pa, their sums zp; the running maximum rises only when it grew by more than 2^8 (weights are at most 256 then)
     auto weigh = [&](uint32_t page, uint32_t p0, uint32_t p1, float f, float lv, float inv_v) {
       float mx[2] = {-INFINITY, -INFINITY};
@@ -155,16 +156,26 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1)); mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-        mx[h] = fmaf(mx[h], f, lv);
       }
-      if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.0f || mx[1] > m[1] + 8.0f)) {
+      const float raw[2] = {mx[0], mx[1]};
+#pragma unroll
+      for (int h = 0; h < 2; h++) mx[h] = fmaf(raw[h], f, lv);
+      // (the difference, not m + 8: where m is large that sum may be m, or 16 more.  Against a maximum of -infinity it is infinity, or no number where the page shows nothing either)
+      if (__any_sync(0xffffffffu, mx[0] - m[0] > 8.0f || mx[1] - m[1] > 8.0f)) {
         const float n0 = fmaxf(m[0], mx[0]), n1 = fmaxf(m[1], mx[1]);
         const float a0 = n0 == -INFINITY ? 1.0f : at_ex2(m[0] - n0), a1 = n1 == -INFINITY ? 1.0f : at_ex2(m[1] - n1);
         m[0] = n0; m[1] = n1; l[0] *= a0; l[1] *= a1;
 #pragma unroll
         for (int d = 0; d < 16; d++) { o[d][0] *= a0; o[d][1] *= a0; o[d][2] *= a1; o[d][3] *= a1; }
+        far = __any_sync(0xffffffffu, cache_far(n0) || cache_far(n1));
       }
-      const float e0 = m[0] == -INFINITY ? 0.0f : lv - m[0], e1 = m[1] == -INFINITY ? 0.0f : lv - m[1];      // (a row that has seen no key yet: all its weights are 0)
+      float e0 = m[0] == -INFINITY ? 0.0f : lv - m[0], e1 = m[1] == -INFINITY ? 0.0f : lv - m[1];      // (a row that has seen no key yet: all its weights are 0)
+      if (far) {                                                           // large scores: see cache_far
+        const float r0 = raw[0] == -INFINITY ? 0.0f : raw[0], r1 = raw[1] == -INFINITY ? 0.0f : raw[1];
+        e0 = raw[0] == -INFINITY ? 0.0f : mx[0] - m[0]; e1 = raw[1] == -INFINITY ? 0.0f : mx[1] - m[1];      // (at most 8)
+#pragma unroll
+        for (uint32_t n = 0; n < 8u; n++) { s[n][0] -= r0; s[n][1] -= r0; s[n][2] -= r1; s[n][3] -= r1; }
+      }
       zp[0] = zp[1] = zp[2] = zp[3] = 0.0f;
       float2 z0 = make_float2(0.0f, 0.0f), z1 = z0;
 #pragma unroll
@@ -232,7 +243,7 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
       }
 #pragma unroll
       for (int d = 0; d < 16; d++) { o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.0f; }
-      m[0] = m[1] = -INFINITY; l[0] = l[1] = 0.0f;
+      m[0] = m[1] = -INFINITY; l[0] = l[1] = 0.0f; far = false;
       for (uint32_t i = 0; i < codes && ok; i++) {
         const uint32_t at = i & 31u;
         if (at == 0u) {                                                    // 32 pages at a time: the next ones' numbers are asked for here, their scales half way

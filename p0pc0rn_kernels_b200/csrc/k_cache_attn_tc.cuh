@@ -404,6 +404,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
       if (t == 1u && g.n <= p.geo.qpt) { pair += cnt; seg_done(seg); continue; }
       const uint32_t pos = g.L - g.n + min(t * p.geo.qpt + qi, g.n - 1u);
       float m_used = -INFINITY, l = 0.0f;
+      bool far = false;                                                   // the maximum is large
       for (uint32_t j = 0; j < cnt; j++, n++, pair++) {
         // (a wait that ran out: the thread goes on without it, so that its partner is not left at the barrier; the status word is set)
         if (ok && !mbar_wait(s_full + 8u * t, n & 1u, p.c.status, 630)) ok = false;
@@ -442,7 +443,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
         bar_sync_named((int)pair_bar, 64);
         tc_fence_after();
         mts = fmaxf(mts, *other);
-        if (__any_sync(0xffffffffu, mts > m_used + 8.0f || (m_used == -INFINITY && mts > -INFINITY))) {
+        if (__any_sync(0xffffffffu, mts - m_used > 8.0f)) {      // (the difference: where the maximum is large, 8 more of it may be none, or 16)
           const float m_new = fmaxf(m_used, mts);
           const float alpha = m_new == -INFINITY ? 1.0f : atc_ex2(m_used - m_new);
           l *= alpha;
@@ -458,9 +459,19 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
             }
           }
           m_used = m_new;
+          far = __any_sync(0xffffffffu, qi < p.geo.qpt && cache_far(m_new));      // (rows behind the last query's hold anything)
         }
         float2 ls[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-        const float nm = m_used == -INFINITY ? 0.0f : lv - m_used;       // (a row that has seen no key yet: all its weights are 0)
+        float nm = m_used == -INFINITY ? 0.0f : lv - m_used;             // (a row that has seen no key yet: all its weights are 0)
+        if (far) {                                                        // large scores: see cache_far
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 64; c++) top = fmaxf(top, __uint_as_float(s[c]));
+          nm = top == -INFINITY ? 0.0f : *mine - m_used;                  // (this page's largest, as above; at most 8)
+          if (top == -INFINITY) top = 0.0f;
+#pragma unroll
+          for (int c = 0; c < 64; c++) s[c] = __float_as_uint(__uint_as_float(s[c]) - top);
+        }
         const float2 sc2 = make_float2(sc, sc), nm2 = make_float2(nm, nm);
 #pragma unroll
         for (int c = 0; c < 2; c++) {

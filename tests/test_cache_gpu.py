@@ -704,3 +704,60 @@ def test_numbers_on_the_device_that_make_no_sense(gpu):
     finally:
         for x in (b, r): gpu.free(x)
         cache.free()
+
+
+# ------------------------------------------------------------------------------------------------------------- errors against the result's own size
+def _check_rms(cache, news, group, window=0, sinks=0, scale=None, without=None, **kw):
+    """The error's root mean square, per sequence and query head, against the wanted result's.  Each weight is off by at most d = 2^-11 + 1e-4, independently
+    of the others (rounding), so that the weighted mean of values that vary around it is off by d of that mean's own spread, at most of its size; the result's
+    rounding adds 2^-11 (2^-25 where it is subnormal): sqrt(d^2 + 2^-22) = 7.6e-4 of the result.  The limit is 1e-3 of it, where one page in a
+    thousand left out, taken twice or given another's scale moves it by more.  `without`: pages (sequence, page) of which that is checked, on the wanted result."""
+    out, q, offs = _attend(cache, news, group, window, sinks, scale, **kw)
+    for b in range(cache.seqs):
+        if not news[b]: continue
+        K, V = cache.held(b)
+        want = _attn_want(q[b], K, V, window, sinks, scale)
+        err = out[offs[b]:offs[b + 1]].astype(np.float64) - want
+        limit = 1e-3 * np.sqrt((want ** 2).mean((0, 2))) + 2.0 ** -25
+        got = np.sqrt((err ** 2).mean((0, 2)))
+        assert (got <= limit).all(), (b, (got / limit).max(), int((got / limit).argmax()))
+        for at, pg in without or ():
+            if at != b: continue
+            keep = np.arange(K.shape[1]) // PAGE != pg
+            less = _attn_want(q[b][:, -1:], K[:, keep], V[:, keep], 0, 0, scale)                 # (the newest query alone: it sees them all)
+            assert (np.sqrt(((less - want[-1:]) ** 2).mean((0, 2))) > limit).all(), (b, pg)
+
+
+@pytest.mark.parametrize("kernel", ["split", "tmem"])
+@pytest.mark.parametrize("scale", [2.0 ** 16, 2.0 ** 22, 2.0 ** 24, 2.0 ** 27, 2.0 ** 31, 2.0 ** 64])
+def test_attention_large_scores(gpu, scale, kernel):
+    """scores of any size that fp32 holds: the value of the largest one (they are far apart: nothing else has weight), never more than that"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 2, 1, 5)
+    rng = np.random.default_rng(7)
+    k = np.zeros((2, 300, 128)); k[:, :, 0] = rng.permutation(300) - 150.0
+    v = rng.normal(0, 1, (2, 300, 128))
+    try:
+        cache.write([300], [k.astype(np.float16)], [v.astype(np.float16)], rows=False)
+        for n in (3, 90):
+            _check_rms(cache, [n], 2, scale=scale, kernel=kernel)
+            _check_rms(cache, [n], 2, window=90, sinks=3, scale=scale, kernel=kernel)
+    finally:
+        cache.free()
+
+
+@pytest.mark.parametrize("kernel", ["split", "tmem"])
+def test_attention_large_scores_from_large_values(gpu, kernel):
+    """the same with the usual scale, from queries and keys of the largest values, positive and negative: products up to 10^11"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 1, 1, 4)
+    rng = np.random.default_rng(7)
+    k = np.repeat(rng.permutation(200)[None, :, None] * 600.0 - 60000.0, 128, 2)
+    v = rng.normal(0, 1, (1, 200, 128))
+    try:
+        cache.write([200], [k.astype(np.float16)], [v.astype(np.float16)], rows=False)
+        for std in (100.0, 10000.0):
+            _check_rms(cache, [3], 2, qstd=std, kernel=kernel)
+            _check_rms(cache, [70], 2, qstd=std, kernel=kernel)
+    finally:
+        cache.free()
