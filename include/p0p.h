@@ -226,9 +226,9 @@ int p0p_attention(p0p_ctx* ctx, const p0p_attn_args* args, double* flops);
  *   tail   [seqs][Hkv][2][64 * 128] fp16: the tokens of each sequence's last, unfinished page, unquantised
  *   table  [seqs][max_pages] u32: the page that holds tokens 64 i .. 64 i + 63        lens [seqs] u32: tokens of each sequence
  * A block of 64 tokens of one head is quantised once, when its last token arrives: scale = (largest magnitude) / 127 rounded up to 12
- * significant bits (1 for a block of zeros), code = x / scale rounded to the nearest, ties to even.  So what the cache holds does not depend on
- * how the tokens were cut into calls.  NaN is stored as 0, an infinity as the largest fp16 of its sign.  Within a block the elements lie as
- * csrc/cache_plan.h says (cache_k_off, cache_v_off), the same for codes and tail.  K and V pages may be shared between sequences
+ * significant bits (for a block of zeros that of the smallest magnitude, 2^-24), code = x / scale rounded to the nearest, ties to even.  So what
+ * the cache holds does not depend on how the tokens were cut into calls.  NaN is stored as 0, an infinity as the largest fp16 of its sign.  Within a
+ * block the elements lie as csrc/cache_plan.h says (cache_k_off, cache_v_off), the same for codes and tail.  K and V pages may be shared between sequences
  * (a common prefix) as long as only one of them writes.
  * `lens`, `table` and `rows` are read on the device when the call runs: a recorded sequence of calls can be replayed with new
  * contents.  `lens` counts the tokens of the present call too: a sequence's n new tokens are its last n, at positions

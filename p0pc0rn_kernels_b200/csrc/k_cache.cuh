@@ -98,9 +98,8 @@ __device__ __forceinline__ uint32_t cache_code(float x, float inv) { return __fl
 __device__ __forceinline__ uint32_t cache_pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-__device__ __forceinline__ float cache_scale(float amax) {
-  return amax > 0.0f ? __uint_as_float((__float_as_uint(__fdiv_rn(amax, 127.0f)) + 4095u) & ~4095u) : 1.0f;
-}
+// A block of zeros gets the smallest scale that any block has: attention weighs a block's values by it, and zeros are to weigh less than any others.
+__device__ __forceinline__ float cache_scale(float amax) { return __uint_as_float((__float_as_uint(__fdiv_rn(fmaxf(amax, 0x1p-24f), 127.0f)) + 4095u) & ~4095u); }
 
 // One block = one touched page of one kv head; 128 threads for K, 128 for V, each half by itself.  A page that the call finishes: its tokens (old ones from
 // the tail, new ones from the rows) are read with their largest magnitude found on the way; K's codes leave from the registers, 8 per thread and store, V's

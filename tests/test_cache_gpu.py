@@ -761,3 +761,21 @@ def test_attention_large_scores_from_large_values(gpu, kernel):
             _check_rms(cache, [70], 2, qstd=std, kernel=kernel)
     finally:
         cache.free()
+
+
+@pytest.mark.parametrize("kernel", ["split", "tmem"])
+@pytest.mark.parametrize("size", [0, 8, 10, 12, 14])
+def test_attention_beside_a_page_of_zeros(gpu, size, kernel):
+    """a page of zero values costs the other pages' weights nothing, however small their values are (its keys are zero as well in the second head)"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 2, 1, 6)
+    rng = np.random.default_rng(size)
+    k = rng.normal(0, 1, (2, 320, 128)); v = rng.normal(0, 2.0 ** -size, (2, 320, 128))
+    v[:, :64] = 0; v[:, 192:256] = 0; k[1, :64] = 0
+    try:
+        cache.write([320], [k.astype(np.float16)], [v.astype(np.float16)], rows=False)
+        scales = gpu.read(cache.d["scales"]["buf"]).view(np.float32)[:cache.pages * 4].reshape(cache.pages, 2, 2)
+        assert (scales[cache.table[0, 0], :, 1] == _quantise(np.full((64, 128), 2.0 ** -24))[1]).all() and scales[cache.table[0, 0], 1, 0] == scales[cache.table[0, 3], 0, 1]
+        for n in (2, 60): _check_rms(cache, [n], 4, kernel=kernel)
+    finally:
+        cache.free()
