@@ -45,11 +45,13 @@ struct CacheTcP {
 // warp loading for all four, or a lane for each of the eight, came late: 4000 cycles from the last read to the next codes).
 constexpr uint32_t CTC_THREADS = 768u, CTC_SLOTS = 4u, CTC_STAGE = CACHE_BLOCK / 2u;
 constexpr int CTC_REGS = 16 * 104 + 4 * 24 + 4 * 40;      // registers per lane of all warps, after setmaxnreg
+constexpr float CTC_TAIL = 15.0f;      // log2 of the tail's largest weight
 constexpr uint32_t CTC_PAIRS = 4u;     // pairs of pages that are described ahead
 constexpr uint32_t CTC_SEGS = 4u;      // items that are announced ahead
 // an item's share
 struct CtcSeg { uint32_t cnt, t, units, r0, n, L, hk, spent; };
-// a page of a pair.  For the softmax: scale_log2 * K scale, log2 and reciprocal of the V scale, its first key | 1 where some key is hidden from some row.
+// a page of a pair.  For the softmax: scale_log2 * K scale, log2 and reciprocal of the V scale, its first key | 1 where some key is hidden from some row | 2 in a
+// pair that holds the tail | 4 for the tail.
 // For the conversion: what it is (codes 0, the tail 1 | its tokens << 8, nothing 2, the end of the work 3), and which block of codes or of the tail.
 struct CtcPage { float f, lv, inv_v; uint32_t key0, is, block, pad[2]; };
 constexpr uint32_t CTC_SMEM = (2u + CTC_SLOTS) * ATC_TILE + 8u * CTC_STAGE + 512u + 2048u + CTC_PAIRS * 2u * (uint32_t)sizeof(CtcPage) + CTC_SEGS * (uint32_t)sizeof(CtcSeg) + 64u;
@@ -196,12 +198,14 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
           mbar_arrive(seg_full + 8u * (seg % CTC_SEGS));
         }
         __syncwarp();
-        CtcPage pg{1.0f, 0.0f, 1.0f, 0xffffffffu, 2u, 0u, {0u, 0u}};
+        CtcPage pg{1.0f, 0.0f, 1.0f, 0u, 2u, 0u, {0u, 0u}};
         for (uint32_t j = 0; j < max(w.cnt, 1u) && ok; j++, pair++) {
           const uint32_t l0 = (2u * j) & 31u;
           if (l0 == 0u) {
             const uint32_t k = 2u * (w.t + j) + lane, page = cache_vis_page(w.v, k);
-            pg = CtcPage{1.0f, 0.0f, 1.0f, 0xffffffffu, w.cnt ? 2u : 3u, 0u, {0u, 0u}};      // no page: every key hidden
+            // (both pages of the tail's pair are marked, as masked too: their rows' threads agree on the maximum)
+            const uint32_t marks = (k | 1u) >= w.v.np - 1u && cache_vis_page(w.v, w.v.np - 1u) == w.s.L / CACHE_PAGE ? 3u : 0u;
+            pg = CtcPage{1.0f, 0.0f, 1.0f, 0u - CACHE_PAGE | marks | 1u, w.cnt ? 2u : 3u, 0u, {0u, 0u}};      // no page: every key hidden
             if (w.cnt && k < w.v.np) {
               float2 sc = make_float2(1.0f, 1.0f);
               if (page < w.s.L / CACHE_PAGE) {
@@ -214,7 +218,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
               }
               pg.f = p.scale_log2 * sc.x; pg.inv_v = __fdividef(1.0f, sc.y);
               asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(pg.lv) : "f"(sc.y));
-              pg.key0 = page * CACHE_PAGE | (cache_page_masked(page, w.part.L - w.part.n, w.part.L - 1u, p.geo.window, p.geo.sinks) ? 1u : 0u);
+              pg.key0 = page * CACHE_PAGE | marks | (pg.is & 1u) << 2 | (cache_page_masked(page, w.part.L - w.part.n, w.part.L - 1u, p.geo.window, p.geo.sinks) ? 1u : 0u);
             }
           }
           if (pair >= CTC_PAIRS) ok = __all_sync(0xffffffffu, mbar_wait(pair_empty + 8u * (pair % CTC_PAIRS), (pair / CTC_PAIRS - 1u) & 1u, p.c.status, 622, 20u));
@@ -416,9 +420,15 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
         const float sc = pg.x, lv = pg.y;
         const uint32_t key0 = __float_as_uint(pg.w);
         tmem_ld_wait();
+        // A page's values are at most 127 times its V scale, the tail's are as they are (scale 1): relative to the tail's largest weight, the weights of the page beside it
+        // would be fp16 subnormals where values are small.  So the tail's weights are up to 2^15 (CTC_TAIL), the others below 1 then: its scores count that much
+        // less for the maximum, which is exact in its pair (no page comes after it).
+        float slack = 8.0f, less = 0.0f;
         if (key0 & 1u) {
           // columns whose key is visible: at most hi, and at least lo or below sk (all relative to the page)
-          const uint32_t k0 = key0 & ~1u;
+          const uint32_t k0 = key0 & ~(CACHE_PAGE - 1u);
+          if (key0 & 2u) slack = 0.0f;
+          if (key0 & 4u) less = CTC_TAIL;
           const int hi = (int)min(pos - min(pos, k0), 64u) - (pos < k0 ? 1 : 0);
           int lo = 0, sk = 0;
           if (p.geo.window && pos >= p.geo.window) {
@@ -437,13 +447,13 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
 #pragma unroll
           for (int e = 0; e < 4; e++) mx[e] = fmaxf(fmaxf(mx[e], __uint_as_float(s[c + 2 * e])), __uint_as_float(s[c + 2 * e + 1]));      // (one instruction: the maximum of three)
         }
-        float mts = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sc, lv);
+        float mts = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), sc, lv - less);
         *mine = mts;                         // (the partner has read the last one: these scores are there because it handed over the weights before them)
         tc_fence_before();                   // this warp's reads of S end before its partner writes P over columns 32..63 of them
         bar_sync_named((int)pair_bar, 64);
         tc_fence_after();
         mts = fmaxf(mts, *other);
-        if (__any_sync(0xffffffffu, mts - m_used > 8.0f)) {      // (the difference: where the maximum is large, 8 more of it may be none, or 16)
+        if (__any_sync(0xffffffffu, mts - m_used > slack)) {      // (the difference: where the maximum is large, 8 more of it may be none, or 16)
           const float m_new = fmaxf(m_used, mts);
           const float alpha = m_new == -INFINITY ? 1.0f : atc_ex2(m_used - m_new);
           l *= alpha;
@@ -467,7 +477,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
           float top = -INFINITY;
 #pragma unroll
           for (int c = 0; c < 64; c++) top = fmaxf(top, __uint_as_float(s[c]));
-          nm = top == -INFINITY ? 0.0f : *mine - m_used;                  // (this page's largest, as above; at most 8)
+          nm = top == -INFINITY ? 0.0f : *mine - m_used + less;           // (this page's largest, as above; at most slack + less)
           if (top == -INFINITY) top = 0.0f;
 #pragma unroll
           for (int c = 0; c < 64; c++) s[c] = __float_as_uint(__uint_as_float(s[c]) - top);

@@ -779,3 +779,20 @@ def test_attention_beside_a_page_of_zeros(gpu, size, kernel):
         for n in (2, 60): _check_rms(cache, [n], 4, kernel=kernel)
     finally:
         cache.free()
+
+
+@pytest.mark.parametrize("kernel", ["split", "tmem"])
+@pytest.mark.parametrize("size", [0, 7, 10, 12, 14, 16])
+def test_attention_beside_a_tail_of_small_values(gpu, size, kernel):
+    """the unfinished page's values are no larger than the others': its weights cost theirs nothing"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 2, 2, 6)
+    rng = np.random.default_rng(size)
+    lens = [101, 4 * 64 + 37]
+    k, v = ([rng.normal(0, s, (2, L, 128)).astype(np.float16) for L in lens] for s in (1.0, 2.0 ** -size))
+    v[1][1, 256:] = 0
+    try:
+        cache.write(lens, k, v)
+        for n in ([1, 2], [40, 70]): _check_rms(cache, n, 4, kernel=kernel)
+    finally:
+        cache.free()
