@@ -133,6 +133,22 @@ struct CacheCursor {
   P0P_HD bool tail(uint32_t k) const { return cache_vis_page(v, k) == s.L / CACHE_PAGE; }      // is visible page k the unfinished one?
 };
 
+// What a block that has units [u0, u1) and gives up still tells the others: tell(x, i0, i1) once for each item whose pages, units [i0, i1), lie in the block only in part
+// (x: where it stands).  That is its first unit's item, its last unit's, or neither; both may be the same one.
+template <class Tell>
+P0P_HD void cache_tell_shares(const CacheGeo& g, const uint64_t* pre, const CacheSeq* seq, uint64_t u0, uint64_t u1, Tell tell) {
+  uint64_t told = ~0ull;
+  for (uint32_t k = 0; k < 2u; k++) {
+    const uint64_t u = k ? u1 - 1u : u0;
+    CacheCursor x;
+    x.seek(g, pre, seq, u);
+    const uint64_t i0 = u - x.at + 1u, i1 = i0 + x.v.np;
+    if (i0 == told || i0 >= u1 || (i0 >= u0 && i1 <= u1)) continue;      // (told already; only the unit before its pages is here; all of it is)
+    told = i0;
+    tell(x, i0, i1);
+  }
+}
+
 // The tensor-memory attention's work: an item = up to 2 * qpt queries of a sequence (qpt: those whose heads of one kv head fill a tile of 128
 // rows) and one kv head, a unit = two visible pages of it.  Per sequence [block of queries][kv head][pair of pages].
 struct CacheTcGeo { uint32_t Hkv, group, seqs, window, sinks, qpt, min_rows; };      // sequences with at most min_rows rows per kv head are the other kernel's

@@ -413,13 +413,10 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
   };
   if (sh.failed) {                                                         // a wait ran out: the arrivals still have to be told, or the counters would not return to zero
     if (warp == 0u)
-      for (uint32_t k = 0; k < 2u; k++) {
-        CacheCursor x;
-        x.seek(geo, sh.pre, sh.seq, k ? u1 - 1u : u0);
-        const uint64_t i0 = (k ? u1 - 1u : u0) - x.at + 1u, i1 = i0 + x.v.np;      // the units of the item's pages
-        if (i0 >= u1 || (i0 >= u0 && i1 <= u1) || (k == 1u && i0 < u0)) continue;  // (nothing of it here; all of it; counted already)
-        for (uint32_t r = 0; r < min(16u, x.s.n * p.group - x.rb * 16u); r++) arrive((uint32_t)deal_owner(i0, U, G), (uint32_t)deal_owner(i1 - 1u, U, G), r);
-      }
+      cache_tell_shares(geo, sh.pre, sh.seq, u0, u1, [&](const CacheCursor& x, uint64_t i0, uint64_t i1) {
+        const uint32_t c0 = (uint32_t)deal_owner(i0, U, G), c1 = (uint32_t)deal_owner(i1 - 1u, U, G), rows = min(16u, x.s.n * p.group - x.rb * 16u);
+        for (uint32_t r = 0; r < rows; r++) arrive(c0, c1, r);
+      });
     return;
   }
   const uint64_t my_i0 = lane < CA_WARPS * 2u && sh.ent[lane].on ? sh.ent[lane].i0 : ~0ull;

@@ -276,3 +276,66 @@ def test_bad_numbers_are_refused_before_the_call():
         P.rope(Gpu(), {"x": {}, "H": 1, "M": 1, "seqs": 1, "lens": None, "mode": "both"})
     with pytest.raises(ValueError, match="unknown kernel"):
         P.cacheAttention(Gpu(), {"q": {}, "o": {}, "kernel": "warp"})
+
+
+TOLD = r"""
+#include <cstdlib>
+#include <map>
+#include <vector>
+#include "cache_plan.h"
+using namespace p0p;
+#define CHECK(c) do { if (!(c)) { printf("line %d: %s\n", __LINE__, #c); exit(1); } } while (0)
+static uint32_t rnd(uint32_t n) { static uint64_t x = 88172645463325252ull; x ^= x << 13; x ^= x >> 7; x ^= x << 17; return (uint32_t)((x >> 11) % n); }
+
+int main() {
+  uint64_t both = 0;
+  for (int it = 0; it < 2000; it++) {
+    const uint32_t seqs = 1 + rnd(rnd(2) ? 2 : 20), most = rnd(2) ? 148 : 1 + rnd(20);
+    const CacheGeo g{1 + rnd(4), 1 + rnd(20), seqs, rnd(2) ? 1 + rnd(300) : 0, rnd(70)};
+    std::vector<CacheSeq> seq(seqs);
+    std::vector<uint64_t> pre(seqs + 1, 0);
+    uint64_t U = 0, items = 0;
+    struct Item { uint64_t i0, i1; uint32_t b, hk, rb; };
+    std::vector<Item> all;
+    for (uint32_t b = 0; b < seqs; b++) {
+      seq[b] = CacheSeq{0, rnd(3) ? rnd(3) : rnd(40), 0};
+      seq[b].L = seq[b].n + rnd(rnd(2) ? 400 : 9000);
+      if (seq[b].n) {
+        const uint32_t np = cache_visible(seq[b], g.window, g.sinks).np;
+        uint64_t u = U;
+        for (uint32_t h = 0; h < g.Hkv; h++) for (uint32_t rb = 0; rb * 16 < seq[b].n * g.group; rb++, u += np + 1, items++) all.push_back({u + 1, u + 1 + np, b, h, rb});
+      }
+      U += cache_units(seq[b], g); pre[b + 1] = U;
+    }
+    if (!U) continue;
+    const uint64_t G = cache_workers(U, items, most);
+    std::map<uint64_t, std::vector<uint64_t>> told;      // an item's first page -> the blocks that told
+    for (uint64_t c = 0; c < G; c++)
+      cache_tell_shares(g, pre.data(), seq.data(), deal_first(c, U, G), deal_first(c + 1, U, G), [&](const CacheCursor& x, uint64_t i0, uint64_t i1) {
+        bool known = false;
+        for (const Item& y : all) if (y.i0 == i0) { known = true; CHECK(y.i1 == i1 && y.b == x.b && y.hk == x.hk && y.rb == x.rb); }
+        CHECK(known);
+        told[i0].push_back(c);
+      });
+    for (const Item& y : all) {                          // every block that has a page of an item that crosses blocks, once
+      const uint64_t c0 = deal_owner(y.i0, U, G), c1 = deal_owner(y.i1 - 1, U, G);
+      std::vector<uint64_t> want;
+      if (c0 != c1) for (uint64_t c = c0; c <= c1; c++) want.push_back(c);
+      CHECK(told[y.i0] == want);
+      if (c0 != c1 && (deal_first(c0, U, G) == y.i0 || deal_first(c0, U, G) + 1 == y.i0)) both++;
+    }
+  }
+  CHECK(both > 100);                                     // (blocks that are a share of one item, which begins with them)
+  printf("fine\n");
+  return 0;
+}
+"""
+
+
+def test_a_block_that_gives_up_tells_each_item_once(tmp_path):
+    src, exe = tmp_path / "told.cpp", tmp_path / "told"
+    src.write_text(TOLD)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-Wall", "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                    "-I", os.path.join(ROOT, "p0pc0rn_kernels_b200", "csrc"), str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
