@@ -383,6 +383,7 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
       u = end;
       cur = nxt; blk = nxt_blk;
     }
+    if (!ok && lane < 2u) mbar_drain(bars + 8u * lane, p.c.status, 613);
   }
   __syncthreads();
   // ---- the warps' shares of one item, merged in order, a row per warp; an item that is all here is finished.  A row of another one goes to memory, and the

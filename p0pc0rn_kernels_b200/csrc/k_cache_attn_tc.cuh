@@ -94,14 +94,14 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
   const uint32_t q_sm = base, kv_sm = base + 2u * ATC_TILE, st_sm = kv_sm + CTC_SLOTS * ATC_TILE, bars = st_sm + 8u * CTC_STAGE;
   const uint32_t q_full = bars, q_empty = bars + 8u, st_full = bars + 16u, kv_full = st_full + 64u, kv_empty = kv_full + 8u * CTC_SLOTS, s_full = kv_empty + 8u * CTC_SLOTS, p_full = s_full + 16u;
   const uint32_t o_full = p_full + 16u, seg_full = o_full + 16u, seg_empty = seg_full + 8u * CTC_SEGS, pair_full = seg_empty + 8u * CTC_SEGS, pair_empty = pair_full + 8u * CTC_PAIRS;
-  const uint32_t tmem_slot = pair_empty + 8u * CTC_PAIRS;
+  const uint32_t all_done = pair_empty + 8u * CTC_PAIRS, tmem_slot = all_done + 8u;
   float* xch = reinterpret_cast<float*>(gbase + (bars + 512u - base));
   CtcPage* scl = reinterpret_cast<CtcPage*>(xch + 512);                   // [pair][page of it]
   volatile CtcSeg* segs = reinterpret_cast<volatile CtcSeg*>(scl + 2u * CTC_PAIRS);
   volatile uint32_t* at = reinterpret_cast<volatile uint32_t*>(const_cast<CtcSeg*>(segs) + CTC_SEGS);
   const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
   if (tid == 0) {
-    mbar_init(q_full, 1u); mbar_init(q_empty, 1u);
+    mbar_init(q_full, 1u); mbar_init(q_empty, 1u); mbar_init(all_done, 1u);
     for (uint32_t s = 0; s < 8u; s++) mbar_init(st_full + 8u * s, 1u);
     for (uint32_t s = 0; s < CTC_SLOTS; s++) { mbar_init(kv_full + 8u * s, 2u); mbar_init(kv_empty + 8u * s, 1u); }
     for (uint32_t t = 0; t < 2u; t++) { mbar_init(s_full + 8u * t, 1u); mbar_init(p_full + 8u * t, 8u); mbar_init(o_full + 8u * t, 1u); }
@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
       }
     } else if (warp == 2u) {
       // ================================================================= queries
-      for (uint32_t seg = 0u;; seg++) {
+      uint32_t seg = 0u;
+      for (;; seg++) {
         if (!__all_sync(0xffffffffu, seg_wait(seg))) break;
         volatile CtcSeg& g = segs[seg % CTC_SEGS];
         if (!g.cnt) break;
@@ -244,6 +245,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
             for (uint32_t c = 0; c < 2u; c++) tma_load_4d(q_sm + t * ATC_TILE + c * 16384u, &mapQ, (int)(c * 64u), 0, (int)(r0 + t * p.geo.qpt), (int)hk, q_full);
         }
       }
+      if (seg > 0u) mbar_wait(q_full, (seg - 1u) & 1u, p.c.status, 635);   // (the last ones are here before the block ends, whatever became of the others)
     } else if (warp == 1u) {
       // ================================================================= multiplies (the whole warp walks the loop, one lane issues)
       const uint32_t idesc = umma_idesc_f16(128u, 128u);
@@ -305,6 +307,9 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
           __syncwarp();
         }
       }
+      if (elect_one()) umma_commit(all_done);                             // (no multiply is under way when the block ends)
+      __syncwarp();
+      mbar_wait(all_done, 0u, p.c.status, 636);
     }
   } else if (warp < 8u) {
     // ================================================================= codes (or the tail's fp16) -> fp16 tiles
@@ -389,6 +394,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
       if (ok && !known && lane < 2u && nx[lane].is == 0u) fetch(nx[lane].block, lane);
       __syncwarp();
     }
+    if (!ok && lane < 2u) mbar_drain(bar + 8u * lane, p.c.status, 637);
   } else {
     // ================================================================= softmax of one tile: two threads per row, one page of a pair each
     regs_up<104>();

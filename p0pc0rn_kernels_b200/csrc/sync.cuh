@@ -38,6 +38,10 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* st
   return true;
 }
 
+// For a kernel that has given up: waits (bounded too) for the copies that complete on `bar`, so that its block does not end while they are under way.  It
+// waits for the barrier's present phase; where nothing is under way that takes the limit once more.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, int* status, int code) { mbar_wait(bar, mbar_try(bar, 0u) ? 1u : 0u, status, code); }
+
 // ---- a pair of blocks (a cluster of two): ranks, the other block's shared memory, barriers across the two
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 // the address, in the cluster's shared window, of this block's shared address `a` in block `rank`
