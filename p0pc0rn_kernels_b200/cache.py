@@ -53,8 +53,14 @@ def kvCache(gpu, a: dict) -> dict:
     can be passed to share them.  The buffers are freed with gpu.free."""
     n = cacheBytes(a["pages"], a["Hkv"], a["seqs"], a["maxPages"])
     c = {k: a[k] for k in ("Hkv", "pages", "seqs", "maxPages")}
-    for k in ("codes", "scales", "tail", "table", "lens"):
-        c[k] = a.get(k) or {"buf": gpu.buffer(n[k], "cache " + k), "off": 0}
+    made = []
+    try:
+        for k in ("codes", "scales", "tail", "table", "lens"):
+            if not a.get(k): made.append(gpu.buffer(n[k], "cache " + k))
+            c[k] = a.get(k) or {"buf": made[-1], "off": 0}
+    except Exception:
+        for b in made: gpu.free(b)           # (no room for a later one: none is left behind)
+        raise
     return c
 
 

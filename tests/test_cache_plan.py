@@ -352,3 +352,31 @@ def test_numbers_that_fp32_does_not_hold_are_refused_before_the_call():
     for bad in (1e39, -1e300):
         with pytest.raises(ValueError, match="cacheAttention: bad argument"):
             P.cacheAttention(Gpu(), {"cache": cache, "q": none, "o": none, "Hq": 1, "M": 1, "scale": bad})
+
+
+def test_a_cache_that_does_not_fit_leaves_no_buffers_behind():
+    import p0pc0rn_kernels_b200 as P
+    import pytest
+
+    class Gpu:
+        def __init__(self, room): self.room, self.held = room, []
+
+        def buffer(self, size, label=""):
+            if len(self.held) == self.room: raise P.GpuError("no room")
+            self.held.append(label)
+            return label
+
+        def free(self, b): self.held.remove(b)
+    a = {"Hkv": 1, "pages": 2, "seqs": 1, "maxPages": 2}
+    for room in range(5):
+        g = Gpu(room)
+        with pytest.raises(P.GpuError, match="no room"): P.kvCache(g, a)
+        assert g.held == []
+    g = Gpu(5)
+    c = P.kvCache(g, a)
+    assert [c[k]["buf"] for k in ("codes", "scales", "tail", "table", "lens")] == g.held and len(g.held) == 5
+    g = Gpu(2)                                            # (a shared table and lengths are another cache's)
+    with pytest.raises(P.GpuError, match="no room"): P.kvCache(g, {**a, "table": {"buf": "t"}, "lens": {"buf": "l"}})
+    assert g.held == []
+    g = Gpu(3)
+    assert P.kvCache(g, {**a, "table": {"buf": "t"}, "lens": {"buf": "l"}})["lens"] == {"buf": "l"}
