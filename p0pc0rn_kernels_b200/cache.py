@@ -67,7 +67,7 @@ def kvCache(gpu, a: dict) -> dict:
 def _pack(op, layout, *values) -> bytes:
     try:
         return layout.pack(*values)
-    except (struct.error, OverflowError) as e:      # a negative or fractional number, or one that its bits do not hold
+    except struct.error as e:                # a negative or fractional number, or one that no 32 (64) bits hold
         raise ValueError(f"{op}: bad argument ({e})") from None
 
 

@@ -341,19 +341,6 @@ def test_a_block_that_gives_up_tells_each_item_once(tmp_path):
     assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
 
 
-def test_numbers_that_fp32_does_not_hold_are_refused_before_the_call():
-    import p0pc0rn_kernels_b200 as P
-    import pytest
-
-    class Gpu:
-        _h = _check = None
-    none = {"buf": type("B", (), {"handle": None})()}
-    cache = {"Hkv": 1, "pages": 1, "seqs": 1, "maxPages": 1, **{k: none for k in ("codes", "scales", "tail", "table", "lens")}}
-    for bad in (1e39, -1e300):
-        with pytest.raises(ValueError, match="cacheAttention: bad argument"):
-            P.cacheAttention(Gpu(), {"cache": cache, "q": none, "o": none, "Hq": 1, "M": 1, "scale": bad})
-
-
 def test_a_cache_that_does_not_fit_leaves_no_buffers_behind():
     import p0pc0rn_kernels_b200 as P
     import pytest
