@@ -44,8 +44,8 @@ extern "C" int p0p_rope(p0p_ctx* c, const p0p_rope_args* a) {
   const double theta = a->theta != 0.0 ? a->theta : 10000.0, factor = a->factor != 0.0 ? a->factor : 1.0, fast = a->fast != 0.0 ? a->fast : 32.0, slow = a->slow != 0.0 ? a->slow : 1.0,
                mscale = a->mscale != 0.0 ? a->mscale : 1.0;
   if (!(theta > 0.0) || !std::isfinite(theta) || !(factor > 0.0) || !std::isfinite(factor) || !(a->original >= 0.0) || !std::isfinite(a->original) || !(fast > slow) || !std::isfinite(fast) ||
-      !(slow >= 0.0) || !std::isfinite(mscale))
-    return fail(c, -2, "rope: theta and factor must be positive, original at least 0, fast above slow");
+      !(slow >= 0.0) || !std::isfinite((float)mscale))
+    return fail(c, -2, "rope: theta and factor must be positive, original at least 0, fast above slow, mscale within fp32");
   const uint32_t M = a->M, ldx = a->ldx ? a->ldx : M, ldy = a->ldy ? a->ldy : (a->y ? M : ldx);
   char msg[256];
   if (int rc = cache_rows_check("rope", M, a->seqs, a->rows != nullptr, cache_room(c, a->rows, a->rows_off), a->rows_off, msg, sizeof msg)) return cache_refuse(c, rc, msg);
@@ -70,6 +70,7 @@ extern "C" int p0p_rope(p0p_ctx* c, const p0p_rope_args* a) {
       f *= g + (1.0 - g) / factor;
     }
     p.turn[i] = f / pi2;
+    if (!(p.turn[i] <= 0x1p990)) return fail(c, -2, "rope: theta or factor too small: the angle of a far position (2^32) has to be a finite number");
   }
   const bool odd = a->mode == 1u && (a->rot & 15u);
   const uint32_t rows_per_block = odd ? 4u : 16u, gx = (M + rows_per_block - 1u) / rows_per_block;

@@ -796,3 +796,20 @@ def test_attention_beside_a_tail_of_small_values(gpu, size, kernel):
         for n in ([1, 2], [40, 70]): _check_rms(cache, n, 4, kernel=kernel)
     finally:
         cache.free()
+
+
+def test_rope_refuses_what_ends_in_no_number(gpu):
+    """a factor that fp32 does not hold, frequencies whose angles are infinite: refused; what is large or small and still a number is not"""
+    import p0pc0rn_kernels_b200 as P
+    b, lens = gpu.upload(np.ones((2, 3, 128), np.float16)), gpu.upload(np.array([4000000000], np.uint32))
+    args = {"x": {"buf": b}, "H": 2, "M": 3, "seqs": 1, "lens": {"buf": lens}, "mode": "half"}
+    try:
+        for kw in (dict(mscale=1e39), dict(mscale=-1e300), dict(mscale=float("nan")), dict(theta=5e-324), dict(factor=1e-308), dict(theta=1e-300, factor=1e-20), dict(factor=1e-308, original=1.0)):
+            with pytest.raises(ValueError, match="rope"): P.rope(gpu, {**args, **kw})
+        for kw in (dict(theta=1e300), dict(factor=1e300), dict(theta=1e-200), dict(factor=1e-200), dict(mscale=0.5)): P.rope(gpu, {**args, **kw})
+        got = gpu.read(b).view(np.float16)[:2 * 3 * 128]
+        # (five turns of pairs of ones, each off by the rounding to fp16, one of them by half: no pair is longer than sqrt 2)
+        assert np.isfinite(got).all() and np.abs(got).max() <= 0.5 * 2.0 ** 0.5 * (1 + 2.0 ** -11) ** 5 + 5 * 2.0 ** -25
+        assert not gpu.lost
+    finally:
+        gpu.free(b); gpu.free(lens)
