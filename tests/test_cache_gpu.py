@@ -813,3 +813,93 @@ def test_rope_refuses_what_ends_in_no_number(gpu):
         assert not gpu.lost
     finally:
         gpu.free(b); gpu.free(lens)
+
+
+def _pages_apart(cache, lens, seed=1, std=1.0):
+    """fills a cache with values that have a mean of their own in each page, and keys of a size of their own"""
+    rng = np.random.default_rng(seed)
+    k, v = [], []
+    for L in lens:
+        n = -(-int(L) // PAGE)
+        size, mean = np.exp(rng.normal(0, 0.1, (cache.Hkv, n, 1))), rng.normal(0, 1, (cache.Hkv, n, 128))
+        spread = np.exp(rng.normal(0, 0.3, (cache.Hkv, n, 1)))
+        def tokens(scale, add):
+            x = rng.normal(0, std, (cache.Hkv, n * PAGE, 128))
+            return (x * np.repeat(scale, PAGE, 1) + np.repeat(add, PAGE, 1))[:, :int(L)].astype(np.float16)
+        k.append(tokens(size, 0 * mean)); v.append(tokens(0.7 * spread, mean))
+    cache.write(list(lens), k, v)
+
+
+LONG = [
+    # (first three: more than 32 and 64 pages of an item in a warp's share, more than 32 pairs of pages in a block's: test_cache_plan.py)
+    dict(label="long contexts among many: shares of many pages", Hkv=8, group=16, lens=[400, 20000, 37], news=[310, 12, 20], kernel="split"),
+    dict(label="a long prompt over a long context: blocks with many pairs of an item", Hkv=8, group=4, lens=[8000], news=[1100], kernel="tmem"),
+    dict(label="a chunk of a prompt, split keys: shares of more pages still", Hkv=4, group=16, lens=[9000], news=[700], kernel="split"),
+    dict(label="one token, four pages per warp", Hkv=4, group=4, lens=[40000], news=[1], kernel="split"),
+    dict(label="few queries over a long context", Hkv=2, group=4, lens=[20000], news=[70], kernel="tmem"),
+    dict(label="few queries over a long context, split keys", Hkv=2, group=4, lens=[20000], news=[70], kernel="split"),
+    dict(label="several long contexts", Hkv=8, group=4, lens=[3000, 9001, 5000, 64 * 70], news=[1, 2, 1, 1], kernel="split"),
+    dict(label="several contexts, prompts", Hkv=2, group=7, lens=[3000, 5001, 64 * 30], news=[40, 90, 150], kernel="tmem"),
+]
+
+
+@pytest.mark.parametrize("c", LONG, ids=lambda c: c["label"])
+def test_attention_reads_every_page_once(gpu, c):
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, c["Hkv"], len(c["lens"]), -(-max(c["lens"]) // PAGE), seed=13)
+    try:
+        _pages_apart(cache, c["lens"])
+        some = [(b, pg) for b, L in enumerate(c["lens"]) for pg in sorted({0, 1, 31, 32, 33, 64, L // PAGE // 2, (L - 1) // PAGE - 1, (L - 1) // PAGE}) if pg <= (L - 1) // PAGE and L > 100]
+        _check_rms(cache, c["news"], c["group"], kernel=c["kernel"], without=some)
+        _check_rms(cache, c["news"], c["group"], kernel=c["kernel"], window=2500, sinks=70)
+    finally:
+        cache.free()
+
+
+ROPE_MORE = [
+    dict(label="many heads per thread, half", mode="half", H=41, M=4200, seqs=3),
+    dict(label="many heads per thread, interleaved", mode="interleaved", H=40, M=4200, seqs=2),
+    dict(label="many heads per thread, half, odd part", mode="half", rot=38, H=23, M=1700, seqs=2),
+    dict(label="part of the head, many heads", mode="half", rot=64, H=33, M=3001, seqs=1),
+    dict(label="equal counts", mode="half", H=3, M=35, seqs=5, rows=False),
+    dict(label="equal counts, odd part", mode="half", rot=10, H=3, M=35, seqs=5, rows=False),
+    dict(label="equal counts, interleaved, many heads", mode="interleaved", H=40, M=4200, seqs=100, rows=False),
+    dict(label="40 sequences, some empty", mode="half", H=3, M=211, seqs=40),
+    dict(label="300 sequences, some empty", mode="interleaved", H=2, M=1201, seqs=300),
+    dict(label="300 sequences, odd part", mode="half", rot=22, H=2, M=1201, seqs=300),
+    dict(label="32 sequences", mode="half", H=2, M=77, seqs=32),
+]
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("c", ROPE_MORE, ids=lambda c: c["label"])
+def test_rope_heads_and_sequences(gpu, c, inplace):
+    """more heads than a thread holds at once, equal counts, more sequences than a warp looks at; tolerances as in test_rope"""
+    import p0pc0rn_kernels_b200 as P
+    rng = np.random.default_rng(3)
+    H, M, seqs, rot, equal = c["H"], c["M"], c["seqs"], c.get("rot", 128), c.get("rows") is False
+    cuts = np.arange(seqs + 1) * (M // seqs) if equal else np.concatenate([[0], np.sort(rng.integers(0, M + 1, seqs - 1)), [M]])
+    if not equal and seqs > 5: cuts[3] = cuts[2]; cuts[-2] = M                                 # (sequences without tokens, the last one too)
+    offs = cuts.astype(np.uint32); news = np.diff(cuts)
+    lens = (news + rng.integers(0, 100000, seqs)).astype(np.uint32)
+    x = rng.normal(0, 1, (H, M, 128)).astype(np.float16)
+    xb, lb = gpu.upload(x), gpu.upload(lens)
+    yb, rb = (None if inplace else gpu.upload(np.full((H, M + 3, 128), 0x7E01, np.uint16))), (None if equal else gpu.upload(offs))
+    try:
+        P.rope(gpu, {"x": {"buf": xb}, "y": {"buf": yb, "ld": M + 3} if yb else None, "H": H, "M": M, "seqs": seqs, "lens": {"buf": lb}, "rows": {"buf": rb} if rb else None, "mode": c["mode"], "rot": rot})
+        got = gpu.read(yb or xb).view(np.float16)[:H * (M if inplace else M + 3) * 128].reshape(H, -1, 128)
+        if not inplace: assert (got[:, M:].view(np.uint16) == 0x7E01).all()
+        got = got[:, :M]
+        pos = np.concatenate([np.arange(L - n, L, dtype=np.float64) for L, n in zip(lens.astype(np.int64), news)])
+        ang = pos[:, None] * _freq(rot); cs, sn = np.cos(ang), np.sin(ang)
+        first, second = (slice(0, rot // 2), slice(rot // 2, rot)) if c["mode"] == "half" else (slice(0, rot, 2), slice(1, rot, 2))
+        for h in range(H):
+            z = x[h].astype(np.float64); want = z.copy(); mag = np.zeros_like(z)
+            a, b = z[:, first], z[:, second]
+            want[:, first], want[:, second] = a * cs - b * sn, a * sn + b * cs
+            mag[:, first] = mag[:, second] = np.abs(a) + np.abs(b)
+            tol = np.abs(want) * 2.0 ** -11 + 2.0 ** -25 + mag * (6 * 2.0 ** -24 + float(pos.max()) * 8 * 2.0 ** -53)
+            assert (np.abs(got[h].astype(np.float64) - want) <= tol).all(), h
+            assert np.array_equal(got[h][:, rot:], x[h][:, rot:])
+    finally:
+        for t in (xb, yb, lb, rb): gpu.free(t)

@@ -367,3 +367,75 @@ def test_a_cache_that_does_not_fit_leaves_no_buffers_behind():
     assert g.held == []
     g = Gpu(3)
     assert P.kvCache(g, {**a, "table": {"buf": "t"}, "lens": {"buf": "l"}})["lens"] == {"buf": "l"}
+
+
+SHARES = r"""
+#include <cstdlib>
+#include <vector>
+#include "cache_plan.h"
+using namespace p0p;
+#define CHECK(c) do { if (!(c)) { printf("line %d: %s\n", __LINE__, #c); exit(1); } } while (0)
+// the longest run of one item's pages in a warp's share (split keys, 148 blocks of 8 warps)
+static uint32_t split_run(uint32_t Hkv, uint32_t group, std::vector<CacheSeq> seq, uint32_t window, uint32_t sinks) {
+  const CacheGeo g{Hkv, group, (uint32_t)seq.size(), window, sinks};
+  std::vector<uint64_t> pre(seq.size() + 1, 0);
+  uint64_t U = 0, items = 0;
+  for (size_t b = 0; b < seq.size(); b++) { U += cache_units(seq[b], g); pre[b + 1] = U; items += (uint64_t)Hkv * ((seq[b].n * group + 15) / 16); }
+  const uint64_t G = cache_workers(U, items, 148);
+  uint32_t most = 0;
+  for (uint64_t c = 0; c < G; c++) {
+    const uint64_t u0 = deal_first(c, U, G), n = deal_first(c + 1, U, G) - u0, W = n < 8 ? n : 8;
+    for (uint64_t w = 0; w < W; w++) {
+      const uint64_t w0 = u0 + deal_first(w, n, W), w1 = u0 + deal_first(w + 1, n, W);
+      CacheCursor x;
+      x.seek(g, pre.data(), seq.data(), w0);
+      for (uint64_t u = w0; u < w1;) {
+        const uint64_t end = u + (x.v.np + 1 - x.at) < w1 ? u + (x.v.np + 1 - x.at) : w1;
+        const uint32_t cnt = (uint32_t)(end - u) - (x.at ? 0 : 1);
+        if (cnt > most) most = cnt;
+        u = end;
+        if (u < w1) x.next_item(g, pre.data(), seq.data());
+      }
+    }
+  }
+  return most;
+}
+// the longest run of one item's pairs of pages in a block's share (tensor memory)
+static uint32_t tc_run(uint32_t Hkv, uint32_t group, std::vector<CacheSeq> seq, uint32_t window, uint32_t sinks) {
+  const CacheTcGeo g{Hkv, group, (uint32_t)seq.size(), window, sinks, 128 / group, 0};
+  struct At { uint32_t b, x, hk, at; };
+  std::vector<At> all;
+  uint64_t items = 0;
+  for (uint32_t b = 0; b < seq.size(); b++)
+    for (uint32_t x = 0; x < cache_tc_blocks(seq[b], g); x++)
+      for (uint32_t h = 0; h < Hkv; h++) { items++; const uint32_t n = cache_tc_cost(cache_tc_part(seq[b], g, x), g); for (uint32_t c = 0; c < n; c++) all.push_back({b, x, h, c}); }
+  const uint64_t U = all.size(), G = cache_tc_workers(U, items, 148);
+  uint32_t most = 0;
+  for (uint64_t c = 0; c < G; c++) {
+    const uint64_t u0 = deal_first(c, U, G), u1 = deal_first(c + 1, U, G);
+    CacheTcWalk w;
+    const auto get = [&](uint32_t b) { return seq[b]; };
+    for (w.begin(g, all[u0].b, all[u0].x, all[u0].hk, all[u0].at, (uint32_t)(u1 - u0), get); w.cnt; w.next(g, get)) if (w.cnt > most) most = w.cnt;
+  }
+  return most;
+}
+static CacheSeq s(uint32_t r0, uint32_t n, uint32_t L) { return CacheSeq{r0, n, L}; }
+int main() {
+  // (the kernels take an item's page numbers and scales 32 pages at a time)
+  const uint32_t a = split_run(8, 16, {s(0, 310, 400), s(310, 12, 20000), s(322, 20, 37)}, 0, 0), b = tc_run(8, 4, {s(0, 1100, 8000)}, 0, 0), c = split_run(4, 16, {s(0, 700, 9000)}, 0, 0);
+  printf("%u %u %u\n", a, b, c);
+  CHECK(a > 32 && b > 32 && c > 64);
+  printf("fine\n");
+  return 0;
+}
+"""
+
+
+def test_the_long_cases_hand_over_page_numbers(tmp_path):
+    """cases of test_cache_gpu.py whose shares of one item are longer than the 32 pages that are looked up at a time"""
+    src, exe = tmp_path / "shares.cpp", tmp_path / "shares"
+    src.write_text(SHARES)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-Wall", "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                    "-I", os.path.join(ROOT, "p0pc0rn_kernels_b200", "csrc"), str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stdout + r.stderr
