@@ -234,7 +234,7 @@ int p0p_attention(p0p_ctx* ctx, const p0p_attn_args* args, double* flops);
  * contents.  `lens` counts the tokens of the present call too: a sequence's n new tokens are its last n, at positions
  * lens - n .. lens - 1.  The new tokens of all sequences are consecutive rows of the call's tensors; sequence b has rows rows[b] ..
  * rows[b + 1] - 1 (u32 [seqs + 1]), or, without row offsets, M / seqs rows each.  A sequence may have none.  Rows behind the
- * last sequence's are neither read nor written.
+ * last sequence's (they belong to the tensors all the same) are not written, and what they hold changes nothing.
  * A sequence whose numbers make no sense (row offsets that fall or exceed M; fewer tokens than rows; more than 64 * max_pages) is
  * left out, a page number outside the cache is not followed; either makes the next p0p_sync / p0p_read return -10. */
 typedef struct p0p_cache {
@@ -269,7 +269,8 @@ typedef struct p0p_cache_attn_args {
 /* causal attention of the call's queries over the cache, which holds their own keys and values already (p0p_cache_write comes first).
  * Query head h reads kv head h / (Hq / Hkv).  Partial results are kept in the context's scratch memory.  o may overlap neither q nor the cache.
  * Arithmetic: scores and sums in fp32 (a score's error is 2^-22 or so of the largest product that it sums: scores beyond 2^20 are told apart only so far);
- * a weight of the softmax, times its block's V scale, is rounded to fp16 relative to the largest such product of its row. */
+ * a weight of the softmax, times its block's V scale, is rounded to fp16 relative to the largest such product of its row
+ * (the tail has no scale: its weights are rounded on their own, and cost the others' nothing). */
 int p0p_cache_attention(p0p_ctx* ctx, const p0p_cache_attn_args* args);
 
 /* rotary positions: y = x with the first `rot` elements of every head turned by its token's position (y may be x, but not overlap it

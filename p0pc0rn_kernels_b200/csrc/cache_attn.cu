@@ -14,10 +14,13 @@ namespace {
 
 constexpr char OP[] = "cacheAttention";
 // Query rows per kv head up to which a sequence is the split-key kernel's.  Its time grows with every 16 rows, the tensor-memory kernel's hardly up to
-// 256, but that one starts later (two launches, a longer pipeline).  Measured, split keys / tensor memory, 8 kv heads:
-//   8 sequences of 16000:  32 rows 84 / 113 us, 48 rows 126 / 114, 64 rows 163 / 116      64 of 4000: 32 rows 177 / 225, 48 rows 254 / 247, 64 rows 330 / 250
-//   1 sequence of 500:     96 rows 13 / 21, 128 rows 14 / 22      of 4000: 96 rows 18 / 25, 128 rows 20 / 24      of 32000: 64 rows 49 / 48, 96 rows 61 / 49, 128 rows 86 / 49
-// so with few sequences and heads, whose contexts hardly fill the machine, the border lies higher.
+// 256, but that one has the longer pipeline.  Measured, split keys / tensor memory, us, 8 kv heads:
+//   8 sequences of 16000:  32 rows 87 / 114, 48 rows 127 / 114, 64 rows 164 / 117      64 of 4000: 32 rows 176 / 221, 48 rows 253 / 251, 64 rows 331 / 246
+//   1 sequence of 500:     96 rows 13 / 22, 128 rows 14 / 22      of 4000: 96 rows 18 / 25, 128 rows 21 / 24      of 32000: 48 rows 38 / 48, 64 rows 50 / 48, 96 rows 63 / 48
+// With few sequences and heads, whose contexts hardly fill the machine, the border lies higher.  The host does not know the lengths, so both borders are a
+// compromise: at 33 to 48 rows (three blocks of 16) the split-key kernel is the slower one over long contexts (above; with 4 heads 86 / 68) and the faster one
+// over shorter ones (8 sequences of 4000: 41 / 43, with 4 heads 28 / 30; of 500 with 4 heads 11 / 19); one sequence of 32000 would be better off with the
+// other kernel from 64 rows on, one of 500 at no size up to 256.
 inline uint32_t split_rows(uint32_t seqs, uint32_t Hkv) { return (uint64_t)seqs * Hkv <= 16u ? 96u : 48u; }
 
 int run_split(p0p_ctx* c, CacheAttnP& p, uint32_t G) {

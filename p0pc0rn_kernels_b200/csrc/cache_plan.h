@@ -169,7 +169,7 @@ P0P_HD constexpr uint32_t cache_col_key(uint32_t c) { return 16u * ((c >> 2) & 3
 // (Dealt out by units alone, a block at the start of a prompt, with many items of one unit or two, took 1.7 times as long as the others.)
 constexpr uint32_t CACHE_TC_ITEM = 2u;
 P0P_HD uint32_t cache_tc_cost(const CacheSeq& part, const CacheTcGeo& g) { return CACHE_TC_ITEM + cache_tc_units(part, g); }
-// What a block does next: units [t, t + cnt) of an item; cnt 0: nothing more.  Every role of the block walks the same list by itself.  get(b): sequence b.
+// What a block does next: units [t, t + cnt) of an item; cnt 0: nothing more.  One warp of the block walks the list and announces it to the others.  get(b): sequence b.
 struct CacheTcWalk {
   CacheSeq s, part; CacheVis v;
   uint32_t b, x, blocks, hk, t, units, cnt, left, spent;      // spent: the cost, from the beginning of the block's share, of unit t

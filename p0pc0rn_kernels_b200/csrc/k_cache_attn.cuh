@@ -7,7 +7,8 @@
 //   rounding: where a page's scale is 2^20 times another's, the other's weights are subnormals or 0, which its own small values bear but the sum would not.
 //   The second term is taken off page by page: left to the end, the sums of u grow 128 times the number of keys and their rounding with
 //   them (8000 keys in one accumulator: 2e-3 of the result; page by page 2.3e-4, of which 2.1e-4 is the result's own rounding).
-// The running maximum m is that of score + log2 vs, raised when it grew by more than 2^8: weights are at most 256.  Statistics and sums are fp32; the weights' rounding to fp16 (2^-11 each,
+// The running maximum m is that of score + log2 vs, raised when it grew by more than 2^8: weights are at most 256.  Scores beyond 2^10 lose their page's largest
+// first, so that no rounding of m comes into the exponent (cache_far).  Statistics and sums are fp32; the weights' rounding to fp16 (2^-11 each,
 // independent from key to key) is what tensor-core products of fp32 sums cost, as in k_attn.cuh.
 //
 // Work: a unit = one visible page of one kv head for up to 16 query rows (the rows of all heads that share the kv head, query-major; more
@@ -19,7 +20,7 @@
 // it), in order: deterministic, one launch.
 // Bound: one pass over the visible codes (HBM).  32:8 heads, 64 sequences of up to 4096 tokens, 328 MB: 62 to 64 us = 5.2 TB/s, 0.79 of the measured copy (while
 // all warps stream, at its rate; the rest is the launch, the first pages' latency and the end: shares of whole pages of 2.3 us, 3 us to
-// merge).  One sequence of 32000, 66 MB: 19.9 us = 0.50 (three or four pages per warp).  One of 300: 7.1 us, all latency.  Tried and slower: K one more page
+// merge).  One sequence of 32000, 66 MB: 20.0 us = 0.50 (three or four pages per warp).  One of 300: 7.2 us, all latency.  Tried and slower: K one more page
 // ahead in a third buffer (66 -> 70 us: V then comes late), asking the L2 for pages 1, 2 or 4 ahead (63 -> 70, 80, 92).
 #pragma once
 #include <cuda_fp16.h>

@@ -7,13 +7,15 @@
 //           16 keys of one d (so V's tile is K-major).  The keys stand in the order of V's elements in both (cache_col_key).
 //   scales  a thread's 64 scores belong to one page: its K scale joins the softmax scale, its V scale the exponent (w = 2^(score + log2 vs - m),
 //           and the sum of the weights is weighted with 1 / vs), as in k_cache_attn.cuh
-//   work    the pairs of visible pages of all items (block of queries, kv head) in one row are dealt out evenly to one block per SM, from the
-//           numbers on the device; the shares of an item that crosses blocks are added up by the warp that arrives last with one
+//           The tail has no scale: its weights are up to 2^15 instead (CTC_TAIL).  Scores beyond 2^10 lose their page's largest first (cache_far).
+//   work    all items (block of queries, kv head) in one row are dealt out by cost, a unit for each pair of visible pages and CACHE_TC_ITEM for the item itself, to
+//           one block per SM, from the numbers on the device.  An item within one block is finished there.  One of two shares is added up by the block that arrives
+//           last with one, its own in tensor memory.  One of more shares is added up from memory: by the last block, or, where items are few (p.desc), by k_cache_merge
 // Roles: warp 0 keeps the list of work (items, and page by page what the others need to know), warp 1 multiplies, warp 2 loads queries, warps 4-7 convert,
 // warps 8-15 and 16-23 are the softmax of the two tiles, two threads per row.  The softmax threads take the registers that the others leave
 // (setmaxnreg; per scheduler 4 x 104 + 24 + 40 = the 6 x 80 of the launch; with 32 for each of the others the converting warps spilled: 249 against 246.5 us).
-// Bound: 2000 tokens over 6100 of 32:8 heads, 233 GFLOP: 232 us = 1000 TFLOP/s, 0.61 of the measured burst, under the power limit (1.6 to 1.7 GHz).  A pair of
-// pages takes about 4200 cycles of a block: its multiplies alone 1900 (tensor pipe active 54 %), its traffic through shared memory 2500 (operands, codes
+// Bound: 2000 tokens over 6100 of 32:8 heads, 233 GFLOP: 233 us = 1000 TFLOP/s, 0.60 of the measured burst, under the power limit (1.6 to 1.7 GHz).  A pair of
+// pages takes about 4200 cycles of a block: its multiplies alone 1900 (tensor pipe active 51 to 54 %), its traffic through shared memory 2500 (operands, codes
 // in, tiles out), the converting warps about 3500 (latency: a warp's 16 units of 32 bytes, waits and fences in a row), a softmax warp 1700.  Tried and slower: conversion
 // by the softmax warps between two tiles (308 us), K as fp16 subnormals with a row sum of q (255 against 260 then, but 147 against 141 for short
 // items), 96 registers for the softmax and 48 for the others (390), three slots of tiles and more codes (256).
