@@ -270,7 +270,7 @@ typedef struct p0p_cache_attn_args {
  * Query head h reads kv head h / (Hq / Hkv).  Partial results are kept in the context's scratch memory.  o may overlap neither q nor the cache.
  * Arithmetic: scores and sums in fp32 (a score's error is 2^-22 or so of the largest product that it sums: scores beyond 2^20 are told apart only so far);
  * a weight of the softmax, times its block's V scale, is rounded to fp16 relative to the largest such product of its row
- * (the tail has no scale: its weights are rounded on their own, and cost the others' nothing). */
+ * (the tail has no scale: its weights are rounded on their own, and cost the others' nothing).  A result beyond the largest fp16 becomes that. */
 int p0p_cache_attention(p0p_ctx* ctx, const p0p_cache_attn_args* args);
 
 /* rotary positions: y = x with the first `rot` elements of every head turned by its token's position (y may be x, but not overlap it

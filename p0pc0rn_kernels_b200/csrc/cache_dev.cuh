@@ -15,6 +15,10 @@ struct CacheP {
   int* status;
 };
 
+// two results as fp16: a mean of finite values stays finite, although a code of 127 times a scale that was rounded up, or weights that were, can pass the
+// largest fp16.  NaN stays NaN
+__device__ __forceinline__ uint32_t cache_result(float a, float b) { uint32_t r; asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a)); return r; }
+
 __device__ __forceinline__ void cache_tell(int* status, int code) { if (code) atomicCAS(status, 0, code); }
 // sequence b of the call; one whose numbers make no sense has n = 0 (every block that meets it says so)
 __device__ __forceinline__ CacheSeq cache_seq(const CacheP& p, uint32_t b) {

@@ -363,9 +363,9 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
         for (uint32_t h = 0; h < 2u; h++) {
           const uint32_t r = cur.rb * 16u + h * 8u + g, i = r / p.group;
           if (r < rows) {
-            __half2* dst = reinterpret_cast<__half2*>(p.O + (size_t)(cur.s.r0 + i) * p.ldo + (cur.hk * p.group + (r - i * p.group)) * 128u + 2u * t4);
+            uint32_t* dst = reinterpret_cast<uint32_t*>(p.O + (size_t)(cur.s.r0 + i) * p.ldo + (cur.hk * p.group + (r - i * p.group)) * 128u + 2u * t4);
 #pragma unroll
-            for (int d = 0; d < 16; d++) dst[4 * d] = __floats2half2_rn(o[d][2 * h] * inv[h], o[d][2 * h + 1] * inv[h]);
+            for (int d = 0; d < 16; d++) dst[4 * d] = cache_result(o[d][2 * h] * inv[h], o[d][2 * h + 1] * inv[h]);
           }
         }
       } else {
@@ -394,8 +394,8 @@ __global__ void __launch_bounds__(CA_WARPS * 32u, 1) k_cache_attn(const CacheAtt
     const CacheSeq q = sh.seq[it.b];
     const uint32_t x = it.rb * 16u + r, i = x / p.group;
     const float inv = L > 0.0f ? 1.0f / L : L;
-    __half2* d = reinterpret_cast<__half2*>(p.O + (size_t)(q.r0 + i) * p.ldo + (it.hk * p.group + (x - i * p.group)) * 128u + 4u * lane);
-    d[0] = __floats2half2_rn(v.x * inv, v.y * inv); d[1] = __floats2half2_rn(v.z * inv, v.w * inv);
+    uint32_t* d = reinterpret_cast<uint32_t*>(p.O + (size_t)(q.r0 + i) * p.ldo + (it.hk * p.group + (x - i * p.group)) * 128u + 4u * lane);
+    d[0] = cache_result(v.x * inv, v.y * inv); d[1] = cache_result(v.z * inv, v.w * inv);
   };
   auto rows_of = [&](const CaEntry& e) { return min(16u, sh.seq[e.b].n * p.group - e.rb * 16u); };
   // one arrival at row r of an item of blocks c0 .. c1; true for the last one

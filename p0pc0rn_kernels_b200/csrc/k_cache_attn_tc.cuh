@@ -609,10 +609,7 @@ __global__ void __launch_bounds__(CTC_THREADS, 1) k_cache_attn_tc(const CacheTcP
         }
         uint32_t v[4][4];                                                 // four pieces of 8 columns
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const __half2 hp = __floats2half2_rn(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-          v[e >> 2][e & 3] = *reinterpret_cast<const uint32_t*>(&hp);
-        }
+        for (int e = 0; e < 16; e++) v[e >> 2][e & 3] = cache_result(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
         if (!vec) {
           if (at_o >= 0) {
 #pragma unroll
@@ -696,8 +693,8 @@ __global__ void __launch_bounds__(256) k_cache_merge(const CacheMergeP p) {
     if (!live(r)) continue;
     const uint32_t x = r & 127u, q = (r >> 7) * p.qpt + x / p.group, h = d.hk * p.group + x % p.group;
     const float4 v = *reinterpret_cast<const float4*>(&tile[r & 31u][lane * 4u]);
-    __half2* o = reinterpret_cast<__half2*>(p.O + (size_t)(d.row0 + q) * p.ldo + h * 128u + 4u * lane);
-    o[0] = __floats2half2_rn(v.x, v.y); o[1] = __floats2half2_rn(v.z, v.w);
+    uint32_t* o = reinterpret_cast<uint32_t*>(p.O + (size_t)(d.row0 + q) * p.ldo + h * 128u + 4u * lane);
+    o[0] = cache_result(v.x, v.y); o[1] = cache_result(v.z, v.w);
   }
 }
 

@@ -903,3 +903,39 @@ def test_rope_heads_and_sequences(gpu, c, inplace):
             assert np.array_equal(got[h][:, rot:], x[h][:, rot:])
     finally:
         for t in (xb, yb, lb, rb): gpu.free(t)
+
+
+@pytest.mark.parametrize("kernel", ["split", "tmem"])
+def test_attention_over_the_largest_values_stays_finite(gpu, kernel):
+    """values of the largest fp16 of either sign (infinities among them, which are stored so): their means are no infinities"""
+    import p0pc0rn_kernels_b200 as P
+    for L, news in ((64, (3, 40)), (40, (3, 40)), (230, (3, 100)), (20000, (3, 70))):
+        cache = Cache(P, gpu, 2, 1, -(-L // PAGE))
+        rng = np.random.default_rng(L)
+        k = rng.normal(0, 1, (2, L, 128)).astype(np.float16)
+        v = np.full((2, L, 128), 65504, np.float16); v[:, ::3, 5] = np.inf; v[1, :, 64:] = -65504; v[1, 1::7, 70] = -np.inf
+        try:
+            cache.write([L], [k], [v], rows=False)
+            for n in news:
+                out, q, offs = _attend(cache, [n], 4, kernel=kernel)
+                want = np.broadcast_to(np.repeat(_clean(v[:, 0]), 4, 0).astype(np.float64), out.shape)
+                # (codes of 127 times a scale rounded up by at most 2^-11, weights off by 2^-11 + 1e-4, the result's rounding; never beyond the largest fp16)
+                assert np.isfinite(out).all() and np.abs(out.astype(np.float64) - want).max() <= 65504 * (3 * 2.0 ** -11 + 1e-4)
+        finally:
+            cache.free()
+
+
+@pytest.mark.parametrize("kernel", [None, "split", "tmem"])
+def test_attention_of_empty_batches(gpu, kernel):
+    """no sequence has new tokens; and as many sequences as a call can have, most of them without any"""
+    import p0pc0rn_kernels_b200 as P
+    cache = Cache(P, gpu, 2, 1024, 2)
+    try:
+        cache.fill([70 if b % 100 == 7 or b == 1023 else 0 for b in range(1024)])
+        out, _, _ = _attend(cache, [0] * 1024, 4, extra=5, kernel=kernel)
+        assert out.shape[0] == 5                                                               # (and nothing was written: _attend looks)
+        _check(cache, [1 + b % 3 if cache.lens[b] else 0 for b in range(1024)], 4, extra=2, kernel=kernel)
+        _check(cache, [70 if cache.lens[b] else 0 for b in range(1024)], 4, kernel=kernel)
+        gpu.done()
+    finally:
+        cache.free()
