@@ -18,7 +18,7 @@
 // sequence, kv head and row block) that lies within one warp's share is finished there; otherwise partial results (maximum, sum, O)
 // are merged in the block, and across blocks by the warp that arrives last (a counter per row of an item that crosses blocks; it resets
 // it), in order: deterministic, one launch.
-// Bound: one pass over the visible codes (HBM).  32:8 heads, 64 sequences of up to 4096 tokens, 328 MB: 62 to 64 us = 5.2 TB/s, 0.79 of the measured copy (while
+// Bound: one pass over the visible codes (HBM).  32:8 heads, 64 sequences of up to 4096 tokens, 328 MB: 61 to 65 us = 5.0 to 5.4 TB/s, 0.77 to 0.82 of the measured copy (while
 // all warps stream, at its rate; the rest is the launch, the first pages' latency and the end: shares of whole pages of 2.3 us, 3 us to
 // merge).  One sequence of 32000, 66 MB: 20.0 us = 0.50 (three or four pages per warp).  One of 300: 7.2 us, all latency.  Tried and slower: K one more page
 // ahead in a third buffer (66 -> 70 us: V then comes late), asking the L2 for pages 1, 2 or 4 ahead (63 -> 70, 80, 92).

@@ -14,7 +14,7 @@
 // Roles: warp 0 keeps the list of work (items, and page by page what the others need to know), warp 1 multiplies, warp 2 loads queries, warps 4-7 convert,
 // warps 8-15 and 16-23 are the softmax of the two tiles, two threads per row.  The softmax threads take the registers that the others leave
 // (setmaxnreg; per scheduler 4 x 104 + 24 + 40 = the 6 x 80 of the launch; with 32 for each of the others the converting warps spilled: 249 against 246.5 us).
-// Bound: 2000 tokens over 6100 of 32:8 heads, 233 GFLOP: 233 us = 1000 TFLOP/s, 0.60 of the measured burst, under the power limit (1.6 to 1.7 GHz).  A pair of
+// Bound: 2000 tokens over 6100 of 32:8 heads, 233 GFLOP: 231 to 237 us = 980 to 1010 TFLOP/s, 0.59 to 0.61 of the measured burst, under the power limit (1.6 to 1.7 GHz).  A pair of
 // pages takes about 4200 cycles of a block: its multiplies alone 1900 (tensor pipe active 51 to 54 %), its traffic through shared memory 2500 (operands, codes
 // in, tiles out), the converting warps about 3500 (latency: a warp's 16 units of 32 bytes, waits and fences in a row), a softmax warp 1700.  Tried and slower: conversion
 // by the softmax warps between two tiles (308 us), K as fp16 subnormals with a row sum of q (255 against 260 then, but 147 against 141 for short
